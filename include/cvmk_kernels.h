@@ -463,6 +463,110 @@ CVMK_API int cvmk_non_max_suppression_static(const int32_t* x, const int32_t* va
 CVMK_API int cvmk_transpose_batched(const void* x, void* y, int32_t dtype, int64_t batch, int32_t rows,
                                     int32_t cols, int32_t clamp, int32_t lo, int32_t hi, cvmk_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * dense with a table as its activation, optionally gated by a second dense (the feed-forward block of a
+ * decoder layer), and a residual in the epilogue, in one launch:
+ *     a[r, u] = chain_w( sum_k x[r, k] * w[u, k] )
+ *     t[r, u] = table[ clamp(a, 0, table_len - 1) ]                 (cvm_lut, cpu/ops/ops.cc:947-956)
+ *     t[r, u] = t * chain_v( sum_k x[r, k] * v[u, k] )              where v is given
+ *     y[r, u] = chain_y( t )                                        stored as int8 (low byte) or int32
+ * Sums, products and sums with tensors are int32 and wrap, as those of dense (:34-75), broadcast_mul
+ * (cpu/ops/broadcast.cc:33-36) and elemwise_add do.
+ *   x : int8 [rows, K], rows x_pitch bytes apart       w, v : int8 [units, K], rows w_pitch bytes apart
+ *   y : [rows, units], rows y_pitch elements apart; nothing between or behind them is written
+ * Pitches of 0 mean packed rows.  x, w, v start on 16 bytes and their pitches are multiples of 16 (K itself
+ * need not be; what lies behind a row's K bytes is not looked at); y starts on an element.  1 <= K < 2^17,
+ * rows >= 0 (none: the launch does nothing), 1 <= units, table_len < 2^31.
+ * chain_w and chain_v may begin with ADD_C (the bias, `units` int32) and hold no other step with an operand;
+ * chain_y may hold one *_T step, whose tensor has y's shape and pitch.  No two tensors overlap, but a *_T
+ * operand may be y itself.
+ *
+ * cvmk_dense_lut_prepare() chooses the kernel and encodes the tensor maps into `plan` (host memory of the
+ * caller, 64-byte aligned; to be repeated if x, w or v move); it wants the device current that will run
+ * the launches.  cvmk_dense_lut_launch() only enqueues the kernel; launches of one plan may be on several
+ * streams at once where y is not read in between.  `status`: as in cvmk_conv_desc, or NULL.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  const int8_t* x;
+  const int8_t* w;
+  const int8_t* v;            /* NULL: not gated */
+  void* y;
+  int64_t x_pitch, w_pitch, y_pitch;
+  int32_t rows, units, K;
+  int32_t y_dtype;
+  const void* table;
+  int32_t table_len, table_dtype;
+  int32_t* status;
+  /* 1: w, v, the biases and the table are model parameters that no kernel ever writes: they may be read
+   * before the previous kernel of the stream has finished. */
+  int32_t params_static;
+  int32_t reserved;
+  cvmk_epilogue chain_w, chain_v, chain_y;
+} cvmk_dense_lut_desc;
+
+typedef struct __attribute__((aligned(64))) {
+  unsigned char tmap_x[128];
+  unsigned char tmap_w[128];
+  unsigned char tmap_v[128];
+  cvmk_dense_lut_desc d;
+  int32_t kernel;       /* 0 the weights are the 128-row operand, 1 pairs of CTAs and tiles of 256 rows */
+  int32_t grid, smem_bytes;
+  int32_t stages;       /* of the operand ring */
+  int32_t split;        /* CTAs of a cluster that share a tile's reduction */
+  int32_t row_tile;     /* rows of x a tile */
+  int32_t table_smem;   /* bytes of the table kept in shared memory, 0: read where it lies */
+  int32_t reserved[5];
+} cvmk_dense_lut_plan;
+
+/* 1 if the sizes, types and chains are taken; looks at no address. */
+CVMK_API int cvmk_dense_lut_supported(const cvmk_dense_lut_desc* d);
+CVMK_API int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_lut_plan* plan);
+CVMK_API int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * One element of every row drawn by its score, in whole numbers: what a language model answers with.
+ * No counterpart in the reference; weights are a table's entries, as in its quantised exponentials
+ * (cvm_lut).  For a row of int32 scores x[0 .. vocab), m their largest, i in 0 .. vocab - 1:
+ *     w[i] = table[ min( ((m - x[i]) * scale) >> 16, table_len - 1 ) ]        (unbounded whole numbers)
+ *     order: larger x first, equal ones by lower i
+ *   top_k : if >= 1, only the first top_k of the order stay
+ *   min_p : of those, the ones with w[i] * 2^30 >= min_p * table[0] stay
+ *   top_p : of those, with the sum W of their weights, stay the ones before which, in the order, lies a
+ *           sum of less than top_p * W / 2^30; the first with a positive weight stays in any case
+ *   mass  = the sum of the weights that are left;  t = floor(random * mass / 2^31)
+ *   token = the lowest i that is left whose weights up to and with i sum to more than t; if mass is 0,
+ *           the first of the order
+ * scale is the inverse temperature: table steps a unit of x, times 2^16; 0 gives every element table[0].
+ * The greedy choice is top_k = 1.  Negative table entries and scales count as 0, min_p and top_p are taken as
+ * within [0, 2^30], `random` by its low 31 bits.
+ *   logits : int32 [rows, vocab], rows pitch elements apart (0: packed)
+ *   scale, random : int32 [rows];  top_k, top_p, min_p : int32 [rows], or NULL: off for every row
+ *   token : int32 [rows];  weight (of the token), kept (how many positive weights are left) : int32 [rows]
+ *   or NULL;  mass : int64 [rows] or NULL
+ * 0 <= rows, 1 <= vocab <= CVMK_SAMPLE_MAX_VOCAB, table_len >= 1.  All pointers aligned to their elements.
+ * No scratch; launches may overlap where their results do not.  A token of -1 says that a bounded wait of
+ * the kernel ran out (the other results of that row are then not written).
+ * ---------------------------------------------------------------------------------------------- */
+#define CVMK_SAMPLE_MAX_VOCAB (384 * 1024)
+typedef struct {
+  const int32_t* logits;
+  int64_t pitch;
+  int32_t rows, vocab;
+  const int32_t* table;
+  int32_t table_len;
+  int32_t reserved;
+  const int32_t* scale;
+  const int32_t* top_k;
+  const int32_t* top_p;
+  const int32_t* min_p;
+  const int32_t* random;
+  int32_t* token;
+  int32_t* weight;
+  int64_t* mass;
+  int32_t* kept;
+} cvmk_sample_desc;
+CVMK_API int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream);
+
 /* Text of the last CUDA / argument error seen by a launcher on this thread. */
 CVMK_API const char* cvmk_last_error(void);
 
