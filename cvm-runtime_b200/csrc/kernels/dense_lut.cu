@@ -8,6 +8,10 @@
 // writes its partial sums (int32: exact in any order) to its shared memory and each finishes its share of the
 // units from all of them.
 //
+// dense_lut_pair_kernel: more rows.  Two CTAs of a cluster multiply a tile of 256 rows by 256 weight rows together
+// (tcgen05 cta_group::2; gated: 128 of w, loaded by the first CTA, and the same 128 of v, loaded by the second), walking
+// tiles with the requantisation of one beside the products of the next (two accumulators).
+//
 // Reproduces dense -> [chain] -> cvm_lut -> broadcast_mul -> [chain] of the reference's operators
 // (src/runtime/cpu/ops/ops.cc:34-75, :947-956, cpu/ops/broadcast.cc:33-36) bit for bit.
 #include <cuda.h>
@@ -27,7 +31,8 @@ constexpr int BLOCK_K = 128;     // bytes of K a ring stage
 constexpr int MAX_STAGES = 12;
 constexpr int W_BYTES = BLOCK_M * BLOCK_K;          // of a stage: 128 rows of weights
 constexpr int TABLE_SMEM_MAX = 16 * 1024;
-constexpr int SMEM_MAX = 226 * 1024;
+constexpr int SMEM_MAX = 224 * 1024;   // of a launch; a kernel's static part is less than the rest
+constexpr uint32_t FULL_MASK = 0xffffffffu;
 
 struct Params {
   void* y;
@@ -266,6 +271,247 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
 }
 
 // ---------------------------------------------------------------------------------------------
+// Pairs of CTAs
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::
+                   "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {   // of either CTA, an address of the cluster's window
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Both halves of a gated chunk with one wait (all the registers pass through it, so that none is read before).
+__device__ __forceinline__ void tmem_ld_two(uint32_t ta, uint32_t tb, int32_t (&a)[32], int32_t (&b)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(a[16]), "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]), "=r"(a[24]), "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]),
+        "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]), "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15]), "=r"(b[16]), "=r"(b[17]), "=r"(b[18]), "=r"(b[19]), "=r"(b[20]), "=r"(b[21]), "=r"(b[22]), "=r"(b[23]), "=r"(b[24]), "=r"(b[25]), "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31])
+      : "r"(ta), "r"(tb)
+      : "memory");
+}
+
+// 32 values of one row from or to memory that may begin and end anywhere: whole 16-byte words where `n` is 32 and the
+// address allows it.
+__device__ __forceinline__ void load_run(const void* base, int dtype, long long lin, int n, int32_t (&t)[32]) {
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(base) + lin * dtype;
+  if (n == 32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    if (dtype == CVMK_I8) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int4 raw = reinterpret_cast<const int4*>(at)[q];
+        const int w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t[q * 16 + k] = (int32_t)(int8_t)(w[k >> 2] >> ((k & 3) * 8));
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int4 raw = reinterpret_cast<const int4*>(at)[q];
+        t[4 * q] = raw.x; t[4 * q + 1] = raw.y; t[4 * q + 2] = raw.z; t[4 * q + 3] = raw.w;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    t[j] = j >= n ? 0 : (dtype == CVMK_I8 ? (int32_t) reinterpret_cast<const int8_t*>(at)[j] : reinterpret_cast<const int32_t*>(at)[j]);
+}
+__device__ __forceinline__ void store_run(void* base, int dtype, long long lin, int n, const int32_t (&t)[32]) {
+  uint8_t* at = reinterpret_cast<uint8_t*>(base) + lin * dtype;
+  if (n == 32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    if (dtype == CVMK_I8) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        reinterpret_cast<uint4*>(at)[q] = make_uint4(pack4(t[16 * q], t[16 * q + 1], t[16 * q + 2], t[16 * q + 3]), pack4(t[16 * q + 4], t[16 * q + 5], t[16 * q + 6], t[16 * q + 7]),
+                                                     pack4(t[16 * q + 8], t[16 * q + 9], t[16 * q + 10], t[16 * q + 11]), pack4(t[16 * q + 12], t[16 * q + 13], t[16 * q + 14], t[16 * q + 15]));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) reinterpret_cast<int4*>(at)[q] = make_int4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < n) {
+      if (dtype == CVMK_I8) reinterpret_cast<int8_t*>(at)[j] = (int8_t)t[j];
+      else reinterpret_cast<int32_t*>(at)[j] = t[j];
+    }
+}
+__device__ __forceinline__ void add_bias(const int32_t* bias_s, int32_t (&v)[32]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int4 b = reinterpret_cast<const int4*>(bias_s)[q];
+    v[4 * q] += b.x; v[4 * q + 1] += b.y; v[4 * q + 2] += b.z; v[4 * q + 3] += b.w;
+  }
+}
+
+constexpr int PAIR_STAGE = 2 * W_BYTES;   // a CTA's 128 rows of x and 128 rows of weights
+constexpr int PAIR_COLS = 256;            // of an accumulator
+constexpr int EPI_WARPS = THREADS / 32 - 2;
+
+__global__ void __launch_bounds__(THREADS, 1)
+dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bar_full[MAX_STAGES];       // of the first CTA: the bytes of both have landed
+  __shared__ uint64_t bar_empty[MAX_STAGES];
+  __shared__ uint64_t bar_acc_full[2];
+  __shared__ uint64_t bar_acc_empty[2];           // of the first CTA: the warps of both have read the accumulator
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ __align__(16) int32_t bias_s[EPI_WARPS][2][32];
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  const int rank = uniform((int)cluster_rank());
+  const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1, tiles = p.unit_tiles * p.row_tiles;
+  const int tile_units = p.gated ? 128 : 256;
+  uint8_t* const table_s = smem + p.stages * PAIR_STAGE;
+  const bool leader = elect_one();
+  touch_params(p);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&bar_full[s], 1);
+      mbar_init(&bar_empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&bar_acc_full[a], 1);
+      mbar_init(&bar_acc_empty[a], 2 * EPI_WARPS);
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(&tmem_slot, 2 * PAIR_COLS);   // before this CTA lets the next kernel start
+    pdl_trigger();
+  }
+  if (warp >= 2) {
+    if (!p.params_static) pdl_wait();
+    if (p.table_smem) copy_table(p, table_s, (int)threadIdx.x - 64, THREADS - 64);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // neither CTA signals the other's barriers or writes its TMEM before both have them
+  tc_fence_after();
+  const uint32_t tmem_base = (uint32_t)uniform((int)tmem_slot);
+  const int my_tiles = first < tiles ? (tiles - first + step - 1) / step : 0;
+  pdl_wait();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA
+    const uint32_t full0 = map_rank(smem_u32(&bar_full[0]), 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool live = leader;
+    for (int tile = first; live && tile < tiles; tile += step) {
+      const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
+      const int row0 = rt * 256 + rank * 128, unit0 = ut * tile_units + (p.gated ? 0 : rank * 128);
+      const CUtensorMap* const weights = p.gated && rank ? &tmap_v : &tmap_w;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait(&bar_empty[stage], phase ^ 1, &abort_flag, 1)) { live = false; break; }
+        if (rank == 0) mbar_expect_tx(&bar_full[stage], 2 * PAIR_STAGE);
+        const uint32_t dst = smem_u32(smem) + (uint32_t)(stage * PAIR_STAGE), bar = full0 + 8u * (uint32_t)stage;
+        load_2d_pair(dst, &tmap_x, bar, kb * BLOCK_K, row0);
+        load_2d_pair(dst + W_BYTES, weights, bar, kb * BLOCK_K, unit0);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA, of both CTAs by the first
+    if (rank == 0) {
+      const uint32_t idesc = umma_idesc_i8(256, 256);
+      const uint64_t desc0 = umma_desc(smem_u32(smem), BLOCK_K);
+      const uint32_t lo0 = (uint32_t)desc0, hi = (uint32_t)(desc0 >> 32);
+      int stage = 0;
+      uint32_t phase = 0;
+      int refills = my_tiles * p.kblocks - p.stages;   // stages, this one included, that are filled again: nobody waits for the others' commits
+      bool live = true;
+      for (int i = 0; live && i < my_tiles; ++i) {
+        const int acc = i & 1;
+        if (!mbar_wait(&bar_acc_empty[acc], (uint32_t)((i >> 1) & 1) ^ 1u, &abort_flag, 2)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * PAIR_COLS);
+        for (int kb = 0; kb < p.kblocks; ++kb, --refills) {
+          if (!mbar_wait(&bar_full[stage], phase, &abort_flag, 3)) { live = false; break; }
+          tc_fence_after();
+          const uint32_t al = lo0 + (uint32_t)(stage * (PAIR_STAGE >> 4));
+          if (leader) {
+            mma_i8_k<4, 2>(d_tmem, al, hi, al + (W_BYTES >> 4), hi, idesc, (uint32_t)kb);
+            mma_commit_pair_if(refills > 0, &bar_empty[stage]);
+          }
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+        if (live && leader) mma_commit<2>(&bar_acc_full[acc]);
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- epilogue: a row a lane, half of the columns a group of four warps
+    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0, columns = tile_units / 2;
+    const uint32_t acc_empty0 = map_rank(smem_u32(&bar_acc_empty[0]), 0);
+    int32_t(&bias)[2][32] = bias_s[warp - 2];
+    int i = 0;
+    for (int tile = first; tile < tiles; tile += step, ++i) {
+      const int acc = i & 1;
+      const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
+      const int row = rt * 256 + rank * 128 + quarter * 32 + lane, unit0 = ut * tile_units + half * columns;
+      const uint32_t t0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * PAIR_COLS + half * columns);
+      if (!__all_sync(FULL_MASK, mbar_wait(&bar_acc_full[acc], (uint32_t)((i >> 1) & 1), &abort_flag, 4))) break;
+      tc_fence_after();
+      for (int c = 0; c < columns; c += 32) {
+        const int unit = unit0 + c, n = min(32, p.units - unit);
+        const bool mine = unit + lane < p.units;
+        __syncwarp();   // (the last chunk's biases have been read)
+        bias[0][lane] = p.bias_w && mine ? p.bias_w[unit + lane] : 0;
+        bias[1][lane] = p.bias_v && mine ? p.bias_v[unit + lane] : 0;
+        int32_t a[32], b[32];
+        if (p.gated) {
+          tmem_ld_two(t0 + (uint32_t)c, t0 + 128u + (uint32_t)c, a, b);
+        } else {
+          tmem_ld32(t0 + (uint32_t)c, a);
+        }
+        if (c + 32 >= columns) {   // the accumulator has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(acc_empty0 + 8u * (uint32_t)acc);
+        }
+        __syncwarp();
+        if (n <= 0 || row >= p.rows) continue;
+        const long long lin = (long long)row * p.y_pitch + unit;
+        add_bias(bias[0], a);
+        activate<32>(p, table_s, a);
+        if (p.gated) {
+          add_bias(bias[1], b);
+          apply_chain<32>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+        }
+        if (p.res) load_run(p.res, p.res_dtype, lin, n, b);
+        apply_chain<32, true>(p.cy, a, 0, 0, 0, b, p.res_step);
+        store_run(p.y, p.y_dtype, lin, n, a);
+      }
+    }
+    __syncwarp();
+  }
+  if (abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies in flight land before shared memory is released
+    if (lane == 0 && p.status) atomicOr(p.status, 0x400 | abort_flag);
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync();   // every accumulator has been read, and nothing is sent to either CTA any more
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem_base, 2 * PAIR_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -294,6 +540,15 @@ CUresult encode_matrix(CUtensorMap* map, const void* base, int64_t rows, int64_t
   cuuint32_t box[2] = {(cuuint32_t)BLOCK_K, (cuuint32_t)box_rows}, estr[2] = {1, 1};
   return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+int encode_operands(cvmk_dense_lut_plan* plan, int x_rows, int w_rows) {
+  const cvmk_dense_lut_desc& d = plan->d;
+  CUresult r = encode_matrix((CUtensorMap*)plan->tmap_x, d.x, d.rows, d.K, d.x_pitch, x_rows, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+  if (r == CUDA_SUCCESS) r = encode_matrix((CUtensorMap*)plan->tmap_w, d.w, d.units, d.K, d.w_pitch, w_rows, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (r == CUDA_SUCCESS) r = encode_matrix((CUtensorMap*)plan->tmap_v, d.v ? d.v : d.w, d.units, d.K, d.w_pitch, w_rows, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (r != CUDA_SUCCESS) { set_error("dense_lut_prepare: tensor map rejected (CUresult %d)", (int)r); return CVMK_ERR_CUDA; }
+  return CVMK_OK;
 }
 
 bool is_tensor_step(const cvmk_ep_step& s) { return s.op == CVMK_EP_ADD_T || s.op == CVMK_EP_SUB_T || s.op == CVMK_EP_RSUB_T; }
@@ -361,6 +616,17 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   const int64_t table_bytes = (int64_t)p.table_len * p.table_dtype;
   plan->table_smem = table_bytes <= TABLE_SMEM_MAX ? (int)table_bytes : 0;
   const int table_room = (plan->table_smem + 15) & ~15;
+  plan->kernel = p.rows > 256 ? 1 : 0;
+  if (plan->kernel == 1) {
+    plan->row_tile = 256;
+    plan->split = 1;
+    plan->stages = 6;
+    // (no other kernel's CTAs fit beside a pair: they could hold TMEM columns and wait for its end)
+    plan->smem_bytes = std::max(1024 + plan->stages * PAIR_STAGE + table_room, 206 * 1024);
+    const int64_t tiles = (int64_t)((p.rows + 255) / 256) * ((p.units + (p.v ? 127 : 255)) / (p.v ? 128 : 256));
+    plan->grid = 2 * (int)std::min<int64_t>(tiles, sms / 2);
+    return encode_operands(plan, 128, 128);
+  }
   const int row_tiles = (p.rows + 255) / 256;
   plan->row_tile = ((p.rows + row_tiles - 1) / row_tiles + 15) & ~15;
   const int64_t unit_tiles = (p.units + tile_units - 1) / tile_units, tiles = unit_tiles * row_tiles;
@@ -374,11 +640,7 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   plan->smem_bytes = std::max(smem_of(plan->stages), 26 * 1024);
   plan->grid = (int)(tiles * plan->split);
 
-  CUresult r = encode_matrix((CUtensorMap*)plan->tmap_x, p.x, p.rows, p.K, p.x_pitch, plan->row_tile, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
-  if (r == CUDA_SUCCESS) r = encode_matrix((CUtensorMap*)plan->tmap_w, p.w, p.units, p.K, p.w_pitch, 64, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-  if (r == CUDA_SUCCESS) r = encode_matrix((CUtensorMap*)plan->tmap_v, p.v ? p.v : p.w, p.units, p.K, p.w_pitch, 64, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
-  if (r != CUDA_SUCCESS) { set_error("dense_lut_prepare: tensor map rejected (CUresult %d)", (int)r); return CVMK_ERR_CUDA; }
-  return CVMK_OK;
+  return encode_operands(plan, plan->row_tile, 64);
 }
 
 extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_stream_t stream) {
@@ -392,7 +654,8 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   p.kblocks = (d.K + BLOCK_K - 1) / BLOCK_K;
   p.gated = d.v != nullptr;
   p.params_static = d.params_static;
-  const int tile_units = p.gated ? 64 : 128;
+  const bool pair = plan->kernel == 1;
+  const int tile_units = (p.gated ? 64 : 128) * (pair ? 2 : 1);
   p.unit_tiles = (d.units + tile_units - 1) / tile_units;
   p.row_tile = plan->row_tile;
   p.row_tiles = (d.rows + p.row_tile - 1) / p.row_tile;
@@ -416,9 +679,11 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_of_device[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(dense_lut_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(dense_lut_small_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (check_cuda(e, "cudaFuncSetAttribute(dense_lut_small_kernel)")) return CVMK_ERR_CUDA;
+    for (auto k : {dense_lut_small_kernel, dense_lut_pair_kernel}) {
+      cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+      if (check_cuda(e, "cudaFuncSetAttribute(dense_lut)")) return CVMK_ERR_CUDA;
+    }
     attr_of_device[dev & 63] = true;
   }
   CUtensorMap tx, tw, tv;
@@ -434,9 +699,9 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)plan->split;
+  attr[1].val.clusterDim.x = pair ? 2u : (unsigned)plan->split;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = plan->split > 1 ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_small_kernel, tx, tw, tv, p), "dense_lut_small_kernel launch");
+  cfg.numAttrs = pair || plan->split > 1 ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, pair ? dense_lut_pair_kernel : dense_lut_small_kernel, tx, tw, tv, p), "dense_lut launch");
 }
