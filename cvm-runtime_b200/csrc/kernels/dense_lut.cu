@@ -34,6 +34,13 @@ constexpr int TABLE_SMEM_MAX = 16 * 1024;
 constexpr int SMEM_MAX = 224 * 1024;   // of a launch; a kernel's static part is less than the rest
 constexpr uint32_t FULL_MASK = 0xffffffffu;
 
+// A chain of a rounding shift with clamps, and for the one in front of a table the sum with a constant and the table's
+// bounds, in three instructions: max(min(sum + (bias + add), hi), lo) >> shift.  The clamps come before the shift, which
+// is monotone; nothing overflows while |bias + add| <= room, which the kernel looks at 32 biases at a time.
+struct Requant {
+  int on, add, lo, hi, shift, room;
+};
+
 struct Params {
   void* y;
   long long y_pitch;
@@ -48,7 +55,10 @@ struct Params {
   const void* res;                 // operand of chain_y's *_T step, or nullptr
   int res_dtype, res_step;
   int* status;
+  Requant qw, qv;
+  int table_s_dtype;               // of the copy in shared memory
   DevChain cw, cv, cy;
+  DevChain ct;                     // ungated: steps of chain_y that the copy of the table has gone through already
 };
 
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
@@ -70,23 +80,42 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int32_t (&v)[16]) {
       : "memory");
 }
 
-// The chain in front of the table, and the table: `table_s` is its copy in shared memory, or nullptr.
+// The table's entries at a[j], which lie within it.  `table_s` is its copy in shared memory (table_smem).
+template <int V>
+__device__ __forceinline__ void look_up(const Params& p, const uint8_t* table_s, int32_t (&a)[V]) {
+  if (p.table_smem) {
+    if (p.table_s_dtype == CVMK_I8) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] = reinterpret_cast<const int8_t*>(table_s)[a[j]];
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] = reinterpret_cast<const int32_t*>(table_s)[a[j]];
+    }
+  } else if (p.table_dtype == CVMK_I8) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] = reinterpret_cast<const int8_t*>(p.table)[a[j]];
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] = reinterpret_cast<const int32_t*>(p.table)[a[j]];
+  }
+}
+// The chain in front of the table, and the table.
 template <int V>
 __device__ __forceinline__ void activate(const Params& p, const uint8_t* table_s, int32_t (&a)[V]) {
   apply_chain<V>(p.cw, a, 0, 0, 0, nullptr, -1, p.first_w);
   const int last = p.table_len - 1;
-  const void* t = p.table_smem ? (const void*)table_s : p.table;
-  if (p.table_dtype == CVMK_I8) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) a[j] = reinterpret_cast<const int8_t*>(t)[min(max(a[j], 0), last)];
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) a[j] = reinterpret_cast<const int32_t*>(t)[min(max(a[j], 0), last)];
-  }
+  for (int j = 0; j < V; ++j) a[j] = min(max(a[j], 0), last);
+  look_up<V>(p, table_s, a);
 }
 
 __device__ __forceinline__ void copy_table(const Params& p, uint8_t* table_s, int t, int threads) {
-  for (int i = t; i < p.table_len * p.table_dtype; i += threads) table_s[i] = reinterpret_cast<const uint8_t*>(p.table)[i];
+  for (int i = t; i < p.table_len; i += threads) {
+    int32_t v[1] = {p.table_dtype == CVMK_I8 ? (int32_t) reinterpret_cast<const int8_t*>(p.table)[i] : reinterpret_cast<const int32_t*>(p.table)[i]};
+    apply_chain<1>(p.ct, v, 0, 0, 0);
+    if (p.table_s_dtype == CVMK_I8) reinterpret_cast<int8_t*>(table_s)[i] = (int8_t)v[0];
+    else reinterpret_cast<int32_t*>(table_s)[i] = v[0];
+  }
 }
 
 // bytes of one row of partial sums: 16 more than the sums, so that eight rows of one column lie in different banks
@@ -347,6 +376,22 @@ __device__ __forceinline__ void add_bias(const int32_t* bias_s, int32_t (&v)[32]
   }
 }
 
+__device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) {
+  const long long b = (long long)bias + q.add;
+  return b <= q.room && b >= -(long long)q.room;
+}
+__device__ __forceinline__ void requant(const int32_t* bias_s, const Requant& q, int32_t (&v)[32]) {   // biases with q.add in them
+  const int hi = q.hi, lo = q.lo, sh = q.shift;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int4 b = reinterpret_cast<const int4*>(bias_s)[i];
+    v[4 * i] = max(__viaddmin_s32(v[4 * i], b.x, hi), lo) >> sh;
+    v[4 * i + 1] = max(__viaddmin_s32(v[4 * i + 1], b.y, hi), lo) >> sh;
+    v[4 * i + 2] = max(__viaddmin_s32(v[4 * i + 2], b.z, hi), lo) >> sh;
+    v[4 * i + 3] = max(__viaddmin_s32(v[4 * i + 3], b.w, hi), lo) >> sh;
+  }
+}
+
 constexpr int PAIR_STAGE = 2 * W_BYTES;   // a CTA's 128 rows of x and 128 rows of weights
 constexpr int PAIR_COLS = 256;            // of an accumulator
 constexpr int EPI_WARPS = THREADS / 32 - 2;
@@ -466,9 +511,11 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
       for (int c = 0; c < columns; c += 32) {
         const int unit = unit0 + c, n = min(32, p.units - unit);
         const bool mine = unit + lane < p.units;
+        const int32_t bw = p.bias_w && mine ? p.bias_w[unit + lane] : 0, bv = p.bias_v && mine ? p.bias_v[unit + lane] : 0;
+        const bool fast_w = p.qw.on && __all_sync(FULL_MASK, in_room(bw, p.qw)), fast_v = p.qv.on && __all_sync(FULL_MASK, in_room(bv, p.qv));
         __syncwarp();   // (the last chunk's biases have been read)
-        bias[0][lane] = p.bias_w && mine ? p.bias_w[unit + lane] : 0;
-        bias[1][lane] = p.bias_v && mine ? p.bias_v[unit + lane] : 0;
+        bias[0][lane] = fast_w ? bw + p.qw.add : bw;
+        bias[1][lane] = fast_v ? bv + p.qv.add : bv;
         int32_t a[32], b[32];
         if (p.gated) {
           tmem_ld_two(t0 + (uint32_t)c, t0 + 128u + (uint32_t)c, a, b);
@@ -483,11 +530,20 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         __syncwarp();
         if (n <= 0 || row >= p.rows) continue;
         const long long lin = (long long)row * p.y_pitch + unit;
-        add_bias(bias[0], a);
-        activate<32>(p, table_s, a);
+        if (fast_w) {
+          requant(bias[0], p.qw, a);
+          look_up<32>(p, table_s, a);
+        } else {
+          add_bias(bias[0], a);
+          activate<32>(p, table_s, a);
+        }
         if (p.gated) {
-          add_bias(bias[1], b);
-          apply_chain<32>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+          if (fast_v) {
+            requant(bias[1], p.qv, b);
+          } else {
+            add_bias(bias[1], b);
+            apply_chain<32>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+          }
 #pragma unroll
           for (int j = 0; j < 32; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
         }
@@ -542,6 +598,29 @@ CUresult encode_matrix(CUtensorMap* map, const void* base, int64_t rows, int64_t
                    CU_TENSOR_MAP_SWIZZLE_128B, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
+// The three-instruction form of a lowered chain from step `first` on, in front of a table of `len` entries or not (0).
+Requant requant_of(const DevChain& c, int first, int len, int K) {
+  Requant q = {0, 0, 0, 0, 0, 0};
+  const int left = c.n - first;
+  if (left < 1 || left > (len ? 2 : 1) || c.s[first].op != K_RS_CLAMP || (left == 2 && c.s[first + 1].op != K_ADD_S)) return q;
+  const DevStep& rs = c.s[first];
+  const int64_t moved = (int64_t)(left == 2 ? c.s[first + 1].a : 0) * ((int64_t)1 << rs.d), add = rs.c + moved;
+  int64_t lo = rs.a + add, hi = rs.b + add;
+  if (len) {
+    lo = std::max<int64_t>(lo, 0);
+    hi = std::min<int64_t>(hi, ((int64_t)len << rs.d) - 1);
+  }
+  const int64_t room = (int64_t)INT32_MAX - ((int64_t)K << 14);
+  if (lo > hi || lo < INT32_MIN || hi > INT32_MAX || add < INT32_MIN || add > INT32_MAX || room < 0) return q;
+  return {1, (int)add, (int)lo, (int)hi, rs.d, (int)room};
+}
+
+// Values that a step leaves within 8 bits, whatever it is given.
+bool to_int8(const DevStep& s) {
+  if (s.op == K_CLIP) return s.a >= -128 && s.b <= 127;
+  return s.op == K_RS_CLAMP && (((int64_t)s.a + s.c) >> s.d) >= -128 && (((int64_t)s.b + s.c) >> s.d) <= 127;
+}
+
 int encode_operands(cvmk_dense_lut_plan* plan, int x_rows, int w_rows) {
   const cvmk_dense_lut_desc& d = plan->d;
   CUresult r = encode_matrix((CUtensorMap*)plan->tmap_x, d.x, d.rows, d.K, d.x_pitch, x_rows, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
@@ -552,6 +631,7 @@ int encode_operands(cvmk_dense_lut_plan* plan, int x_rows, int w_rows) {
 }
 
 bool is_tensor_step(const cvmk_ep_step& s) { return s.op == CVMK_EP_ADD_T || s.op == CVMK_EP_SUB_T || s.op == CVMK_EP_RSUB_T; }
+bool is_tensor_op(int op) { return op == K_ADD_T || op == K_SUB_T || op == K_RSUB_T; }
 bool is_type(int t) { return t == CVMK_I8 || t == CVMK_I32; }
 
 const char* refusal(const cvmk_dense_lut_desc& d) {
@@ -669,9 +749,23 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   if (lower_chain(d.chain_w, &p.cw) || lower_chain(d.chain_v, &p.cv) || lower_chain(d.chain_y, &p.cy)) return CVMK_ERR_ARG;
   if (p.cw.n && p.cw.s[0].op == K_ADD_C) { p.bias_w = (const int32_t*)p.cw.s[0].ptr; p.first_w = 1; }
   if (p.cv.n && p.cv.s[0].op == K_ADD_C) { p.bias_v = (const int32_t*)p.cv.s[0].ptr; p.first_v = 1; }
+  p.qw = requant_of(p.cw, p.first_w, d.table_len, d.K);
+  p.qv = requant_of(p.cv, p.first_v, 0, d.K);
+  // Ungated, the first steps of chain_y are functions of a table entry: the copy of the table goes through them.
+  p.table_s_dtype = d.table_dtype;
+  if (!p.gated && p.table_smem) {
+    while (p.ct.n < p.cy.n && !is_tensor_op(p.cy.s[p.ct.n].op)) { p.ct.s[p.ct.n] = p.cy.s[p.ct.n]; ++p.ct.n; }
+    if (p.ct.n) p.table_s_dtype = to_int8(p.ct.s[p.ct.n - 1]) ? CVMK_I8 : CVMK_I32;
+    if (p.table_s_dtype * (int64_t)d.table_len > p.table_smem) {   // (wider than the room the plan has for it)
+      p.ct.n = 0;
+      p.table_s_dtype = d.table_dtype;
+    }
+    for (int i = p.ct.n; i < p.cy.n; ++i) p.cy.s[i - p.ct.n] = p.cy.s[i];
+    p.cy.n -= p.ct.n;
+  }
   p.res_step = -1;
   for (int i = 0; i < p.cy.n; ++i)
-    if (p.cy.s[i].op == K_ADD_T || p.cy.s[i].op == K_SUB_T || p.cy.s[i].op == K_RSUB_T) {
+    if (is_tensor_op(p.cy.s[i].op)) {
       p.res = p.cy.s[i].ptr; p.res_dtype = p.cy.s[i].dt; p.res_step = i;
     }
 
