@@ -31,7 +31,7 @@ constexpr int BLOCK_K = 128;     // bytes of K a ring stage
 constexpr int MAX_STAGES = 12;
 constexpr int W_BYTES = BLOCK_M * BLOCK_K;          // of a stage: 128 rows of weights
 constexpr int TABLE_SMEM_MAX = 16 * 1024;
-constexpr int SMEM_MAX = 224 * 1024;   // of a launch; a kernel's static part is less than the rest
+constexpr int SMEM_MAX = 222 * 1024;   // of a launch; a kernel's static part is less than the rest
 constexpr uint32_t FULL_MASK = 0xffffffffu;
 
 // A chain of a rounding shift with clamps, and for the one in front of a table the sum with a constant and the table's
@@ -309,68 +309,56 @@ __device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* ma
 __device__ __forceinline__ void arrive_at(uint32_t bar) {   // of either CTA, an address of the cluster's window
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Both halves of a gated chunk with one wait (all the registers pass through it, so that none is read before).
-__device__ __forceinline__ void tmem_ld_two(uint32_t ta, uint32_t tb, int32_t (&a)[32], int32_t (&b)[32]) {
+// Both sums of a gated chunk with one wait.
+__device__ __forceinline__ void tmem_ld_two(uint32_t ta, uint32_t tb, int32_t (&a)[16], int32_t (&b)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(a[16]), "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]), "=r"(a[24]), "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]),
-        "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]), "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15]), "=r"(b[16]), "=r"(b[17]), "=r"(b[18]), "=r"(b[19]), "=r"(b[20]), "=r"(b[21]), "=r"(b[22]), "=r"(b[23]), "=r"(b[24]), "=r"(b[25]), "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31])
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]),
+        "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]), "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15])
       : "r"(ta), "r"(tb)
       : "memory");
 }
 
-// 32 values of one row from or to memory that may begin and end anywhere: whole 16-byte words where `n` is 32 and the
-// address allows it.
-__device__ __forceinline__ void load_run(const void* base, int dtype, long long lin, int n, int32_t (&t)[32]) {
+// 16 values of one row from or to memory that may begin and end anywhere: whole 16-byte words where all `n` = 16 are there
+// and the address allows it.
+__device__ __forceinline__ void load_run(const void* base, int dtype, long long lin, int n, int32_t (&t)[16]) {
   const uint8_t* at = reinterpret_cast<const uint8_t*>(base) + lin * dtype;
-  if (n == 32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-    if (dtype == CVMK_I8) {
+  if (dtype == CVMK_I32 && n == 16 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int4 raw = reinterpret_cast<const int4*>(at)[q];
-        const int w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int k = 0; k < 16; ++k) t[q * 16 + k] = (int32_t)(int8_t)(w[k >> 2] >> ((k & 3) * 8));
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int4 raw = reinterpret_cast<const int4*>(at)[q];
-        t[4 * q] = raw.x; t[4 * q + 1] = raw.y; t[4 * q + 2] = raw.z; t[4 * q + 3] = raw.w;
-      }
+    for (int q = 0; q < 4; ++q) {
+      const int4 raw = reinterpret_cast<const int4*>(at)[q];
+      t[4 * q] = raw.x; t[4 * q + 1] = raw.y; t[4 * q + 2] = raw.z; t[4 * q + 3] = raw.w;
     }
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
+  for (int j = 0; j < 16; ++j)
     t[j] = j >= n ? 0 : (dtype == CVMK_I8 ? (int32_t) reinterpret_cast<const int8_t*>(at)[j] : reinterpret_cast<const int32_t*>(at)[j]);
 }
-__device__ __forceinline__ void store_run(void* base, int dtype, long long lin, int n, const int32_t (&t)[32]) {
+__device__ __forceinline__ void store_run(void* base, int dtype, long long lin, int n, const int32_t (&t)[16]) {
   uint8_t* at = reinterpret_cast<uint8_t*>(base) + lin * dtype;
-  if (n == 32 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+  if (n == 16 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
     if (dtype == CVMK_I8) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        reinterpret_cast<uint4*>(at)[q] = make_uint4(pack4(t[16 * q], t[16 * q + 1], t[16 * q + 2], t[16 * q + 3]), pack4(t[16 * q + 4], t[16 * q + 5], t[16 * q + 6], t[16 * q + 7]),
-                                                     pack4(t[16 * q + 8], t[16 * q + 9], t[16 * q + 10], t[16 * q + 11]), pack4(t[16 * q + 12], t[16 * q + 13], t[16 * q + 14], t[16 * q + 15]));
+      *reinterpret_cast<uint4*>(at) = make_uint4(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]), pack4(t[8], t[9], t[10], t[11]),
+                                                 pack4(t[12], t[13], t[14], t[15]));
     } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) reinterpret_cast<int4*>(at)[q] = make_int4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
+      for (int q = 0; q < 4; ++q) reinterpret_cast<int4*>(at)[q] = make_int4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
     }
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
+  for (int j = 0; j < 16; ++j)
     if (j < n) {
       if (dtype == CVMK_I8) reinterpret_cast<int8_t*>(at)[j] = (int8_t)t[j];
       else reinterpret_cast<int32_t*>(at)[j] = t[j];
     }
 }
-__device__ __forceinline__ void add_bias(const int32_t* bias_s, int32_t (&v)[32]) {
+__device__ __forceinline__ void add_bias(const int32_t* bias_s, int32_t (&v)[16]) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
+  for (int q = 0; q < 4; ++q) {
     const int4 b = reinterpret_cast<const int4*>(bias_s)[q];
     v[4 * q] += b.x; v[4 * q + 1] += b.y; v[4 * q + 2] += b.z; v[4 * q + 3] += b.w;
   }
@@ -380,10 +368,10 @@ __device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) {
   const long long b = (long long)bias + q.add;
   return b <= q.room && b >= -(long long)q.room;
 }
-__device__ __forceinline__ void requant(const int32_t* bias_s, const Requant& q, int32_t (&v)[32]) {   // biases with q.add in them
+__device__ __forceinline__ void requant(const int32_t* bias_s, const Requant& q, int32_t (&v)[16]) {   // biases with q.add in them
   const int hi = q.hi, lo = q.lo, sh = q.shift;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const int4 b = reinterpret_cast<const int4*>(bias_s)[i];
     v[4 * i] = max(__viaddmin_s32(v[4 * i], b.x, hi), lo) >> sh;
     v[4 * i + 1] = max(__viaddmin_s32(v[4 * i + 1], b.y, hi), lo) >> sh;
@@ -394,9 +382,10 @@ __device__ __forceinline__ void requant(const int32_t* bias_s, const Requant& q,
 
 constexpr int PAIR_STAGE = 2 * W_BYTES;   // a CTA's 128 rows of x and 128 rows of weights
 constexpr int PAIR_COLS = 256;            // of an accumulator
-constexpr int EPI_WARPS = THREADS / 32 - 2;
+constexpr int PAIR_THREADS = 576;         // warp 0: TMA, warp 1: MMA + TMEM, warps 2..17: epilogue
+constexpr int EPI_WARPS = PAIR_THREADS / 32 - 2;
 
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
 dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -406,7 +395,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   __shared__ uint64_t bar_acc_empty[2];           // of the first CTA: the warps of both have read the accumulator
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ __align__(16) int32_t bias_s[EPI_WARPS][2][32];
+  __shared__ __align__(16) int32_t bias_s[EPI_WARPS][64];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
@@ -435,7 +424,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   }
   if (warp >= 2) {
     if (!p.params_static) pdl_wait();
-    if (p.table_smem) copy_table(p, table_s, (int)threadIdx.x - 64, THREADS - 64);
+    if (p.table_smem) copy_table(p, table_s, (int)threadIdx.x - 64, PAIR_THREADS - 64);
   }
   tc_fence_before();
   __syncthreads();
@@ -496,60 +485,78 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     }
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- epilogue: a row a lane, half of the columns a group of four warps
-    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0, columns = tile_units / 2;
+    // ---------------------------------------------------------------- epilogue: a row a lane, a quarter of the columns a group of four warps
+    const int quarter = warp & 3, group = (warp - 2) >> 2, columns = tile_units / 4;   // 32 units, ungated 64
     const uint32_t acc_empty0 = map_rank(smem_u32(&bar_acc_empty[0]), 0);
-    int32_t(&bias)[2][32] = bias_s[warp - 2];
+    int32_t* const bias = bias_s[warp - 2];   // of w's columns, gated: 32 of w's and 32 of v's
+    const int32_t* const bias2 = p.gated ? p.bias_v : p.bias_w;
     int i = 0;
     for (int tile = first; tile < tiles; tile += step, ++i) {
       const int acc = i & 1;
       const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
-      const int row = rt * 256 + rank * 128 + quarter * 32 + lane, unit0 = ut * tile_units + half * columns;
-      const uint32_t t0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * PAIR_COLS + half * columns);
+      const int row = rt * 256 + rank * 128 + quarter * 32 + lane, unit0 = ut * tile_units + group * columns;
+      const uint32_t t0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * PAIR_COLS + group * columns);
+      // what the tile needs beside the sums travels while the products are computed: the biases, and an int8 residual
+      const int u1 = unit0 + lane, u2 = p.gated ? u1 : u1 + 32;
+      const int32_t b1 = p.bias_w && u1 < p.units ? p.bias_w[u1] : 0, b2 = bias2 && u2 < p.units ? bias2[u2] : 0;
+      uint4 res[4];
+      const int8_t* res_row = reinterpret_cast<const int8_t*>(p.res) + (long long)row * p.y_pitch + unit0;
+      const bool res_here = p.res && p.res_dtype == CVMK_I8 && row < p.rows && (reinterpret_cast<uintptr_t>(res_row) & 15) == 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (res_here && 16 * q < columns && unit0 + 16 * q + 16 <= p.units) res[q] = reinterpret_cast<const uint4*>(res_row)[q];
+      const Requant& q2 = p.gated ? p.qv : p.qw;
+      bool fast1 = __all_sync(FULL_MASK, in_room(b1, p.qw)) && p.qw.on, fast2 = __all_sync(FULL_MASK, in_room(b2, q2)) && q2.on;
+      if (!p.gated) fast1 = fast2 = fast1 && fast2;
+      __syncwarp();   // (the last tile's biases have been read)
+      bias[lane] = fast1 ? b1 + p.qw.add : b1;
+      bias[lane + 32] = fast2 ? b2 + q2.add : b2;
+      __syncwarp();
       if (!__all_sync(FULL_MASK, mbar_wait(&bar_acc_full[acc], (uint32_t)((i >> 1) & 1), &abort_flag, 4))) break;
       tc_fence_after();
-      for (int c = 0; c < columns; c += 32) {
-        const int unit = unit0 + c, n = min(32, p.units - unit);
-        const bool mine = unit + lane < p.units;
-        const int32_t bw = p.bias_w && mine ? p.bias_w[unit + lane] : 0, bv = p.bias_v && mine ? p.bias_v[unit + lane] : 0;
-        const bool fast_w = p.qw.on && __all_sync(FULL_MASK, in_room(bw, p.qw)), fast_v = p.qv.on && __all_sync(FULL_MASK, in_room(bv, p.qv));
-        __syncwarp();   // (the last chunk's biases have been read)
-        bias[0][lane] = fast_w ? bw + p.qw.add : bw;
-        bias[1][lane] = fast_v ? bv + p.qv.add : bv;
-        int32_t a[32], b[32];
-        if (p.gated) {
-          tmem_ld_two(t0 + (uint32_t)c, t0 + 128u + (uint32_t)c, a, b);
-        } else {
-          tmem_ld32(t0 + (uint32_t)c, a);
-        }
-        if (c + 32 >= columns) {   // the accumulator has been read
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 16 * q;
+        if (c >= columns) break;
+        const int unit = unit0 + c, n = min(16, p.units - unit);
+        int32_t a[16], b[16];
+        if (p.gated) tmem_ld_two(t0 + (uint32_t)c, t0 + 128u + (uint32_t)c, a, b);
+        else tmem_ld16(t0 + (uint32_t)c, a);
+        if (c + 16 >= columns) {   // the accumulator has been read
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_at(acc_empty0 + 8u * (uint32_t)acc);
         }
-        __syncwarp();
-        if (n <= 0 || row >= p.rows) continue;
-        const long long lin = (long long)row * p.y_pitch + unit;
-        if (fast_w) {
-          requant(bias[0], p.qw, a);
-          look_up<32>(p, table_s, a);
-        } else {
-          add_bias(bias[0], a);
-          activate<32>(p, table_s, a);
-        }
-        if (p.gated) {
-          if (fast_v) {
-            requant(bias[1], p.qv, b);
+        if (n > 0 && row < p.rows) {
+          const long long lin = (long long)row * p.y_pitch + unit;
+          if (fast1) {
+            requant(bias + c, p.qw, a);
+            look_up<16>(p, table_s, a);
           } else {
-            add_bias(bias[1], b);
-            apply_chain<32>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+            add_bias(bias + c, a);
+            activate<16>(p, table_s, a);
           }
+          if (p.gated) {
+            if (fast2) {
+              requant(bias + 32 + c, p.qv, b);
+            } else {
+              add_bias(bias + 32 + c, b);
+              apply_chain<16>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+            }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+            for (int j = 0; j < 16; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+          }
+          if (res_here && n == 16) {
+            const uint32_t w[4] = {res[q].x, res[q].y, res[q].z, res[q].w};
+#pragma unroll
+            for (int j = 0; j < 16; ++j) b[j] = (int32_t)(int8_t)(w[j >> 2] >> ((j & 3) * 8));
+          } else if (p.res) {
+            load_run(p.res, p.res_dtype, lin, n, b);
+          }
+          apply_chain<16, true>(p.cy, a, 0, 0, 0, b, p.res_step);
+          store_run(p.y, p.y_dtype, lin, n, a);
         }
-        if (p.res) load_run(p.res, p.res_dtype, lin, n, b);
-        apply_chain<32, true>(p.cy, a, 0, 0, 0, b, p.res_step);
-        store_run(p.y, p.y_dtype, lin, n, a);
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -786,7 +793,7 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   memcpy(&tv, plan->tmap_v, sizeof(tv));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)plan->grid);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(pair ? PAIR_THREADS : THREADS);
   cfg.dynamicSmemBytes = (size_t)plan->smem_bytes;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];
