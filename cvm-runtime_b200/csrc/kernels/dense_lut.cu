@@ -31,7 +31,7 @@ constexpr int BLOCK_K = 128;     // bytes of K a ring stage
 constexpr int MAX_STAGES = 12;
 constexpr int W_BYTES = BLOCK_M * BLOCK_K;          // of a stage: 128 rows of weights
 constexpr int TABLE_SMEM_MAX = 16 * 1024;
-constexpr int SMEM_MAX = 222 * 1024;   // of a launch; a kernel's static part is less than the rest
+constexpr int SMALL_SMEM_MAX = 224 * 1024, PAIR_SMEM_MAX = 206 * 1024;   // of a launch; a kernel's static part is less than the rest
 constexpr uint32_t FULL_MASK = 0xffffffffu;
 
 // A chain of a rounding shift with clamps, and for the one in front of a table the sum with a constant and the table's
@@ -58,6 +58,11 @@ struct Params {
   Requant qw, qv;
   int table_s_dtype;               // of the copy in shared memory
   DevChain cw, cv, cy;
+  int straight;                    // 1: straight_part() takes the chains and the table, and the tensor operand if there is one
+  int io;                          // 1: and y, and that operand, go through shared memory by TMA
+  int tail;                        // 1: chain_y ends with an int8 tensor and a clip, which run on packed 16-bit words
+  uint32_t tail_lo, tail_hi;       // the clip's bounds in both halves
+  DevChain head;                   // chain_y without those two steps
   DevChain ct;                     // ungated: steps of chain_y that the copy of the table has gone through already
 };
 
@@ -337,12 +342,14 @@ __device__ __forceinline__ void load_run(const void* base, int dtype, long long 
   for (int j = 0; j < 16; ++j)
     t[j] = j >= n ? 0 : (dtype == CVMK_I8 ? (int32_t) reinterpret_cast<const int8_t*>(at)[j] : reinterpret_cast<const int32_t*>(at)[j]);
 }
+__device__ __forceinline__ uint4 packed(const int32_t (&t)[16]) {
+  return make_uint4(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]), pack4(t[8], t[9], t[10], t[11]), pack4(t[12], t[13], t[14], t[15]));
+}
 __device__ __forceinline__ void store_run(void* base, int dtype, long long lin, int n, const int32_t (&t)[16]) {
   uint8_t* at = reinterpret_cast<uint8_t*>(base) + lin * dtype;
   if (n == 16 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
     if (dtype == CVMK_I8) {
-      *reinterpret_cast<uint4*>(at) = make_uint4(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]), pack4(t[8], t[9], t[10], t[11]),
-                                                 pack4(t[12], t[13], t[14], t[15]));
+      *reinterpret_cast<uint4*>(at) = packed(t);
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q) reinterpret_cast<int4*>(at)[q] = make_int4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
@@ -355,6 +362,27 @@ __device__ __forceinline__ void store_run(void* base, int dtype, long long lin, 
       if (dtype == CVMK_I8) reinterpret_cast<int8_t*>(at)[j] = (int8_t)t[j];
       else reinterpret_cast<int32_t*>(at)[j] = t[j];
     }
+}
+// Values within 8 bits, the int8 operand `r` added to or subtracted from them (or they from it) and a clip, two elements an
+// instruction: the low bytes.
+__device__ __forceinline__ uint4 packed_tail(const Params& p, const uint4& r, const int32_t (&a)[16]) {
+  const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+  const int op = p.cy.s[p.cy.n - 2].op;
+  uint32_t w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t h0 = __byte_perm((uint32_t)a[4 * q], (uint32_t)a[4 * q + 1], 0x5410), h1 = __byte_perm((uint32_t)a[4 * q + 2], (uint32_t)a[4 * q + 3], 0x5410);
+    const uint32_t r0 = prmt(rw[q], 0, 0x9180), r1 = prmt(rw[q], 0, 0xB3A2);   // bytes sign-extended to 16 bits
+    if (op == K_ADD_T) {
+      h0 = __vmaxs2(__viaddmin_s16x2(h0, r0, p.tail_hi), p.tail_lo);
+      h1 = __vmaxs2(__viaddmin_s16x2(h1, r1, p.tail_hi), p.tail_lo);
+    } else {
+      h0 = __vmaxs2(__vmins2(op == K_SUB_T ? __vsub2(h0, r0) : __vsub2(r0, h0), p.tail_hi), p.tail_lo);
+      h1 = __vmaxs2(__vmins2(op == K_SUB_T ? __vsub2(h1, r1) : __vsub2(r1, h1), p.tail_hi), p.tail_lo);
+    }
+    w[q] = __byte_perm(h0, h1, 0x6420);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ void add_bias(const int32_t* bias_s, int32_t (&v)[16]) {
 #pragma unroll
@@ -385,24 +413,109 @@ constexpr int PAIR_COLS = 256;            // of an accumulator
 constexpr int PAIR_THREADS = 576;         // warp 0: TMA, warp 1: MMA + TMEM, warps 2..17: epilogue
 constexpr int EPI_WARPS = PAIR_THREADS / 32 - 2;
 
+// A warp's columns of a tile: 32 rows (`row` is the lane's) by `columns` units from unit0 on; `t0`: their sums in TMEM, `bias`:
+// their biases in shared memory (with Requant::add in them where fast_w, fast_v), `acc_free`: the barrier that hands the accumulator back.
+struct Part {
+  int row, unit0, columns;
+  uint32_t t0, acc_free;
+  const int32_t* bias;
+  const uint8_t* table_s;
+};
+__device__ __forceinline__ void hand_back(uint32_t acc_free) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) arrive_at(acc_free);
+}
+
+// Everything that the straight form below does not take: step by step.
+__device__ __noinline__ void general_part(const Params& p, const Part t, bool fast_w, bool fast_v) {
+#pragma unroll 1
+  for (int c = 0; c < t.columns; c += 16) {
+    const int unit = t.unit0 + c, n = min(16, p.units - unit);
+    int32_t a[16], b[16];
+    __syncwarp();
+    if (p.gated) tmem_ld_two(t.t0 + (uint32_t)c, t.t0 + 128u + (uint32_t)c, a, b);
+    else tmem_ld16(t.t0 + (uint32_t)c, a);
+    if (c + 16 >= t.columns) hand_back(t.acc_free);
+    if (n <= 0 || t.row >= p.rows) continue;
+    const long long lin = (long long)t.row * p.y_pitch + unit;
+    if (fast_w) {
+      requant(t.bias + c, p.qw, a);
+      look_up<16>(p, t.table_s, a);
+    } else {
+      add_bias(t.bias + c, a);
+      activate<16>(p, t.table_s, a);
+    }
+    if (p.gated) {
+      if (fast_v) {
+        requant(t.bias + 32 + c, p.qv, b);
+      } else {
+        add_bias(t.bias + 32 + c, b);
+        apply_chain<16>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+    }
+    if (p.res) load_run(p.res, p.res_dtype, lin, n, b);
+    apply_chain<16, true>(p.cy, a, 0, 0, 0, b, p.res_step);
+    store_run(p.y, p.y_dtype, lin, n, a);
+  }
+  __syncwarp();
+}
+
+// Both sides in the three-instruction form and an int8 table in shared memory.  IO: `staged` is the warp's piece of the tile as
+// it will lie in memory, 32 rows of t.columns bytes in the TMA swizzle of that width; RES: there the int8 operand of the tensor
+// step lies already.  Little code: what a tile's loop holds has to come to the SM's instruction cache.
+template <bool GATED, bool RES, bool IO>
+__device__ __forceinline__ void straight_part(const Params& p, const Part& t, const int8_t* table_s, uint8_t* staged) {
+  const int lane = threadIdx.x & 31;
+  constexpr int COLUMNS = GATED ? 32 : 64;
+#pragma unroll 1
+  for (int c = 0; c < COLUMNS; c += 16) {
+    int32_t a[16], b[16];
+    if (GATED) tmem_ld_two(t.t0 + (uint32_t)c, t.t0 + 128u + (uint32_t)c, a, b);
+    else tmem_ld16(t.t0 + (uint32_t)c, a);
+    if (c + 16 >= COLUMNS) hand_back(t.acc_free);
+    requant(t.bias + c, p.qw, a);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) a[j] = table_s[a[j]];
+    if (GATED) {
+      requant(t.bias + 32 + c, p.qv, b);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+    }
+    apply_chain<16>(RES ? p.head : p.cy, a, 0, 0, 0);
+    if (IO) {
+      uint4* at = reinterpret_cast<uint4*>(staged + panel_offset(lane, c >> 4, COLUMNS));
+      *at = RES ? packed_tail(p, *at, a) : packed(a);
+    } else if (t.row < p.rows) {
+      const int unit = t.unit0 + c;
+      store_run(p.y, p.y_dtype, (long long)t.row * p.y_pitch + unit, min(16, p.units - unit), a);
+    }
+    __syncwarp();
+  }
+}
+
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
-                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Params p) {
+                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_y,
+                      const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_full[MAX_STAGES];       // of the first CTA: the bytes of both have landed
   __shared__ uint64_t bar_empty[MAX_STAGES];
   __shared__ uint64_t bar_acc_full[2];
+  __shared__ uint64_t bar_res[EPI_WARPS][2];      // [warp][buffer]: the tensor operand of a tile has landed
   __shared__ uint64_t bar_acc_empty[2];           // of the first CTA: the warps of both have read the accumulator
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   __shared__ __align__(16) int32_t bias_s[EPI_WARPS][64];
+  __shared__ __align__(16) uint8_t table_s[TABLE_SMEM_MAX];   // (at a place the compiler knows: no addition per look-up)
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int rank = uniform((int)cluster_rank());
   const int first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1, tiles = p.unit_tiles * p.row_tiles;
   const int tile_units = p.gated ? 128 : 256;
-  uint8_t* const table_s = smem + p.stages * PAIR_STAGE;
   const bool leader = elect_one();
   touch_params(p);
 
@@ -414,6 +527,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     for (int a = 0; a < 2; ++a) {
       mbar_init(&bar_acc_full[a], 1);
       mbar_init(&bar_acc_empty[a], 2 * EPI_WARPS);
+      for (int w = 0; w < EPI_WARPS; ++w) mbar_init(&bar_res[w][a], 1);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -490,21 +604,33 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     const uint32_t acc_empty0 = map_rank(smem_u32(&bar_acc_empty[0]), 0);
     int32_t* const bias = bias_s[warp - 2];   // of w's columns, gated: 32 of w's and 32 of v's
     const int32_t* const bias2 = p.gated ? p.bias_v : p.bias_w;
+    // the warp's piece of a tile on its way, in one buffer or (tensor operands, which come a tile early) two
+    const int piece = 32 * columns;
+    uint8_t* const staged0 = smem + p.stages * PAIR_STAGE + (warp - 2) * piece * (p.res ? 2 : 1);
+    uint32_t res_phase = 0;
+    auto request = [&](int tile, int buffer) {   // (one lane)
+      const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
+      const int row = rt * 256 + rank * 128 + quarter * 32, unit = ut * tile_units + group * columns;
+      if (row >= p.rows || unit >= p.units) return;
+      mbar_expect_tx(&bar_res[warp - 2][buffer], (uint32_t)piece);
+      tma_load_2d(staged0 + buffer * piece, &tmap_r, &bar_res[warp - 2][buffer], unit, row);
+    };
+    if (p.io && p.res && lane == 0 && first < tiles) request(first, 0);
     int i = 0;
     for (int tile = first; tile < tiles; tile += step, ++i) {
       const int acc = i & 1;
       const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
-      const int row = rt * 256 + rank * 128 + quarter * 32 + lane, unit0 = ut * tile_units + group * columns;
+      const int warp_row = rt * 256 + rank * 128 + quarter * 32, row = warp_row + lane, unit0 = ut * tile_units + group * columns;
       const uint32_t t0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * PAIR_COLS + group * columns);
       // what the tile needs beside the sums travels while the products are computed: the biases, and an int8 residual
       const int u1 = unit0 + lane, u2 = p.gated ? u1 : u1 + 32;
       const int32_t b1 = p.bias_w && u1 < p.units ? p.bias_w[u1] : 0, b2 = bias2 && u2 < p.units ? bias2[u2] : 0;
-      uint4 res[4];
-      const int8_t* res_row = reinterpret_cast<const int8_t*>(p.res) + (long long)row * p.y_pitch + unit0;
-      const bool res_here = p.res && p.res_dtype == CVMK_I8 && row < p.rows && (reinterpret_cast<uintptr_t>(res_row) & 15) == 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (res_here && 16 * q < columns && unit0 + 16 * q + 16 <= p.units) res[q] = reinterpret_cast<const uint4*>(res_row)[q];
+      // (p.io: the operand of the next tile sets out into the buffer that the last tile's results have left)
+      const bool live = warp_row < p.rows && unit0 < p.units;
+      if (p.io && lane == 0) {
+        tma_store_wait_read();
+        if (p.res && tile + step < tiles) request(tile + step, (i + 1) & 1);
+      }
       const Requant& q2 = p.gated ? p.qv : p.qw;
       bool fast1 = __all_sync(FULL_MASK, in_room(b1, p.qw)) && p.qw.on, fast2 = __all_sync(FULL_MASK, in_room(b2, q2)) && q2.on;
       if (!p.gated) fast1 = fast2 = fast1 && fast2;
@@ -514,51 +640,29 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
       __syncwarp();
       if (!__all_sync(FULL_MASK, mbar_wait(&bar_acc_full[acc], (uint32_t)((i >> 1) & 1), &abort_flag, 4))) break;
       tc_fence_after();
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 16 * q;
-        if (c >= columns) break;
-        const int unit = unit0 + c, n = min(16, p.units - unit);
-        int32_t a[16], b[16];
-        if (p.gated) tmem_ld_two(t0 + (uint32_t)c, t0 + 128u + (uint32_t)c, a, b);
-        else tmem_ld16(t0 + (uint32_t)c, a);
-        if (c + 16 >= columns) {   // the accumulator has been read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(acc_empty0 + 8u * (uint32_t)acc);
-        }
-        if (n > 0 && row < p.rows) {
-          const long long lin = (long long)row * p.y_pitch + unit;
-          if (fast1) {
-            requant(bias + c, p.qw, a);
-            look_up<16>(p, table_s, a);
-          } else {
-            add_bias(bias + c, a);
-            activate<16>(p, table_s, a);
-          }
-          if (p.gated) {
-            if (fast2) {
-              requant(bias + 32 + c, p.qv, b);
-            } else {
-              add_bias(bias + 32 + c, b);
-              apply_chain<16>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
-          }
-          if (res_here && n == 16) {
-            const uint32_t w[4] = {res[q].x, res[q].y, res[q].z, res[q].w};
-#pragma unroll
-            for (int j = 0; j < 16; ++j) b[j] = (int32_t)(int8_t)(w[j >> 2] >> ((j & 3) * 8));
-          } else if (p.res) {
-            load_run(p.res, p.res_dtype, lin, n, b);
-          }
-          apply_chain<16, true>(p.cy, a, 0, 0, 0, b, p.res_step);
-          store_run(p.y, p.y_dtype, lin, n, a);
-        }
+      const Part part = {row, unit0, columns, t0, acc_empty0 + 8u * (uint32_t)acc, bias, table_s};
+      const int buffer = p.res ? acc : 0;
+      uint8_t* const staged = staged0 + buffer * piece;
+      const int8_t* const table8 = reinterpret_cast<const int8_t*>(table_s);
+      if (p.io && p.res && live) {
+        if (!__all_sync(FULL_MASK, mbar_wait(&bar_res[warp - 2][buffer], (res_phase >> buffer) & 1u, &abort_flag, 5))) break;
+        res_phase ^= 1u << buffer;
+      }
+      const bool straight = fast1 && fast2 && p.straight;
+      if (!straight) general_part(p, part, fast1, fast2);
+      else if (p.io && p.res) p.gated ? straight_part<true, true, true>(p, part, table8, staged) : straight_part<false, true, true>(p, part, table8, staged);
+      else if (p.io) p.gated ? straight_part<true, false, true>(p, part, table8, staged) : straight_part<false, false, true>(p, part, table8, staged);
+      else p.gated ? straight_part<true, false, false>(p, part, table8, staged) : straight_part<false, false, false>(p, part, table8, staged);
+      if (straight && p.io) {
+        fence_async_smem();
         __syncwarp();
+        if (lane == 0 && live) {
+          tma_store_2d(&tmap_y, staged, unit0, warp_row);
+          tma_store_commit();
+        }
       }
     }
+    if (p.io && lane == 0) tma_store_wait_all();   // (shared memory goes with the CTA)
     __syncwarp();
   }
   if (abort_flag) {
@@ -597,12 +701,13 @@ int sm_count() {
   return sms;
 }
 
-// A row-major int8 matrix, read in boxes of BLOCK_K bytes of `box_rows` rows; zeros outside.
-CUresult encode_matrix(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows, CUtensorMapL2promotion promo) {
+// A row-major int8 matrix, in boxes of `box_cols` bytes of `box_rows` rows; zeros outside.
+CUresult encode_matrix(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows, CUtensorMapL2promotion promo,
+                       int box_cols = BLOCK_K) {
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  cuuint32_t box[2] = {(cuuint32_t)BLOCK_K, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
   return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B), promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // The three-instruction form of a lowered chain from step `first` on, in front of a table of `len` entries or not (0).
@@ -707,17 +812,34 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   if (plan->kernel == 1) {
     plan->row_tile = 256;
     plan->split = 1;
-    plan->stages = 6;
+    // y in int8 leaves, and an int8 tensor operand comes, by TMA; a warp's piece of the tile waits in shared memory, twice with
+    // an operand, for which the ring gives up two of its six stages
+    plan->io = p.y_dtype == CVMK_I8 && !((uintptr_t)p.y & 15) && p.y_pitch % 16 == 0;
+    const void* operand = nullptr;
+    for (int i = 0; i < p.chain_y.n; ++i)
+      if (is_tensor_step(p.chain_y.s[i])) {
+        operand = p.chain_y.s[i].ptr;
+        if (p.chain_y.s[i].ptr_dtype != CVMK_I8 || ((uintptr_t)operand & 15)) plan->io = 0;
+      }
+    const int staged = plan->io ? 128 * (p.v ? 128 : 256) * (operand ? 2 : 1) : 0;
+    plan->stages = std::min(6, (PAIR_SMEM_MAX - 1024 - staged) / PAIR_STAGE);
     // (no other kernel's CTAs fit beside a pair: they could hold TMEM columns and wait for its end)
-    plan->smem_bytes = std::max(1024 + plan->stages * PAIR_STAGE + table_room, 206 * 1024);
+    plan->smem_bytes = std::max(1024 + plan->stages * PAIR_STAGE + staged, 206 * 1024);
     const int64_t tiles = (int64_t)((p.rows + 255) / 256) * ((p.units + (p.v ? 127 : 255)) / (p.v ? 128 : 256));
     plan->grid = 2 * (int)std::min<int64_t>(tiles, sms / 2);
+    if (plan->io) {
+      const int columns = p.v ? 32 : 64;
+      CUresult r = encode_matrix((CUtensorMap*)plan->tmap_y, p.y, p.rows, p.units, p.y_pitch, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE, columns);
+      if (r == CUDA_SUCCESS && operand)
+        r = encode_matrix((CUtensorMap*)plan->tmap_r, operand, p.rows, p.units, p.y_pitch, 32, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, columns);
+      if (r != CUDA_SUCCESS) { set_error("dense_lut_prepare: tensor map rejected (CUresult %d)", (int)r); return CVMK_ERR_CUDA; }
+    }
     return encode_operands(plan, 128, 128);
   }
   const int row_tiles = (p.rows + 255) / 256;
   plan->row_tile = ((p.rows + row_tiles - 1) / row_tiles + 15) & ~15;
   const int64_t unit_tiles = (p.units + tile_units - 1) / tile_units, tiles = unit_tiles * row_tiles;
-  const int per_sm = plan->row_tile <= 64 ? 2 : 1, limit = per_sm == 2 ? 112 * 1024 : SMEM_MAX;
+  const int per_sm = plan->row_tile <= 64 ? 2 : 1, limit = per_sm == 2 ? 112 * 1024 : SMALL_SMEM_MAX;
   plan->split = 1;
   while (plan->split < 8 && kblocks >= 4 * plan->split && tiles * 2 * plan->split <= (int64_t)per_sm * sms) plan->split *= 2;
   auto smem_of = [&](int stages) { return 1024 + small_ring_bytes(plan->row_tile, stages) + table_room; };
@@ -770,24 +892,42 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
     for (int i = p.ct.n; i < p.cy.n; ++i) p.cy.s[i - p.ct.n] = p.cy.s[i];
     p.cy.n -= p.ct.n;
   }
+  const int at = p.cy.n - 2;
+  if (at >= 0 && is_tensor_op(p.cy.s[at].op) && p.cy.s[at].dt == CVMK_I8 && p.cy.s[at + 1].op == K_CLIP && d.y_dtype == CVMK_I8 &&
+      p.cy.s[at + 1].a >= -32767 && p.cy.s[at + 1].b <= 32767 &&
+      (at ? to_int8(p.cy.s[at - 1]) : !p.gated && p.table_s_dtype == CVMK_I8)) {
+    p.tail = 1;
+    p.head = p.cy;
+    p.head.n = at;
+    p.tail_lo = both_halves(p.cy.s[at + 1].a);
+    p.tail_hi = both_halves(p.cy.s[at + 1].b);
+  }
   p.res_step = -1;
   for (int i = 0; i < p.cy.n; ++i)
     if (is_tensor_op(p.cy.s[i].op)) {
       p.res = p.cy.s[i].ptr; p.res_dtype = p.cy.s[i].dt; p.res_step = i;
     }
 
+  p.straight = p.qw.on && (!p.gated || p.qv.on) && p.table_smem && p.table_s_dtype == CVMK_I8 && (!p.res || p.tail);
+  p.io = plan->io && p.straight;
+  if (p.res && !p.io) p.straight = 0;
+
   static bool attr_of_device[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_of_device[dev & 63]) {
-    for (auto k : {dense_lut_small_kernel, dense_lut_pair_kernel}) {
-      cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-      if (check_cuda(e, "cudaFuncSetAttribute(dense_lut)")) return CVMK_ERR_CUDA;
-    }
+    auto allow = [](auto k, int bytes) {
+      const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      return e == cudaSuccess ? cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100) : e;
+    };
+    if (check_cuda(allow(dense_lut_small_kernel, SMALL_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_small_kernel)") ||
+        check_cuda(allow(dense_lut_pair_kernel, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)"))
+      return CVMK_ERR_CUDA;
     attr_of_device[dev & 63] = true;
   }
-  CUtensorMap tx, tw, tv;
+  CUtensorMap tx, tw, tv, ty, tr;
+  memcpy(&ty, plan->tmap_y, sizeof(ty));
+  memcpy(&tr, plan->tmap_r, sizeof(tr));
   memcpy(&tx, plan->tmap_x, sizeof(tx));
   memcpy(&tw, plan->tmap_w, sizeof(tw));
   memcpy(&tv, plan->tmap_v, sizeof(tv));
@@ -804,5 +944,6 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pair || plan->split > 1 ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, pair ? dense_lut_pair_kernel : dense_lut_small_kernel, tx, tw, tv, p), "dense_lut launch");
+  if (pair) return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_pair_kernel, tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_small_kernel, tx, tw, tv, p), "dense_lut_small_kernel launch");
 }

@@ -508,6 +508,8 @@ typedef struct __attribute__((aligned(64))) {
   unsigned char tmap_x[128];
   unsigned char tmap_w[128];
   unsigned char tmap_v[128];
+  unsigned char tmap_y[128];
+  unsigned char tmap_r[128];
   cvmk_dense_lut_desc d;
   int32_t kernel;       /* 0 the weights are the 128-row operand, 1 pairs of CTAs and tiles of 256 rows */
   int32_t grid, smem_bytes;
@@ -515,7 +517,8 @@ typedef struct __attribute__((aligned(64))) {
   int32_t split;        /* CTAs of a cluster that share a tile's reduction */
   int32_t row_tile;     /* rows of x a tile */
   int32_t table_smem;   /* bytes of the table kept in shared memory, 0: read where it lies */
-  int32_t reserved[5];
+  int32_t io;           /* 1: y and an int8 tensor operand go through shared memory by TMA */
+  int32_t reserved[4];
 } cvmk_dense_lut_plan;
 
 /* 1 if the sizes, types and chains are taken; looks at no address. */

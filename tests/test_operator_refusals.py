@@ -87,8 +87,8 @@ def test_sample_null_argument(kn, rt):
 
 
 def test_binding_matches_the_header(kn):
-    """The sizes of the C structures: a plan begins with three 128-byte maps and is a whole number of 64 bytes."""
+    """The sizes of the C structures: a plan begins with five 128-byte maps and is a whole number of 64 bytes."""
     assert ct.sizeof(kn.Chain) == 8 + 8 * 24
     assert ct.sizeof(kn.DenseLutDesc) == 4 * 8 + 3 * 8 + 4 * 4 + 8 + 2 * 4 + 8 + 2 * 4 + 3 * ct.sizeof(kn.Chain)
-    assert kn.DenseLutPlan.kernel.offset == 384 + ct.sizeof(kn.DenseLutDesc)
+    assert kn.DenseLutPlan.kernel.offset == 640 + ct.sizeof(kn.DenseLutDesc)
     assert ct.sizeof(kn.SampleDesc) == 8 + 8 + 4 * 2 + 8 + 4 * 2 + 9 * 8
