@@ -1,11 +1,18 @@
 // Sampling with temperature, top-k, min-p and top-p from given random numbers, in whole numbers (cvmk_sample).
 //
-// A row belongs to one CTA, or to a cluster of them with a contiguous slice each.  A slice is read once, by a bulk
-// copy into shared memory; every later pass over it (maximum, the histograms of a cut, the draw) reads it there.
-// A cut (the k-th place, or the place where the running weight reaches the top_p share) is found digit by digit: a
-// histogram of the next ten bits of d = max - x over the elements that share the bits before, summed over the cluster,
-// and the bin in which the running count or weight reaches the target.  What is left of a row is then all elements with
-// d < D and the first `ties` ones, in index order, with d = D: neither a sort nor a list.
+// A row belongs to one CTA, or to a cluster of them with a contiguous slice each.  A slice is read once, by a bulk copy into
+// shared memory; every later pass over it reads it there.  What is left of a row after its filters is all elements with
+// d = max - x < D and the first `ties` ones, in index order, with d = D: the filters only look for that cut, and neither sort
+// nor list the row.
+//   top_k   In a CTA, the k-th largest of the maxima of its threads is a lower bound of its k-th largest element (that many
+//           threads have one as large).  The elements not below the largest of the CTAs' bounds are few more than k; they are
+//           put on a list, and the cut is found on it.
+//   top_p   An element's weight is a function of its table index, so the elements of every index are counted; the running
+//           sum of count * weight gives the index in which the share is reached and how many of its elements are needed, and
+//           the cut among those is one by count again.
+//   A cut by count, or by weight on a list, is found digit by digit: a histogram of the next ten bits of d over the elements
+//   that share the bits before, and the bin in which the running count or weight reaches the target.
+// The draw then sums the weights in blocks of 512 elements, finds the block, and looks up the element in it.
 // Counts and weights are whole numbers, so their order of summation changes nothing.
 #include <cuda_runtime.h>
 #include "common.cuh"
@@ -13,11 +20,13 @@
 namespace cvmk {
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int MAX_WARPS = 32;
 constexpr int DIGIT = 10, BINS = 1 << DIGIT;
-constexpr int TABLE_SMEM_MAX = 4096;   // entries
-constexpr int SMEM_MAX = 226 * 1024;
+constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
+constexpr int LIST = 1024, ALL = 2048;  // elements on a CTA's list, on a cluster's
+constexpr int BLOCK = 512, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / 8 / BLOCK + 2;
 constexpr uint32_t FULL = 0xffffffffu;
+constexpr uint64_t ONE = 1u << 30;
 
 struct Params {
   cvmk_sample_desc d;
@@ -31,6 +40,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// The address, in the cluster's shared window, of `p` in the CTA of rank `rank` (of a cluster of one as well).
 __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
   uint32_t d;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(p)), "r"(rank));
@@ -46,11 +56,6 @@ __device__ __forceinline__ uint64_t load64(uint32_t addr) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-  return v;
-}
 __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {   // inclusive
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -61,67 +66,100 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {   // inclusive
   return v;
 }
 
-// What a thread knows of its row.
-struct Row {
-  const int32_t* x;      // the slice in shared memory
-  const int32_t* table;
-  int first, last;       // valid places of the slice: first <= j < last
-  int32_t top;           // the largest score
-  uint32_t scale, last_entry;
-  uint64_t min_weight;   // weights below this over 2^30 are filtered out
-  uint32_t split;
-  __device__ __forceinline__ uint32_t dist(int j) const { return (uint32_t)top - (uint32_t)x[j]; }
-  __device__ __forceinline__ uint32_t raw_weight(uint32_t d) const {
-    const uint64_t q = (uint64_t)d * scale >> 16;
-    const int32_t w = table[q < last_entry ? (uint32_t)q : last_entry];
-    return (uint32_t)max(w, 0);
-  }
-  __device__ __forceinline__ uint32_t weight(uint32_t d) const {   // 0 where min_p filters it out
-    const uint32_t w = raw_weight(d);
-    return ((uint64_t)w << 30) >= min_weight ? w : 0u;
-  }
-  __device__ __forceinline__ void sync() const {
-    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    else __syncthreads();
-  }
-};
-
-struct Shared {
-  uint32_t hist[2][2][BINS];   // [buffer][low 16 bits and rest of a weight | count, -][bin]
-  uint64_t scan[WARPS];
-  uint64_t mass[WARPS];        // of this CTA's warps: weight of what lies in front of the cut
-  uint32_t ties[WARPS], kept[WARPS];
-  int32_t lo[WARPS], hi[WARPS];
-  int32_t slice_lo, slice_hi;
-  uint32_t late;               // the slice has not arrived
-  uint64_t cta_mass;
-  uint32_t cta_ties, cta_kept;
-  uint64_t found_before, found_size, total;
-  int found;
-  uint64_t bar;
-};
-
 // The elements in front of a cut: all with d < D and the first `ties`, in index order, with d = D.
 struct Cut {
   uint64_t D;
   uint32_t ties;
 };
 
-// One digit: the histogram of `count or weight` over the elements with d < limit whose bits from `shift + bits` on are `prefix`,
-// summed over the cluster; buffer alternates from call to call, so that one barrier a call is enough.
+struct Shared {
+  uint32_t hist[4 * BINS];     // counts by table index; or [buffer][low 16 bits and rest of a weight | count, -][bin]
+  uint64_t scan[MAX_WARPS];
+  int32_t lo[MAX_WARPS], hi[MAX_WARPS];
+  uint32_t kept[MAX_WARPS];
+  uint64_t block_mass[MAX_BLOCKS];
+  uint32_t block_ties[MAX_BLOCKS];
+  int32_t list[LIST], all[ALL];
+  uint32_t listed;
+  // read by the other CTAs
+  int32_t slice_lo, slice_hi, slice_bound;
+  uint32_t late;               // the slice has not arrived
+  uint64_t cta_mass;
+  uint32_t cta_ties, cta_kept;
+  uint64_t found_before, found_size, found_count, total;
+  int found;
+  uint64_t bar;
+};
+
+// What a thread knows of its row, or (find_cut) of a list of some of its elements.
+struct Row {
+  const int32_t* x;
+  const int32_t* table;
+  int first, last;       // valid places: first <= j < last
+  int32_t top;           // the largest score
+  uint32_t scale, last_entry, saturated;
+  uint32_t min_weight;   // lighter elements are filtered out; 0 where the table has gone through that already
+  uint32_t split;
+  bool wide;             // the table lies in global memory
+  __device__ __forceinline__ uint32_t dist(int32_t v) const { return (uint32_t)top - (uint32_t)v; }
+  // min((d * scale) >> 16, last_entry): a table in shared memory has less than 2^15 entries, and every d above
+  // saturated = (2^32 - 1) / scale has a product above 2^31.
+  __device__ __forceinline__ uint32_t entry(uint32_t d) const { return min(min(d, saturated) * scale >> 16, last_entry); }
+  __device__ __forceinline__ uint32_t weight(uint32_t d) const {   // 0 where min_p filters it out
+    if (!wide) return (uint32_t)table[entry(d)];
+    const uint64_t q = (uint64_t)d * scale >> 16;
+    const int32_t w = table[q < last_entry ? (uint32_t)q : last_entry];
+    return w > 0 && (uint32_t)w >= min_weight ? (uint32_t)w : 0u;
+  }
+  // The smallest d whose entry is e or more, e <= last_entry (2^32: none).
+  __device__ __forceinline__ uint64_t first_of(uint32_t e) const {
+    if (e == 0) return 0;
+    if (scale == 0) return (uint64_t)1 << 32;
+    return min((((uint64_t)e << 16) + scale - 1) / scale, (uint64_t)1 << 32);
+  }
+  __device__ __forceinline__ void sync() const {
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
+  }
+  // Calls f(value, valid) for the places 4g .. 4g + 3 of group g.
+  template <typename F>
+  __device__ __forceinline__ void group(int g, const F& f) const {
+    const int4 v = reinterpret_cast<const int4*>(x)[g];
+    const int j = 4 * g;
+    f(v.x, j >= first && j < last);
+    f(v.y, j + 1 >= first && j + 1 < last);
+    f(v.z, j + 2 >= first && j + 2 < last);
+    f(v.w, j + 3 >= first && j + 3 < last);
+  }
+};
+
+// Exclusive sum of v over the threads of the CTA, and the sum of all.
+__device__ __forceinline__ uint64_t block_scan(Shared& s, uint64_t v, uint64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const uint64_t inc = warp_scan(v);
+  __syncthreads();   // (the scan before has been read)
+  if (lane == 31) s.scan[warp] = inc;
+  __syncthreads();
+  const uint64_t w = lane < warps ? s.scan[lane] : 0, sums = warp_scan(w);
+  total = __shfl_sync(FULL, sums, 31);
+  return __shfl_sync(FULL, sums - w, warp) + inc - v;
+}
+
+// One digit: the histogram of the count (or weight) of the elements with d < limit whose bits from `shift + bits` on are `prefix`.
+// The buffer alternates from call to call, so that one barrier a call is enough.
 template <bool WEIGHT>
 __device__ void histogram(const Row& r, Shared& s, int buffer, uint64_t limit, uint32_t prefix, int shift, int bits) {
-  uint32_t* h0 = s.hist[buffer][0];
-  uint32_t* h1 = s.hist[buffer][1];
-  for (int i = threadIdx.x; i < BINS; i += THREADS) h0[i] = h1[i] = 0;
+  uint32_t* h0 = s.hist + buffer * 2 * BINS;
+  uint32_t* h1 = h0 + BINS;
+  for (int i = threadIdx.x; i < BINS; i += blockDim.x) h0[i] = h1[i] = 0;
   __syncthreads();
   const int lane = threadIdx.x & 31;
-  for (int j0 = r.first & ~31; j0 < r.last; j0 += THREADS) {
+  for (int j0 = r.first & ~31; j0 < r.last; j0 += blockDim.x) {
     const int j = j0 + (int)threadIdx.x;
     bool in = j >= r.first && j < r.last;
     uint32_t d = 0, w = 1;
     if (in) {
-      d = r.dist(j);
+      d = r.dist(r.x[j]);
       in = d < limit && ((uint64_t)d >> (shift + bits)) == prefix;
     }
     if (WEIGHT && in) {
@@ -149,36 +187,8 @@ __device__ void histogram(const Row& r, Shared& s, int buffer, uint64_t limit, u
   r.sync();
 }
 
-// Sums of the cluster's histograms in bins 2t, 2t + 1 (t: the thread) and the running sum in front of them.
-template <bool WEIGHT>
-__device__ void running(const Row& r, Shared& s, int buffer, uint64_t (&own)[2], uint64_t& before, uint64_t& total) {
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  own[0] = own[1] = 0;
-  for (uint32_t c = 0; c < r.split; ++c) {
-    const uint64_t a = load64(r.split > 1 ? remote(&s.hist[buffer][0][2 * t], c) : smem_addr(&s.hist[buffer][0][2 * t]));
-    own[0] += (uint32_t)a;
-    own[1] += a >> 32;
-    if (WEIGHT) {
-      const uint64_t b = load64(r.split > 1 ? remote(&s.hist[buffer][1][2 * t], c) : smem_addr(&s.hist[buffer][1][2 * t]));
-      own[0] += (uint64_t)(uint32_t)b << 16;
-      own[1] += b >> 32 << 16;
-    }
-  }
-  const uint64_t sum = own[0] + own[1], inc = warp_scan(sum);
-  if (lane == 31) s.scan[warp] = inc;
-  __syncthreads();
-  if (warp == 0) {
-    const uint64_t v = lane < WARPS ? s.scan[lane] : 0, all = warp_scan(v);
-    if (lane < WARPS) s.scan[lane] = all - v;
-    if (lane == WARPS - 1) s.total = all;
-  }
-  __syncthreads();
-  before = s.scan[warp] + inc - sum;
-  total = s.total;
-}
-
-// Where, in the order of d, the count (or the weight) of the elements with d < limit reaches need(total); `fallback` is the
-// cut if the total is less than that.
+// Where, in the order of d, the count (or the weight) of the elements with d < limit reaches need(total); if the total is
+// less than that, a cut among the ties of `whole`, of tie_weight each.
 template <bool WEIGHT, typename Need>
 __device__ Cut find_cut(const Row& r, Shared& s, int& buffer, uint64_t limit, int range_bits, const Need& need_of, const Cut& whole, uint32_t tie_weight) {
   int bits = min(range_bits, DIGIT), shift = range_bits - bits;
@@ -186,21 +196,27 @@ __device__ Cut find_cut(const Row& r, Shared& s, int& buffer, uint64_t limit, in
   uint64_t need = 0;
   for (bool first = true;; first = false) {
     histogram<WEIGHT>(r, s, buffer, limit, prefix, shift, bits);
-    uint64_t own[2], before, total;
-    running<WEIGHT>(r, s, buffer, own, before, total);
+    const uint32_t* h0 = s.hist + buffer * 2 * BINS;
     buffer ^= 1;
+    const int per = BINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // one or two bins a thread
+    uint64_t own[2] = {0, 0};
+    for (uint32_t c = 0; c < r.split; ++c)
+      for (int k = 0; k < per; ++k) {
+        own[k] += load32(remote(h0 + bin0 + k, r.split > 1 ? c : cluster_rank()));
+        if (WEIGHT) own[k] += (uint64_t)load32(remote(h0 + BINS + bin0 + k, r.split > 1 ? c : cluster_rank())) << 16;
+      }
+    uint64_t total, before = block_scan(s, own[0] + own[1], total);
     if (first) {
       need = need_of(total);
-      if (need > total) {   // the cut lies among the ties of `whole`
+      if (need > total) {
         Cut c = whole;
         if (tie_weight) c.ties = (uint32_t)min((uint64_t)whole.ties, (need - total + tie_weight - 1) / tie_weight);
         return c;
       }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < per; ++k) {
       if (before < need && need <= before + own[k]) {
-        s.found = 2 * (int)threadIdx.x + k;
+        s.found = bin0 + k;
         s.found_before = before;
         s.found_size = own[k];
       }
@@ -228,10 +244,38 @@ __device__ Cut find_cut(const Row& r, Shared& s, int& buffer, uint64_t limit, in
   }
 }
 
-__global__ void __launch_bounds__(THREADS) sample_kernel(const __grid_constant__ Params p) {
+// The elements for which take(d) holds, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are too many.
+template <typename Take>
+__device__ int collect(const Row& r, Shared& s, const Take& take) {
+  if (threadIdx.x == 0) s.listed = 0;
+  __syncthreads();
+  for (int g = (r.first >> 2) + (int)threadIdx.x; 4 * g < r.last; g += blockDim.x)
+    r.group(g, [&](int32_t v, bool valid) {
+      if (valid && take(r.dist(v))) {
+        const uint32_t at = atomicAdd(&s.listed, 1u);
+        if (at < LIST) s.list[at] = v;
+      }
+    });
+  r.sync();
+  uint32_t n = 0;
+  bool fits = true;
+  for (uint32_t c = 0; c < r.split; ++c) {
+    const uint32_t m = r.split > 1 ? load32(remote(&s.listed, c)) : s.listed;
+    fits = fits && m <= LIST && n + m <= ALL;
+    if (fits)
+      for (uint32_t i = threadIdx.x; i < m; i += blockDim.x) s.all[n + i] = r.split > 1 ? (int32_t)load32(remote(&s.list[i], c)) : s.list[i];
+    n += m;
+  }
+  __syncthreads();
+  return fits ? (int)n : -1;
+}
+
+__device__ __forceinline__ int bits_of(uint64_t range) { return max(1, 64 - __clzll((long long)range)); }   // of the largest distance
+
+__global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ Shared s;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   const int rank = p.split > 1 ? (int)cluster_rank() : 0, row = (int)blockIdx.x / p.split;
   int32_t* const x = reinterpret_cast<int32_t*>(smem_raw);
   int32_t* const table_s = x + p.slice;
@@ -266,16 +310,21 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const __grid_constant__
   }
   if (tid >= 32 && tid < 35 && r.first + tid - 32 < b0) x[r.first + tid - 32] = at[r.first + tid - 32];
   if (tid >= 35 && tid < 38 && b1 + tid - 35 < r.last) x[b1 + tid - 35] = at[b1 + tid - 35];
-  if (p.table_smem)
-    for (int i = tid; i < d.table_len; i += THREADS) table_s[i] = d.table[i];
-  r.table = p.table_smem ? table_s : d.table;
-  r.last_entry = (uint32_t)d.table_len - 1u;
-  r.scale = (uint32_t)max(d.scale[row], 0);
   const int k = d.top_k ? d.top_k[row] : 0;
-  const uint64_t one = 1u << 30;
-  const uint64_t top_p = d.top_p ? (uint64_t)min(max(d.top_p[row], 0), (int)one) : one;
-  const uint64_t min_p = d.min_p ? (uint64_t)min(max(d.min_p[row], 0), (int)one) : 0;
+  const uint64_t top_p = d.top_p ? (uint64_t)min(max(d.top_p[row], 0), (int)ONE) : ONE;
+  const uint64_t min_p = d.min_p ? (uint64_t)min(max(d.min_p[row], 0), (int)ONE) : 0;
   const uint64_t u = (uint64_t)(d.random[row] & 0x7fffffff);
+  r.scale = (uint32_t)max(d.scale[row], 0);
+  r.saturated = r.scale ? 0xffffffffu / r.scale : 0xffffffffu;
+  r.last_entry = (uint32_t)d.table_len - 1u;
+  r.min_weight = (uint32_t)((min_p * (uint64_t)max(d.table[0], 0) + ONE - 1) >> 30);
+  r.wide = !p.table_smem;
+  r.table = p.table_smem ? table_s : d.table;
+  if (p.table_smem)
+    for (int i = tid; i < d.table_len; i += threads) {
+      const int32_t w = max(d.table[i], 0);
+      table_s[i] = (uint32_t)w >= r.min_weight ? w : 0;
+    }
   __syncthreads();
   // (bounded: the copy is the only thing that is waited for)
   bool landed = false;
@@ -289,29 +338,51 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const __grid_constant__
     landed = ok != 0;
   }
 
-  // ---- the largest and the smallest score
+  // ---- the largest and the smallest score, and the bound of the k-th largest
   int32_t lo = INT32_MAX, hi = INT32_MIN;
-  for (int j = r.first + tid; j < r.last; j += THREADS) {
-    lo = min(lo, x[j]);
-    hi = max(hi, x[j]);
-  }
+  for (int g = (r.first >> 2) + tid; 4 * g < r.last; g += threads)
+    r.group(g, [&](int32_t v, bool valid) {
+      if (valid) {
+        lo = min(lo, v);
+        hi = max(hi, v);
+      }
+    });
+  const bool some = lo <= hi;   // the thread has seen an element
+  const int32_t mine = hi;
   lo = __reduce_min_sync(FULL, lo);
   hi = __reduce_max_sync(FULL, hi);
   if (lane == 0) { s.lo[warp] = lo; s.hi[warp] = hi; }
   __syncthreads();
-  if (warp == 0) {
-    lo = __reduce_min_sync(FULL, lane < WARPS ? s.lo[lane] : INT32_MAX);
-    hi = __reduce_max_sync(FULL, lane < WARPS ? s.hi[lane] : INT32_MIN);
-    if (lane == 0) { s.slice_lo = lo; s.slice_hi = hi; s.late = landed ? 0u : 1u; }
+  lo = __reduce_min_sync(FULL, lane < warps ? s.lo[lane] : INT32_MAX);
+  hi = __reduce_max_sync(FULL, lane < warps ? s.hi[lane] : INT32_MIN);
+  const bool by_count = k >= 1 && k < vocab;
+  int32_t bound = INT32_MIN;
+  if (by_count && k <= threads) {
+    for (int i = tid; i < BINS; i += threads) s.hist[i] = 0;
+    if (tid == 0) s.found = -1;
+    __syncthreads();
+    const int shift = max(0, bits_of((uint32_t)hi - (uint32_t)lo) - DIGIT);
+    if (some) atomicAdd(&s.hist[((uint32_t)hi - (uint32_t)mine) >> shift], 1u);
+    __syncthreads();
+    const int per = BINS / threads, bin0 = per * tid;
+    const uint32_t n0 = s.hist[bin0], n1 = per > 1 ? s.hist[bin0 + 1] : 0;
+    uint64_t total;
+    const uint64_t before = block_scan(s, n0 + n1, total), need = (uint64_t)k;
+    if (before < need && need <= before + n0 + n1) s.found = need <= before + n0 ? bin0 : bin0 + 1;
+    __syncthreads();
+    if (s.found >= 0) {
+      const int64_t b = (int64_t)hi - ((((int64_t)s.found + 1) << shift) - 1);
+      bound = b > INT32_MIN ? (int32_t)b : INT32_MIN;
+    }
   }
+  if (tid == 0) { s.slice_lo = lo; s.slice_hi = hi; s.slice_bound = bound; s.late = landed ? 0u : 1u; }
   r.sync();
-  lo = s.slice_lo;
-  hi = s.slice_hi;
   uint32_t late = s.late;
   for (int c = 0; p.split > 1 && c < p.split; ++c) {
     late |= load32(remote(&s.late, (uint32_t)c));
     lo = min(lo, (int32_t)load32(remote(&s.slice_lo, (uint32_t)c)));
     hi = max(hi, (int32_t)load32(remote(&s.slice_hi, (uint32_t)c)));
+    bound = max(bound, (int32_t)load32(remote(&s.slice_bound, (uint32_t)c)));
   }
   if (late) {   // a copy that never came (its wait is bounded): no element is drawn
     if (rank == 0 && tid == 0) d.token[row] = -1;
@@ -321,53 +392,149 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const __grid_constant__
     return;
   }
   r.top = hi;
-  r.min_weight = 0;
-  r.min_weight = min_p * (uint64_t)r.raw_weight(0);
-  const uint32_t range = (uint32_t)hi - (uint32_t)lo;
-  const int range_bits = max(1, 32 - __clz((int)range));
+  const int range_bits = bits_of((uint32_t)hi - (uint32_t)lo);
 
   // ---- the cuts
   Cut cut = {(uint64_t)1 << 32, 0};   // everything
   int buffer = 0;
-  if (k >= 1 && k < vocab)
-    cut = find_cut<false>(r, s, buffer, (uint64_t)1 << 32, range_bits, [=](uint64_t) { return (uint64_t)k; }, cut, 0u);
-  if (top_p < one) {
-    const uint32_t w = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
-    const uint32_t ties = cut.ties;
-    cut = find_cut<true>(r, s, buffer, cut.D, range_bits, [=](uint64_t strict) {
-      const uint64_t all = strict + (uint64_t)ties * w;
-      const uint64_t need = top_p * (all >> 30) + ((top_p * (all & (one - 1)) + one - 1) >> 30);
+  const Cut everything = cut;
+  // The cut that leaves `count` elements, all of them with from <= d < to except `known` ones in front of `from`.
+  auto cut_by_count = [&](uint64_t count, uint64_t known, uint64_t from, uint64_t to, Row* list) {
+    const int n = collect(r, s, [&](uint32_t dj) { return dj >= from && dj < to; });
+    if (n < 0) return find_cut<false>(r, s, buffer, everything.D, range_bits, [=](uint64_t) { return count; }, everything, 0u);
+    list->x = s.all;
+    list->first = 0;
+    list->last = n;
+    list->split = 1;
+    Row near = *list;
+    near.top = (int32_t)((uint32_t)r.top - (uint32_t)from);
+    Cut c = find_cut<false>(near, s, buffer, to - from, bits_of(min(to - 1 - from, (uint64_t)0xffffffffu)), [=](uint64_t) { return count - known; }, everything, 0u);
+    c.D += from;
+    return c;
+  };
+  Row list = r;   // what find_cut may look at instead of the row: a list that holds everything in front of the cut
+  if (by_count) cut = cut_by_count((uint64_t)k, 0, 0, (uint64_t)r.dist(bound) + 1, &list);
+  if (top_p < ONE) {
+    const auto share_of = [=](uint64_t all) {
+      const uint64_t need = top_p * (all >> 30) + ((top_p * (all & (ONE - 1)) + ONE - 1) >> 30);
       return need > 1 ? need : (uint64_t)1;
-    }, cut, w);
-  }
-
-  // ---- the draw: every warp sums a contiguous run of the slice
-  const uint32_t tie_weight = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
-  const int run = ((p.slice + WARPS - 1) / WARPS + 31) & ~31;
-  const int j0 = warp * run, j1 = min(j0 + run, r.last);
-  uint64_t mass = 0;
-  uint32_t ties = 0, kept = 0;
-  for (int j = max(j0, r.first & ~31) + lane; j < j1; j += 32) {
-    if (j < r.first) continue;
-    const uint32_t dj = r.dist(j);
-    if (dj < cut.D) {
-      const uint32_t w = r.weight(dj);
-      mass += w;
-      kept += w > 0;
+    };
+    if (by_count || r.wide) {
+      const uint32_t w = cut.ties ? r.weight((uint32_t)cut.D) : 0u, ties = cut.ties;
+      cut = find_cut<true>(list, s, buffer, cut.D, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
     } else {
-      ties += dj == cut.D;
+      const uint32_t entries = (uint32_t)d.table_len;
+      for (uint32_t i = tid; i < 4 * BINS; i += threads) s.hist[i] = 0;
+      if (tid == 0) s.found = -1;
+      __syncthreads();
+      uint32_t last = 0;   // (elements far behind the first: one counter, kept in registers)
+      for (int g = (r.first >> 2) + tid; 4 * g < r.last; g += threads)
+        r.group(g, [&](int32_t v, bool valid) {
+          const uint32_t e = r.entry(r.dist(v));
+          if (valid) {
+            if (e == r.last_entry) ++last;
+            else atomicAdd(&s.hist[e], 1u);
+          }
+        });
+      last = __reduce_add_sync(FULL, last);
+      if (lane == 0 && last) atomicAdd(&s.hist[r.last_entry], last);
+      r.sync();
+      const int per = 4 * BINS / threads;   // four or eight entries a thread
+      const uint32_t e0 = (uint32_t)(per * tid);
+      uint32_t n[8];
+      uint64_t count = 0, mass = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        n[i] = 0;
+        if (i >= per || e0 + i >= entries) continue;
+        for (uint32_t c = 0; c < r.split; ++c) n[i] += r.split > 1 ? load32(remote(&s.hist[e0 + i], c)) : s.hist[e0 + i];
+        count += n[i];
+        mass += (uint64_t)n[i] * (uint32_t)table_s[e0 + i];
+      }
+      uint64_t all, elements;
+      uint64_t before = block_scan(s, mass, all), in_front = block_scan(s, count, elements);
+      const uint64_t need = share_of(all);
+      if (before < need && need <= before + mass) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i >= per || e0 + i >= entries) continue;
+          const uint64_t w = (uint32_t)table_s[e0 + i], here = n[i] * w;
+          if (before < need && need <= before + here) {
+            s.found = (int)(e0 + i);
+            s.found_before = (need - before + w - 1) / w;   // elements of this entry that are needed
+            s.found_size = n[i];
+            s.found_count = in_front;
+          }
+          before += here;
+          in_front += n[i];
+        }
+      }
+      __syncthreads();
+      const int e = s.found;
+      const uint64_t wanted = s.found_before, size = s.found_size, front = s.found_count;
+      __syncthreads();
+      if (e >= 0) {   // (else nothing weighs anything, and no cut is needed)
+        const uint64_t from = r.first_of((uint32_t)e), to = (uint32_t)e == r.last_entry ? everything.D : r.first_of((uint32_t)e + 1);
+        if (wanted == size) cut = {to, 0};
+        else if (to - from == 1) cut = {from, (uint32_t)wanted};
+        else cut = cut_by_count(front + wanted, front, from, to, &list);
+      }
     }
   }
-  mass = warp_sum(mass);
-  ties = __reduce_add_sync(FULL, ties);
+
+  // ---- the draw: weights and ties of every block of the slice
+  uint32_t tie_weight = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
+  const int blocks = (r.last + BLOCK - 1) / BLOCK;
+  uint32_t kept = 0;
+  const uint32_t D32 = (uint32_t)min(cut.D, (uint64_t)0xffffffffu);
+  const bool beyond = cut.D > 0xffffffffu;
+  for (int b = warp; b < blocks; b += warps) {
+    uint32_t low = 0, high = 0, ties = 0;
+#pragma unroll
+    for (int i = 0; i < BLOCK / 128; ++i) {
+      const int g = b * (BLOCK / 4) + i * 32 + lane;
+      if (4 * g >= r.last) break;
+      r.group(g, [&](int32_t v, bool valid) {
+        const uint32_t dj = r.dist(v);
+        if (valid && (dj < D32 || beyond)) {
+          const uint32_t w = r.weight(dj);
+          low += w & 0xffffu;
+          high += w >> 16;
+          kept += w > 0;
+        } else {
+          ties += valid && dj == D32;
+        }
+      });
+    }
+    __syncwarp();
+    low = __reduce_add_sync(FULL, low);
+    high = __reduce_add_sync(FULL, high);
+    ties = __reduce_add_sync(FULL, ties);
+    if (lane == 0) {
+      s.block_mass[b] = low + ((uint64_t)high << 16);
+      s.block_ties[b] = ties;
+    }
+  }
   kept = __reduce_add_sync(FULL, kept);
-  if (lane == 0) { s.mass[warp] = mass; s.ties[warp] = ties; s.kept[warp] = kept; }
+  if (lane == 0) s.kept[warp] = kept;
   __syncthreads();
-  if (tid == 0) {
-    uint64_t m = 0;
-    uint32_t t = 0, n = 0;
-    for (int i = 0; i < WARPS; ++i) { m += s.mass[i]; t += s.ties[i]; n += s.kept[i]; }
-    s.cta_mass = m; s.cta_ties = t; s.cta_kept = n;
+  constexpr int PER = (MAX_BLOCKS + 31) / 32;   // blocks a lane of warp 0
+  uint64_t mass_in_front = 0;
+  uint32_t ties_in_front = 0;                   // of the lane's blocks
+  auto scan_blocks = [&]() {
+    uint64_t m = 0, t = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane * PER + i < blocks) { m += s.block_mass[lane * PER + i]; t += s.block_ties[lane * PER + i]; }
+    const uint64_t mi = warp_scan(m), ti = warp_scan(t);
+    mass_in_front = mi - m;
+    ties_in_front = (uint32_t)(ti - t);
+    if (lane == 31) { s.cta_mass = mi; s.cta_ties = (uint32_t)ti; }
+  };
+  if (warp == 0) {
+    scan_blocks();
+    kept = __reduce_add_sync(FULL, lane < warps ? s.kept[lane] : 0u);
+    if (lane == 0) s.cta_kept = kept;
   }
   r.sync();
   uint64_t all = 0, front_mass = 0;
@@ -375,65 +542,92 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const __grid_constant__
   for (int c = 0; c < p.split; ++c) {
     const uint64_t m = p.split > 1 ? load64(remote(&s.cta_mass, (uint32_t)c)) : s.cta_mass;
     const uint32_t t = p.split > 1 ? load32(remote(&s.cta_ties, (uint32_t)c)) : s.cta_ties;
-    const uint32_t n = p.split > 1 ? load32(remote(&s.cta_kept, (uint32_t)c)) : s.cta_kept;
+    all_kept += p.split > 1 ? load32(remote(&s.cta_kept, (uint32_t)c)) : s.cta_kept;
     all += m;
-    all_kept += n;
     if (c < rank) { front_mass += m; front_ties += t; }
   }
   all += (uint64_t)cut.ties * tie_weight;
-  // of a mass of nothing the first of the order is taken: the first element with d = 0 then weighs 1, all others nothing
-  const bool nothing = all == 0;
-  const uint64_t target = nothing ? 0 : u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
-  if (nothing) {
-    cut.D = 0;
-    cut.ties = 1;
-  }
-  const uint32_t each = nothing ? 1u : tie_weight;
-  if (nothing) {   // (rare: the ties of the new cut are counted again)
-    uint32_t n = 0;
-    for (int j = max(j0, r.first & ~31) + lane; j < j1; j += 32) n += j >= r.first && r.dist(j) == 0;
-    n = __reduce_add_sync(FULL, n);
-    if (lane == 0) { s.mass[warp] = 0; s.ties[warp] = n; }
-    __syncthreads();
+  const uint64_t target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
+  if (all == 0) {
+    // Nothing weighs anything: the first of the order is taken, as if the first element with d = 0 weighed 1 and all others
+    // nothing (rare: the ties are counted again).
+    cut = {0, 1};
+    tie_weight = 1;
     r.sync();   // (nobody still reads the sums of before)
-    if (tid == 0) {
-      uint32_t t = 0;
-      for (int i = 0; i < WARPS; ++i) t += s.ties[i];
-      s.cta_ties = t;
+    for (int b = warp; b < blocks; b += warps) {
+      uint32_t ties = 0;
+      for (int i = 0; i < BLOCK / 128; ++i) {
+        const int g = b * (BLOCK / 4) + i * 32 + lane;
+        if (4 * g < r.last) r.group(g, [&](int32_t v, bool valid) { ties += valid && r.dist(v) == 0; });
+      }
+      __syncwarp();
+      ties = __reduce_add_sync(FULL, ties);
+      if (lane == 0) { s.block_mass[b] = 0; s.block_ties[b] = ties; }
     }
+    __syncthreads();
+    if (warp == 0) scan_blocks();
     r.sync();
     front_mass = 0;
     front_ties = 0;
     for (int c = 0; c < rank; ++c) front_ties += load32(remote(&s.cta_ties, (uint32_t)c));
   }
-  // every warp: the weight in front of its run, and whether the target lies in it
-  for (int i = 0; i < warp; ++i) { front_mass += s.mass[i]; front_ties += s.ties[i]; }
-  const auto running_at = [&](uint64_t m, uint32_t t) { return m + (uint64_t)min(t, cut.ties) * each; };
-  if (running_at(front_mass, front_ties) <= target && target < running_at(front_mass + s.mass[warp], front_ties + s.ties[warp])) {
-    for (int j = max(j0, r.first & ~31); j < j1; j += 32) {
-      const int at_j = j + lane;
-      uint64_t w = 0;
-      uint32_t tie = 0;
-      if (at_j >= r.first && at_j < j1) {
-        const uint32_t dj = r.dist(at_j);
-        if (dj < cut.D) w = r.weight(dj);
-        else tie = dj == cut.D;
+  if (warp == 0) {
+    // the lane and the block of it in which the running weight passes the target
+    const auto passed = [&](uint64_t m, uint32_t t) { return m + (uint64_t)min(t, cut.ties) * tie_weight > target; };
+    uint64_t m = front_mass + mass_in_front;
+    uint32_t t = front_ties + ties_in_front;
+    int hit = -1;
+    if (!passed(m, t)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = lane * PER + i;
+        if (hit >= 0 || b >= blocks) continue;
+        if (passed(m + s.block_mass[b], t + s.block_ties[b])) { hit = b; continue; }
+        m += s.block_mass[b];
+        t += s.block_ties[b];
       }
-      const uint32_t tie_mask = __ballot_sync(FULL, tie != 0);
-      const uint64_t inc = front_mass + warp_scan(w);
-      const uint32_t tie_inc = front_ties + (uint32_t)__popc(tie_mask & (FULL >> (31 - lane)));
-      const uint32_t hit = __ballot_sync(FULL, running_at(inc, tie_inc) > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          d.token[row] = begin + at_j - skew;
-          if (d.weight) d.weight[row] = (int32_t)r.raw_weight(r.dist(at_j));
-          if (d.mass) d.mass[row] = (int64_t)all;
-          if (d.kept) d.kept[row] = (int32_t)all_kept;
+    }
+    const uint32_t who = __ballot_sync(FULL, hit >= 0);   // one lane of one CTA
+    if (who) {
+      const int from = __ffs(who) - 1;
+      const int b = __shfl_sync(FULL, hit, from);
+      m = __shfl_sync(FULL, m, from);
+      t = __shfl_sync(FULL, t, from);
+      // sixteen elements a lane
+      const int g0 = b * (BLOCK / 4) + lane * (BLOCK / 128);
+      uint64_t mass = 0;
+      uint32_t ties = 0;
+      const auto each = [&](const auto& f) {   // f(place, weight, tie) for the lane's elements
+        for (int i = 0; i < BLOCK / 128; ++i) {
+          int j = 4 * (g0 + i);
+          if (j >= r.last) break;
+          r.group(g0 + i, [&](int32_t v, bool valid) {
+            const uint32_t dj = r.dist(v);
+            f(j++, valid && dj < cut.D ? r.weight(dj) : 0u, valid && dj == cut.D ? 1u : 0u);
+          });
         }
-        break;
+      };
+      each([&](int, uint32_t w, uint32_t tie) { mass += w; ties += tie; });
+      __syncwarp();
+      m += warp_scan(mass) - mass;
+      t += (uint32_t)(warp_scan(ties) - ties);
+      if (!passed(m, t) && passed(m + mass, t + ties)) {
+        int token = -1;
+        uint32_t weight = 0;
+        each([&](int j, uint32_t w, uint32_t tie) {
+          if (token >= 0) return;
+          m += w;
+          t += tie;
+          if (passed(m, t)) {
+            token = begin + j - skew;
+            weight = tie ? (all ? tie_weight : 0u) : w;
+          }
+        });
+        d.token[row] = token;
+        if (d.weight) d.weight[row] = (int32_t)weight;
+        if (d.mass) d.mass[row] = (int64_t)all;
+        if (d.kept) d.kept[row] = (int32_t)all_kept;
       }
-      front_mass = __shfl_sync(FULL, inc, 31);
-      front_ties += (uint32_t)__popc(tie_mask);
     }
   }
   __syncwarp();
@@ -452,6 +646,7 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
     return CVMK_ERR_ARG;
   }
   if (d->pitch && (d->pitch < d->vocab || d->pitch >> 40)) { set_error("sample: bad pitch"); return CVMK_ERR_ARG; }
+  if (d->rows > INT32_MAX / 8) { set_error("sample: too many rows for one launch"); return CVMK_ERR_ARG; }
   if (d->rows == 0) return CVMK_OK;
   if (!d->logits || !d->table || !d->scale || !d->random || !d->token) { set_error("sample: null operand"); return CVMK_ERR_ARG; }
   const uintptr_t odd = (uintptr_t)d->logits | (uintptr_t)d->table | (uintptr_t)d->scale | (uintptr_t)d->top_k | (uintptr_t)d->top_p |
@@ -466,12 +661,15 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   auto slice_of = [&](int split) { return ((d->vocab + 3 + split - 1) / split + 3) & ~3; };
   auto smem_of = [&](int split) { return slice_of(split) * 4 + (p.table_smem ? d->table_len * 4 : 0); };
-  const int room = SMEM_MAX - (int)sizeof(Shared);
+  const int room = 226 * 1024 - (int)sizeof(Shared), half = 113 * 1024 - (int)sizeof(Shared) - 1024;
   p.split = 1;
-  while (p.split < 8 && (smem_of(p.split) > 90 * 1024 || ((int64_t)d->rows * p.split * 2 <= 2 * sms && slice_of(p.split) > 2048))) p.split *= 2;
+  while (p.split < 8 && (smem_of(p.split) > half || ((int64_t)d->rows * p.split * 2 <= 2 * sms && slice_of(p.split) > 2048))) p.split *= 2;
+  if (const char* e = dev_env("CVM_B200_SAMPLE_SPLIT")) p.split = atoi(e);
   p.slice = slice_of(p.split);
   const int smem = smem_of(p.split);
-  if (smem > room || (int64_t)d->rows * p.split > INT32_MAX) { set_error("sample: too large"); return CVMK_ERR_ARG; }
+  int threads = smem > half ? 1024 : 512;
+  if (const char* e = dev_env("CVM_B200_SAMPLE_THREADS")) threads = atoi(e);
+  if (smem > room) { set_error("sample: too large"); return CVMK_ERR_ARG; }
 
   static bool attr_of_device[64] = {false};
   if (!attr_of_device[dev & 63]) {
@@ -482,7 +680,7 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(d->rows * p.split));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];

@@ -13,7 +13,7 @@ I8, I32 = 1, 4
 (RELU, RSHIFT, LSHIFT, CLIP, ADD_T, SUB_T, RSUB_T, ADD_C, MUL_S, ADD_S, RSUB_S, MAX_S, DIV_S, RDIV_S, GT_S, LT_S, ABS, NEG,
  PRECISION) = range(1, 20)
 MAX_STEPS = 8
-MAX_VOCAB = 384 * 1024
+MAX_VOCAB = 320 * 1024
 
 
 class KernelError(RuntimeError):

@@ -550,7 +550,7 @@ CVMK_API int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_stream_
  * No scratch; launches may overlap where their results do not.  A token of -1 says that a bounded wait of
  * the kernel ran out (the other results of that row are then not written).
  * ---------------------------------------------------------------------------------------------- */
-#define CVMK_SAMPLE_MAX_VOCAB (384 * 1024)
+#define CVMK_SAMPLE_MAX_VOCAB (320 * 1024)
 typedef struct {
   const int32_t* logits;
   int64_t pitch;

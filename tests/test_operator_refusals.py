@@ -70,7 +70,7 @@ def sample(kn, **change):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(rows=-1), "sizes"), (dict(vocab=0), "sizes"), (dict(vocab=384 * 1024 + 1), "sizes"), (dict(table_len=0), "sizes"),
+    (dict(rows=-1), "sizes"), (dict(vocab=0), "sizes"), (dict(vocab=320 * 1024 + 1), "sizes"), (dict(table_len=0), "sizes"),
     (dict(pitch=99), "bad pitch"), (dict(pitch=-5), "bad pitch"), (dict(pitch=1 << 41), "bad pitch"),
     (dict(logits=0), "null operand"), (dict(table=0), "null operand"), (dict(scale=0), "null operand"), (dict(random=0), "null operand"),
     (dict(token=0), "null operand"),

@@ -82,7 +82,7 @@ def test_counts_of_rows(kn, rows):
     run(kn, logits(rng, rows, 3001, "normal"), EXP, rng.randint(10000, 60000, rows), rng.randint(0, 2**31, rows), **settings(rng, rows))
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 393216), (2, 300000), (2, 131072), (1, 50021), (30, 32000), (160, 70003)])
+@pytest.mark.parametrize("rows,vocab", [(1, 327680), (2, 300000), (2, 131072), (1, 50021), (30, 32000), (160, 70003)])
 def test_large_vocabularies(kn, rows, vocab):
     rng = np.random.RandomState(vocab)
     few = min(rows, 6)   # (the definition in Python takes a second a row: the rows behind are the first ones again)
