@@ -10,8 +10,9 @@
 //   top_p   An element's weight is a function of its table index, so the elements of every index are counted; the running
 //           sum of count * weight gives the index in which the share is reached and how many of its elements are needed, and
 //           the cut among those is one by count again.
-//   A cut by count, or by weight on a list, is found digit by digit: a histogram of the next ten bits of d over the elements
-//   that share the bits before, and the bin in which the running count or weight reaches the target.
+//   A cut by count is found digit by digit: a histogram of the next twelve bits of d over the elements that share the bits
+//   before, and the bin in which the running count reaches the target.  (With a table too long for shared memory top_p goes
+//   that way too, by weight.)
 // The draw then sums the weights in blocks of 512 elements, finds the block, and looks up the element in it.
 // Counts and weights are whole numbers, so their order of summation changes nothing.
 #include <cuda_runtime.h>
@@ -21,9 +22,11 @@ namespace cvmk {
 namespace {
 
 constexpr int MAX_WARPS = 32;
-constexpr int DIGIT = 10, BINS = 1 << DIGIT;
+constexpr int DIGIT = 12, BINS = 1 << DIGIT;       // of counts
+constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bin
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
 constexpr int LIST = 1024, ALL = 2048;  // elements on a CTA's list, on a cluster's
+constexpr int MAX_SPLIT = 8;
 constexpr int BLOCK = 512, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / 8 / BLOCK + 2;
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr uint64_t ONE = 1u << 30;
@@ -66,6 +69,37 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {   // inclusive
   return v;
 }
 
+__device__ __forceinline__ uint4 load128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// The sums over the cluster of four words at p.  A word of another CTA takes a fifth of a microsecond to come: four requests
+// are under way at a time.
+__device__ __forceinline__ uint4 sum_of_cluster(const uint32_t* p, uint32_t split) {
+  if (split == 1) return *reinterpret_cast<const uint4*>(p);
+  uint4 sum = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int c0 = 0; c0 < MAX_SPLIT; c0 += 4) {
+    if (c0 >= (int)split) break;
+    uint4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = c0 + c < (int)split ? load128(remote(p, (uint32_t)(c0 + c))) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) { sum.x += v[c].x; sum.y += v[c].y; sum.z += v[c].z; sum.w += v[c].w; }
+  }
+  return sum;
+}
+
+// The same where the sums may not fit 32 bits.
+__device__ __forceinline__ void sum_of_cluster(const uint32_t* p, uint32_t split, uint64_t (&sum)[4]) {
+  sum[0] = sum[1] = sum[2] = sum[3] = 0;
+  for (uint32_t c = 0; c < split; ++c) {
+    const uint4 v = split > 1 ? load128(remote(p, c)) : *reinterpret_cast<const uint4*>(p);
+    sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+  }
+}
+
 // The elements in front of a cut: all with d < D and the first `ties`, in index order, with d = D.
 struct Cut {
   uint64_t D;
@@ -73,20 +107,21 @@ struct Cut {
 };
 
 struct Shared {
-  uint32_t hist[4 * BINS];     // counts by table index; or [buffer][low 16 bits and rest of a weight | count, -][bin]
+  alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 16 bits, and the rest
   uint64_t scan[MAX_WARPS];
   int32_t lo[MAX_WARPS], hi[MAX_WARPS];
   uint32_t kept[MAX_WARPS];
   uint64_t block_mass[MAX_BLOCKS];
   uint32_t block_ties[MAX_BLOCKS];
-  int32_t list[LIST], all[ALL];
+  alignas(16) int32_t list[LIST];
+  alignas(16) int32_t all[ALL];
   uint32_t listed;
   // read by the other CTAs
   int32_t slice_lo, slice_hi, slice_bound;
   uint32_t late;               // the slice has not arrived
   uint64_t cta_mass;
   uint32_t cta_ties, cta_kept;
-  uint64_t found_before, found_size, found_count, total;
+  uint64_t found_before, found_size;
   int found;
   uint64_t bar;
 };
@@ -121,15 +156,23 @@ struct Row {
     if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
   }
-  // Calls f(value, valid) for the places 4g .. 4g + 3 of group g.
+  // Calls f(value) for the thread's share of the valid elements: whole groups of four, and the ragged ends by a few threads.
   template <typename F>
-  __device__ __forceinline__ void group(int g, const F& f) const {
-    const int4 v = reinterpret_cast<const int4*>(x)[g];
-    const int j = 4 * g;
-    f(v.x, j >= first && j < last);
-    f(v.y, j + 1 >= first && j + 1 < last);
-    f(v.z, j + 2 >= first && j + 2 < last);
-    f(v.w, j + 3 >= first && j + 3 < last);
+  __device__ __forceinline__ void each(const F& f) const {
+    const int g0 = (first + 3) >> 2, g1 = last >> 2, tid = threadIdx.x;
+    if (g0 > g1) {   // (less than a group)
+      if (first + tid < last) f(x[first + tid]);
+      return;
+    }
+    for (int g = g0 + tid; g < g1; g += blockDim.x) {
+      const int4 v = reinterpret_cast<const int4*>(x)[g];
+      f(v.x);
+      f(v.y);
+      f(v.z);
+      f(v.w);
+    }
+    if (first + tid < 4 * g0) f(x[first + tid]);
+    if (4 * g1 + tid < last) f(x[4 * g1 + tid]);
   }
 };
 
@@ -145,67 +188,85 @@ __device__ __forceinline__ uint64_t block_scan(Shared& s, uint64_t v, uint64_t& 
   return __shfl_sync(FULL, sums - w, warp) + inc - v;
 }
 
-// One digit: the histogram of the count (or weight) of the elements with d < limit whose bits from `shift + bits` on are `prefix`.
-// The buffer alternates from call to call, so that one barrier a call is enough.
-template <bool WEIGHT>
-__device__ void histogram(const Row& r, Shared& s, int buffer, uint64_t limit, uint32_t prefix, int shift, int bits) {
-  uint32_t* h0 = s.hist + buffer * 2 * BINS;
-  uint32_t* h1 = h0 + BINS;
-  for (int i = threadIdx.x; i < BINS; i += blockDim.x) h0[i] = h1[i] = 0;
+// (no CTA still reads what was there: `r`, whose histogram it was)
+__device__ __forceinline__ void clear(const Row& r, uint32_t* hist) {
+  r.sync();
+  for (int i = threadIdx.x; i < BINS / 4; i += blockDim.x) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  for (int j0 = r.first & ~31; j0 < r.last; j0 += blockDim.x) {
-    const int j = j0 + (int)threadIdx.x;
-    bool in = j >= r.first && j < r.last;
-    uint32_t d = 0, w = 1;
-    if (in) {
-      d = r.dist(r.x[j]);
-      in = d < limit && ((uint64_t)d >> (shift + bits)) == prefix;
-    }
-    if (WEIGHT && in) {
-      w = r.weight(d);
-      in = w > 0;
-    }
-    const uint32_t bin = (d >> shift) & ((1u << bits) - 1u);
-    const uint32_t mask = __ballot_sync(FULL, in);
-    if (in) {
-      int same;
-      __match_all_sync(mask, bin, &same);
-      if (same) {   // one bin for the whole warp
-        const uint32_t a = WEIGHT ? __reduce_add_sync(mask, w & 0xffffu) : (uint32_t)__popc(mask);
-        const uint32_t b = WEIGHT ? __reduce_add_sync(mask, w >> 16) : 0u;
-        if (lane == __ffs(mask) - 1) {
-          atomicAdd(&h0[bin], a);
-          if (WEIGHT && b) atomicAdd(&h1[bin], b);
+}
+// The cut that leaves `need` of the elements with from <= d < to (there are as many), and all in front of them.
+__device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t from, uint64_t to) {
+  const uint32_t span = (uint32_t)(to - 1 - from), base = (uint32_t)from;   // (distances are 32 bits wide, `to` may be 2^32)
+  const int all_bits = max(1, 32 - __clz((int)span));
+  int bits = min(all_bits, DIGIT), shift = all_bits - bits;
+  uint32_t prefix = 0;
+  while (true) {
+    uint32_t* const hist = s.hist;
+    clear(r, hist);
+    r.each([&](int32_t v) {
+      const uint32_t d = r.dist(v) - base;
+      if (r.dist(v) >= base && d <= span && (uint64_t)d >> (shift + bits) == prefix) atomicAdd(&hist[(d >> shift) & (BINS - 1)], 1u);
+    });
+    r.sync();
+    const int per = BINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // four or eight bins a thread
+    uint32_t own[8];
+    const uint4 a = sum_of_cluster(hist + bin0, r.split), b = per > 4 ? sum_of_cluster(hist + bin0 + 4, r.split) : make_uint4(0, 0, 0, 0);
+    own[0] = a.x; own[1] = a.y; own[2] = a.z; own[3] = a.w; own[4] = b.x; own[5] = b.y; own[6] = b.z; own[7] = b.w;
+    uint64_t sum = 0, total;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += own[k];
+    uint64_t before = block_scan(s, sum, total);
+    if (before < need && need <= before + sum) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (before < need && need <= before + own[k]) {
+          s.found = bin0 + k;
+          s.found_before = before;
+          s.found_size = own[k];
         }
-      } else {
-        atomicAdd(&h0[bin], WEIGHT ? w & 0xffffu : 1u);
-        if (WEIGHT && w >> 16) atomicAdd(&h1[bin], w >> 16);
+        before += own[k];
       }
     }
+    __syncthreads();
+    need -= s.found_before;
+    prefix = (prefix << bits) | (uint32_t)s.found;
+    if (need == s.found_size) return {min(from + (((uint64_t)prefix + 1) << shift), to), 0};   // all of the bin
+    if (shift == 0) return {from + prefix, (uint32_t)need};
+    bits = min(shift, DIGIT);
+    shift -= bits;
   }
-  r.sync();
 }
 
-// Where, in the order of d, the count (or the weight) of the elements with d < limit reaches need(total); if the total is
-// less than that, a cut among the ties of `whole`, of tie_weight each.
-template <bool WEIGHT, typename Need>
-__device__ Cut find_cut(const Row& r, Shared& s, int& buffer, uint64_t limit, int range_bits, const Need& need_of, const Cut& whole, uint32_t tie_weight) {
-  int bits = min(range_bits, DIGIT), shift = range_bits - bits;
+// Where, in the order of d, the weight of the elements with d < limit reaches need(total); if the total is less than that, a
+// cut among the ties of `whole`, of tie_weight each.
+template <typename Need>
+__device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need& need_of, const Cut& whole, uint32_t tie_weight) {
+  int bits = min(range_bits, WDIGIT), shift = range_bits - bits;
   uint32_t prefix = 0;
   uint64_t need = 0;
   for (bool first = true;; first = false) {
-    histogram<WEIGHT>(r, s, buffer, limit, prefix, shift, bits);
-    const uint32_t* h0 = s.hist + buffer * 2 * BINS;
-    buffer ^= 1;
-    const int per = BINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // one or two bins a thread
-    uint64_t own[2] = {0, 0};
-    for (uint32_t c = 0; c < r.split; ++c)
-      for (int k = 0; k < per; ++k) {
-        own[k] += load32(remote(h0 + bin0 + k, r.split > 1 ? c : cluster_rank()));
-        if (WEIGHT) own[k] += (uint64_t)load32(remote(h0 + BINS + bin0 + k, r.split > 1 ? c : cluster_rank())) << 16;
+    uint32_t* const hist = s.hist;
+    clear(r, hist);
+    r.each([&](int32_t v) {
+      const uint32_t d = r.dist(v);
+      if (d < whole.D && (uint64_t)d >> (shift + bits) == prefix) {
+        const uint32_t w = r.weight(d), bin = (d >> shift) & ((1u << bits) - 1u);
+        if (w & 0xffffu) atomicAdd(&hist[bin], w & 0xffffu);
+        if (w >> 16) atomicAdd(&hist[WBINS + bin], w >> 16);
       }
-    uint64_t total, before = block_scan(s, own[0] + own[1], total);
+    });
+    r.sync();
+    const int per = WBINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // two or four bins a thread
+    uint64_t own[4], high[4];
+    sum_of_cluster(hist + (bin0 & ~3), r.split, own);
+    sum_of_cluster(hist + WBINS + (bin0 & ~3), r.split, high);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) own[k] += high[k] << 16;
+    if (per == 2) {
+      if (bin0 & 2) { own[0] = own[2]; own[1] = own[3]; }
+      own[2] = own[3] = 0;
+    }
+    uint64_t total, before = block_scan(s, own[0] + own[1] + own[2] + own[3], total);
     if (first) {
       need = need_of(total);
       if (need > total) {
@@ -214,7 +275,8 @@ __device__ Cut find_cut(const Row& r, Shared& s, int& buffer, uint64_t limit, in
         return c;
       }
     }
-    for (int k = 0; k < per; ++k) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
       if (before < need && need <= before + own[k]) {
         s.found = bin0 + k;
         s.found_before = before;
@@ -223,49 +285,46 @@ __device__ Cut find_cut(const Row& r, Shared& s, int& buffer, uint64_t limit, in
       before += own[k];
     }
     __syncthreads();
-    const uint64_t rest = need - s.found_before, size = s.found_size;
+    need -= s.found_before;
     prefix = (prefix << bits) | (uint32_t)s.found;
-    __syncthreads();
-    Cut c;
-    if (rest == size) {   // all of the bin, as far as it lies in front of the limit
-      c.D = min(((uint64_t)prefix + 1) << shift, limit);
-      c.ties = 0;
-      return c;
-    }
+    if (need == s.found_size) return {min(((uint64_t)prefix + 1) << shift, whole.D), 0};   // all of the bin
     if (shift == 0) {
-      const uint32_t w = WEIGHT ? r.weight(prefix) : 1u;
-      c.D = prefix;
-      c.ties = (uint32_t)((rest + w - 1) / w);
-      return c;
+      const uint32_t w = r.weight(prefix);
+      return {prefix, (uint32_t)((need + w - 1) / w)};
     }
-    need = rest;
-    bits = min(shift, DIGIT);
+    bits = min(shift, WDIGIT);
     shift -= bits;
   }
 }
 
-// The elements for which take(d) holds, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are too many.
-template <typename Take>
-__device__ int collect(const Row& r, Shared& s, const Take& take) {
+// Puts the elements with from <= d < to, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are too many.
+__device__ int collect(const Row& r, Shared& s, uint64_t from, uint64_t to) {
+  const uint32_t span = (uint32_t)(to - 1 - from), base = (uint32_t)from;
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  for (int g = (r.first >> 2) + (int)threadIdx.x; 4 * g < r.last; g += blockDim.x)
-    r.group(g, [&](int32_t v, bool valid) {
-      if (valid && take(r.dist(v))) {
-        const uint32_t at = atomicAdd(&s.listed, 1u);
-        if (at < LIST) s.list[at] = v;
-      }
-    });
+  r.each([&](int32_t v) {
+    const uint32_t d = r.dist(v);
+    if (d >= base && d - base <= span) {
+      const uint32_t at = atomicAdd(&s.listed, 1u);
+      if (at < LIST) s.list[at] = v;
+    }
+  });
   r.sync();
-  uint32_t n = 0;
-  bool fits = true;
-  for (uint32_t c = 0; c < r.split; ++c) {
-    const uint32_t m = r.split > 1 ? load32(remote(&s.listed, c)) : s.listed;
-    fits = fits && m <= LIST && n + m <= ALL;
-    if (fits)
-      for (uint32_t i = threadIdx.x; i < m; i += blockDim.x) s.all[n + i] = r.split > 1 ? (int32_t)load32(remote(&s.list[i], c)) : s.list[i];
-    n += m;
+  if (r.split == 1) {
+    const int n = (int)s.listed;
+    if (n <= LIST)
+      for (int i = threadIdx.x; i < n; i += blockDim.x) s.all[i] = s.list[i];
+    __syncthreads();
+    return n <= LIST ? n : -1;
   }
+  // (a warp for every CTA's list)
+  const int lane = threadIdx.x & 31;
+  const uint32_t mine = lane < (int)r.split ? load32(remote(&s.listed, (uint32_t)lane)) : 0u;
+  const uint32_t sums = (uint32_t)warp_scan(mine), n = __shfl_sync(FULL, sums, 31);
+  const bool fits = !__any_sync(FULL, mine > LIST) && n <= ALL;
+  const uint32_t c = threadIdx.x >> 5, count = __shfl_sync(FULL, mine, (int)(c & 31)), at = __shfl_sync(FULL, sums - mine, (int)(c & 31));
+  if (fits && c < r.split)
+    for (uint32_t i = lane; i < count; i += 32) s.all[at + i] = (int32_t)load32(remote(&s.list[i], c));
   __syncthreads();
   return fits ? (int)n : -1;
 }
@@ -340,13 +399,10 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 
   // ---- the largest and the smallest score, and the bound of the k-th largest
   int32_t lo = INT32_MAX, hi = INT32_MIN;
-  for (int g = (r.first >> 2) + tid; 4 * g < r.last; g += threads)
-    r.group(g, [&](int32_t v, bool valid) {
-      if (valid) {
-        lo = min(lo, v);
-        hi = max(hi, v);
-      }
-    });
+  r.each([&](int32_t v) {
+    lo = min(lo, v);
+    hi = max(hi, v);
+  });
   const bool some = lo <= hi;   // the thread has seen an element
   const int32_t mine = hi;
   lo = __reduce_min_sync(FULL, lo);
@@ -365,10 +421,15 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     if (some) atomicAdd(&s.hist[((uint32_t)hi - (uint32_t)mine) >> shift], 1u);
     __syncthreads();
     const int per = BINS / threads, bin0 = per * tid;
-    const uint32_t n0 = s.hist[bin0], n1 = per > 1 ? s.hist[bin0 + 1] : 0;
-    uint64_t total;
-    const uint64_t before = block_scan(s, n0 + n1, total), need = (uint64_t)k;
-    if (before < need && need <= before + n0 + n1) s.found = need <= before + n0 ? bin0 : bin0 + 1;
+    uint32_t sum = 0;
+    for (int i = 0; i < per; ++i) sum += s.hist[bin0 + i];
+    uint64_t total, before = block_scan(s, sum, total);
+    const uint64_t need = (uint64_t)k;
+    if (before < need && need <= before + sum)
+      for (int i = 0; i < per; ++i) {
+        if (before < need && need <= before + s.hist[bin0 + i]) s.found = bin0 + i;
+        before += s.hist[bin0 + i];
+      }
     __syncthreads();
     if (s.found >= 0) {
       const int64_t b = (int64_t)hi - ((((int64_t)s.found + 1) << shift) - 1);
@@ -377,12 +438,15 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   }
   if (tid == 0) { s.slice_lo = lo; s.slice_hi = hi; s.slice_bound = bound; s.late = landed ? 0u : 1u; }
   r.sync();
-  uint32_t late = s.late;
-  for (int c = 0; p.split > 1 && c < p.split; ++c) {
-    late |= load32(remote(&s.late, (uint32_t)c));
-    lo = min(lo, (int32_t)load32(remote(&s.slice_lo, (uint32_t)c)));
-    hi = max(hi, (int32_t)load32(remote(&s.slice_hi, (uint32_t)c)));
-    bound = max(bound, (int32_t)load32(remote(&s.slice_bound, (uint32_t)c)));
+  bool late = s.late != 0;
+  if (p.split > 1) {   // (a lane for every CTA)
+    const uint32_t c = (uint32_t)min(lane, p.split - 1);
+    const uint32_t l = load32(remote(&s.late, c));
+    const int32_t a = (int32_t)load32(remote(&s.slice_lo, c)), b = (int32_t)load32(remote(&s.slice_hi, c)), e = (int32_t)load32(remote(&s.slice_bound, c));
+    late = __any_sync(FULL, l != 0);
+    lo = __reduce_min_sync(FULL, a);
+    hi = __reduce_max_sync(FULL, b);
+    bound = __reduce_max_sync(FULL, e);
   }
   if (late) {   // a copy that never came (its wait is bounded): no element is drawn
     if (rank == 0 && tid == 0) d.token[row] = -1;
@@ -395,89 +459,91 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   const int range_bits = bits_of((uint32_t)hi - (uint32_t)lo);
 
   // ---- the cuts
-  Cut cut = {(uint64_t)1 << 32, 0};   // everything
-  int buffer = 0;
-  const Cut everything = cut;
-  // The cut that leaves `count` elements, all of them with from <= d < to except `known` ones in front of `from`.
-  auto cut_by_count = [&](uint64_t count, uint64_t known, uint64_t from, uint64_t to, Row* list) {
-    const int n = collect(r, s, [&](uint32_t dj) { return dj >= from && dj < to; });
-    if (n < 0) return find_cut<false>(r, s, buffer, everything.D, range_bits, [=](uint64_t) { return count; }, everything, 0u);
-    list->x = s.all;
-    list->first = 0;
-    list->last = n;
-    list->split = 1;
-    Row near = *list;
-    near.top = (int32_t)((uint32_t)r.top - (uint32_t)from);
-    Cut c = find_cut<false>(near, s, buffer, to - from, bits_of(min(to - 1 - from, (uint64_t)0xffffffffu)), [=](uint64_t) { return count - known; }, everything, 0u);
-    c.D += from;
-    return c;
+  const uint64_t end = (uint64_t)1 << 32;
+  Cut cut = {end, 0};   // everything
+  // What the cuts look at instead of the row: a list that holds all that the last one has left, and more.
+  Row list = r;
+  auto look_at_list = [&](int n) {
+    list.x = s.all;
+    list.first = 0;
+    list.last = n;
+    list.split = 1;
   };
-  Row list = r;   // what find_cut may look at instead of the row: a list that holds everything in front of the cut
-  if (by_count) cut = cut_by_count((uint64_t)k, 0, 0, (uint64_t)r.dist(bound) + 1, &list);
+  if (by_count) {
+    const uint64_t to = (uint64_t)r.dist(bound) + 1;
+    const int n = collect(r, s, 0, to);
+    if (n >= 0) look_at_list(n);
+    cut = cut_by_count(list, s, (uint64_t)k, 0, n >= 0 ? to : (uint64_t)r.dist(lo) + 1);
+  }
   if (top_p < ONE) {
     const auto share_of = [=](uint64_t all) {
       const uint64_t need = top_p * (all >> 30) + ((top_p * (all & (ONE - 1)) + ONE - 1) >> 30);
       return need > 1 ? need : (uint64_t)1;
     };
-    if (by_count || r.wide) {
+    if (r.wide) {
       const uint32_t w = cut.ties ? r.weight((uint32_t)cut.D) : 0u, ties = cut.ties;
-      cut = find_cut<true>(list, s, buffer, cut.D, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
+      cut = cut_by_weight(list, s, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
     } else {
-      const uint32_t entries = (uint32_t)d.table_len;
-      for (uint32_t i = tid; i < 4 * BINS; i += threads) s.hist[i] = 0;
+      // the elements that are left, by table entry
+      uint32_t* const hist = s.hist;
+      clear(list, hist);
       if (tid == 0) s.found = -1;
-      __syncthreads();
-      uint32_t last = 0;   // (elements far behind the first: one counter, kept in registers)
-      for (int g = (r.first >> 2) + tid; 4 * g < r.last; g += threads)
-        r.group(g, [&](int32_t v, bool valid) {
-          const uint32_t e = r.entry(r.dist(v));
-          if (valid) {
-            if (e == r.last_entry) ++last;
-            else atomicAdd(&s.hist[e], 1u);
-          }
-        });
+      uint32_t last = 0;   // (of the last entry, which elements far behind the first one share: counted in registers)
+      const uint32_t left = (uint32_t)min(cut.D, end - 1);
+      const bool beyond = cut.D == end;
+      list.each([&](int32_t v) {
+        const uint32_t dj = list.dist(v), e = list.entry(dj);
+        if (beyond || dj < left) {
+          if (e == list.last_entry) ++last;
+          else atomicAdd(&hist[e], 1u);
+        }
+      });
       last = __reduce_add_sync(FULL, last);
-      if (lane == 0 && last) atomicAdd(&s.hist[r.last_entry], last);
-      r.sync();
-      const int per = 4 * BINS / threads;   // four or eight entries a thread
+      if (lane == 0 && last) atomicAdd(&hist[list.last_entry], last);
+      if (tid == 0 && cut.ties && (list.split == 1 || rank == 0)) atomicAdd(&hist[list.entry((uint32_t)cut.D)], cut.ties);
+      list.sync();
+      const int per = BINS / threads;   // four or eight entries a thread
       const uint32_t e0 = (uint32_t)(per * tid);
-      uint32_t n[8];
-      uint64_t count = 0, mass = 0;
+      const uint4 a = sum_of_cluster(hist + e0, list.split), b = per > 4 ? sum_of_cluster(hist + e0 + 4, list.split) : make_uint4(0, 0, 0, 0);
+      const uint32_t n[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      uint64_t mass = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        n[i] = 0;
-        if (i >= per || e0 + i >= entries) continue;
-        for (uint32_t c = 0; c < r.split; ++c) n[i] += r.split > 1 ? load32(remote(&s.hist[e0 + i], c)) : s.hist[e0 + i];
-        count += n[i];
-        mass += (uint64_t)n[i] * (uint32_t)table_s[e0 + i];
+        if (n[i]) mass += (uint64_t)n[i] * (uint32_t)table_s[e0 + i];   // (entries behind the table are not counted)
       }
-      uint64_t all, elements;
-      uint64_t before = block_scan(s, mass, all), in_front = block_scan(s, count, elements);
+      uint64_t all, before = block_scan(s, mass, all);
       const uint64_t need = share_of(all);
       if (before < need && need <= before + mass) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (i >= per || e0 + i >= entries) continue;
+          if (!n[i]) continue;
           const uint64_t w = (uint32_t)table_s[e0 + i], here = n[i] * w;
           if (before < need && need <= before + here) {
             s.found = (int)(e0 + i);
             s.found_before = (need - before + w - 1) / w;   // elements of this entry that are needed
             s.found_size = n[i];
-            s.found_count = in_front;
           }
           before += here;
-          in_front += n[i];
         }
       }
       __syncthreads();
       const int e = s.found;
-      const uint64_t wanted = s.found_before, size = s.found_size, front = s.found_count;
+      const uint64_t wanted = s.found_before, size = s.found_size;
       __syncthreads();
       if (e >= 0) {   // (else nothing weighs anything, and no cut is needed)
-        const uint64_t from = r.first_of((uint32_t)e), to = (uint32_t)e == r.last_entry ? everything.D : r.first_of((uint32_t)e + 1);
-        if (wanted == size) cut = {to, 0};
-        else if (to - from == 1) cut = {from, (uint32_t)wanted};
-        else cut = cut_by_count(front + wanted, front, from, to, &list);
+        const uint64_t from = r.first_of((uint32_t)e);
+        const uint64_t to = min((uint32_t)e == r.last_entry ? end : r.first_of((uint32_t)e + 1), cut.D + (cut.ties ? 1 : 0));
+        if (wanted < size && to - from == 1) {
+          cut = {from, (uint32_t)wanted};
+        } else if (wanted < size) {
+          if (list.split > 1 || !by_count) {
+            const int m = collect(r, s, from, to);
+            if (m >= 0) look_at_list(m);
+          }
+          cut = cut_by_count(list, s, wanted, from, to);
+        } else if (to <= cut.D) {   // (all of the entry; the cut that was there may lie in it)
+          cut = {to, 0};
+        }
       }
     }
   }
@@ -486,32 +552,41 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   uint32_t tie_weight = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
   const int blocks = (r.last + BLOCK - 1) / BLOCK;
   uint32_t kept = 0;
-  const uint32_t D32 = (uint32_t)min(cut.D, (uint64_t)0xffffffffu);
-  const bool beyond = cut.D > 0xffffffffu;
+  const uint32_t D32 = (uint32_t)min(cut.D, end - 1);
+  const bool beyond = cut.D == end;
   for (int b = warp; b < blocks; b += warps) {
-    uint32_t low = 0, high = 0, ties = 0;
+    const bool whole = b * BLOCK >= r.first && (b + 1) * BLOCK <= r.last;
+    const int4* const at4 = reinterpret_cast<const int4*>(x) + b * (BLOCK / 4) + lane;
+    uint64_t mass = 0;
+    uint32_t ties = 0;
 #pragma unroll
     for (int i = 0; i < BLOCK / 128; ++i) {
-      const int g = b * (BLOCK / 4) + i * 32 + lane;
-      if (4 * g >= r.last) break;
-      r.group(g, [&](int32_t v, bool valid) {
-        const uint32_t dj = r.dist(v);
-        if (valid && (dj < D32 || beyond)) {
-          const uint32_t w = r.weight(dj);
-          low += w & 0xffffu;
-          high += w >> 16;
-          kept += w > 0;
-        } else {
-          ties += valid && dj == D32;
+      const int j = b * BLOCK + 4 * (i * 32 + lane);
+      const int4 v = whole || j < r.last ? at4[i * 32] : make_int4(0, 0, 0, 0);
+      const int32_t e[4] = {v.x, v.y, v.z, v.w};
+      uint32_t dj[4];
+      bool in[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool valid = whole || (j + q >= r.first && j + q < r.last);
+        dj[q] = r.dist(e[q]);
+        in[q] = valid && (beyond || dj[q] < D32);
+        ties += valid && !beyond && dj[q] == D32;
+      }
+      if (__any_sync(FULL, in[0] || in[1] || in[2] || in[3])) {   // (behind a cut hardly any)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t w = in[q] ? r.weight(dj[q]) : 0u;
+          mass += w;
+          kept += min(w, 1u);
         }
-      });
+      }
     }
-    __syncwarp();
-    low = __reduce_add_sync(FULL, low);
-    high = __reduce_add_sync(FULL, high);
+    // a lane's sum is below 2^35
+    const uint32_t low = __reduce_add_sync(FULL, (uint32_t)mass & 0xfffffu), high = __reduce_add_sync(FULL, (uint32_t)(mass >> 20));
     ties = __reduce_add_sync(FULL, ties);
     if (lane == 0) {
-      s.block_mass[b] = low + ((uint64_t)high << 16);
+      s.block_mass[b] = low + ((uint64_t)high << 20);
       s.block_ties[b] = ties;
     }
   }
@@ -537,15 +612,20 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     if (lane == 0) s.cta_kept = kept;
   }
   r.sync();
-  uint64_t all = 0, front_mass = 0;
-  uint32_t front_ties = 0, all_kept = cut.ties && tie_weight ? cut.ties : 0;
-  for (int c = 0; c < p.split; ++c) {
-    const uint64_t m = p.split > 1 ? load64(remote(&s.cta_mass, (uint32_t)c)) : s.cta_mass;
-    const uint32_t t = p.split > 1 ? load32(remote(&s.cta_ties, (uint32_t)c)) : s.cta_ties;
-    all_kept += p.split > 1 ? load32(remote(&s.cta_kept, (uint32_t)c)) : s.cta_kept;
-    all += m;
-    if (c < rank) { front_mass += m; front_ties += t; }
+  uint64_t all = s.cta_mass, front_mass = 0;
+  uint32_t front_ties = 0, all_kept = s.cta_kept;
+  if (p.split > 1) {   // (a lane for every CTA)
+    const uint32_t c = (uint32_t)min(lane, p.split - 1);
+    const uint64_t m = load64(remote(&s.cta_mass, c));
+    const uint32_t t = load32(remote(&s.cta_ties, c)), n = load32(remote(&s.cta_kept, c));
+    const uint64_t sums = warp_scan(lane < p.split ? m : 0);
+    const uint32_t tie_sums = (uint32_t)warp_scan(lane < p.split ? t : 0);
+    all = __shfl_sync(FULL, sums, 31);
+    all_kept = __reduce_add_sync(FULL, lane < p.split ? n : 0u);
+    front_mass = __shfl_sync(FULL, sums - (lane < p.split ? m : 0), rank);
+    front_ties = __shfl_sync(FULL, tie_sums - (lane < p.split ? t : 0), rank);
   }
+  if (cut.ties && tie_weight) all_kept += cut.ties;
   all += (uint64_t)cut.ties * tie_weight;
   const uint64_t target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
   if (all == 0) {
@@ -556,10 +636,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     r.sync();   // (nobody still reads the sums of before)
     for (int b = warp; b < blocks; b += warps) {
       uint32_t ties = 0;
-      for (int i = 0; i < BLOCK / 128; ++i) {
-        const int g = b * (BLOCK / 4) + i * 32 + lane;
-        if (4 * g < r.last) r.group(g, [&](int32_t v, bool valid) { ties += valid && r.dist(v) == 0; });
-      }
+      for (int j = max(b * BLOCK, r.first & ~31) + lane; j < min((b + 1) * BLOCK, r.last); j += 32) ties += j >= r.first && r.dist(x[j]) == 0;
       __syncwarp();
       ties = __reduce_add_sync(FULL, ties);
       if (lane == 0) { s.block_mass[b] = 0; s.block_ties[b] = ties; }
@@ -594,17 +671,13 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       m = __shfl_sync(FULL, m, from);
       t = __shfl_sync(FULL, t, from);
       // sixteen elements a lane
-      const int g0 = b * (BLOCK / 4) + lane * (BLOCK / 128);
+      const int first = max(b * BLOCK + lane * (BLOCK / 32), r.first), last = min(b * BLOCK + (lane + 1) * (BLOCK / 32), r.last);
       uint64_t mass = 0;
       uint32_t ties = 0;
       const auto each = [&](const auto& f) {   // f(place, weight, tie) for the lane's elements
-        for (int i = 0; i < BLOCK / 128; ++i) {
-          int j = 4 * (g0 + i);
-          if (j >= r.last) break;
-          r.group(g0 + i, [&](int32_t v, bool valid) {
-            const uint32_t dj = r.dist(v);
-            f(j++, valid && dj < cut.D ? r.weight(dj) : 0u, valid && dj == cut.D ? 1u : 0u);
-          });
+        for (int j = first; j < last; ++j) {
+          const uint32_t dj = r.dist(x[j]);
+          f(j, dj < cut.D ? r.weight(dj) : 0u, dj == cut.D ? 1u : 0u);
         }
       };
       each([&](int, uint32_t w, uint32_t tie) { mass += w; ties += tie; });
