@@ -4,9 +4,10 @@
 // shared memory; every later pass over it reads it there.  What is left of a row after its filters is all elements with
 // d = max - x < D and the first `ties` ones, in index order, with d = D: the filters only look for that cut, and neither sort
 // nor list the row.
-//   top_k   In a CTA, the k-th largest of the maxima of its threads is a lower bound of its k-th largest element (that many
-//           threads have one as large).  The elements not below the largest of the CTAs' bounds are few more than k; they are
-//           put on a list, and the cut is found on it.
+//   top_k   In a CTA, the n-th largest of the maxima of its threads is a lower bound of its n-th largest element (that many
+//           threads have one as large).  So the row's k-th is not below any CTA's bound for n = k, nor below the least of the
+//           bounds for n = k / CTAs.  The elements that are not below these are few more than k; they are put on a list, and
+//           the cut is found on it.
 //   top_p   An element's weight is a function of its table index, so the elements of every index are counted; the running
 //           sum of count * weight gives the index in which the share is reached and how many of its elements are needed, and
 //           the cut among those is one by count again.
@@ -27,7 +28,7 @@ constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bi
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
 constexpr int LIST = 1024, ALL = 2048;  // elements on a CTA's list, on a cluster's
 constexpr int MAX_SPLIT = 8;
-constexpr int BLOCK = 512, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / 8 / BLOCK + 2;
+constexpr int BLOCK = 512, GROUPS = BLOCK / 128, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / 8 / BLOCK + 2;
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr uint64_t ONE = 1u << 30;
 
@@ -117,12 +118,12 @@ struct Shared {
   alignas(16) int32_t all[ALL];
   uint32_t listed;
   // read by the other CTAs
-  int32_t slice_lo, slice_hi, slice_bound;
+  int32_t slice_lo, slice_hi, slice_bound, slice_share;
   uint32_t late;               // the slice has not arrived
   uint64_t cta_mass;
   uint32_t cta_ties, cta_kept;
   uint64_t found_before, found_size;
-  int found;
+  int found, found_share;
   uint64_t bar;
 };
 
@@ -164,7 +165,21 @@ struct Row {
       if (first + tid < last) f(x[first + tid]);
       return;
     }
-    for (int g = g0 + tid; g < g1; g += blockDim.x) {
+    const int step = blockDim.x;
+    int g = g0 + tid;
+    for (; g + 3 * step < g1; g += 4 * step) {   // (four requests under way)
+      int4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const int4*>(x)[g + i * step];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f(v[i].x);
+        f(v[i].y);
+        f(v[i].z);
+        f(v[i].w);
+      }
+    }
+    for (; g < g1; g += step) {
       const int4 v = reinterpret_cast<const int4*>(x)[g];
       f(v.x);
       f(v.y);
@@ -356,6 +371,11 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
+  // (what the set-up needs of global memory is requested at once: a trip each would be longer than the slice takes)
+  constexpr int EARLY = TABLE_SMEM_MAX / 512;
+  int32_t entry[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) entry[i] = p.table_smem && tid + i * threads < d.table_len ? d.table[tid + i * threads] : 0;
   // whole 16-byte words by the bulk engine, the ragged ends by threads
   const int b0 = min((r.first + 3) & ~3, r.last), b1 = max(b0, r.last & ~3);
   const int32_t* at = src - skew + begin;                 // of place 0
@@ -379,10 +399,11 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   r.min_weight = (uint32_t)((min_p * (uint64_t)max(d.table[0], 0) + ONE - 1) >> 30);
   r.wide = !p.table_smem;
   r.table = p.table_smem ? table_s : d.table;
-  if (p.table_smem)
-    for (int i = tid; i < d.table_len; i += threads) {
-      const int32_t w = max(d.table[i], 0);
-      table_s[i] = (uint32_t)w >= r.min_weight ? w : 0;
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+    if (p.table_smem && tid + i * threads < d.table_len) {
+      const int32_t w = max(entry[i], 0);
+      table_s[tid + i * threads] = (uint32_t)w >= r.min_weight ? w : 0;
     }
   __syncthreads();
   // (bounded: the copy is the only thing that is waited for)
@@ -412,10 +433,10 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   lo = __reduce_min_sync(FULL, lane < warps ? s.lo[lane] : INT32_MAX);
   hi = __reduce_max_sync(FULL, lane < warps ? s.hi[lane] : INT32_MIN);
   const bool by_count = k >= 1 && k < vocab;
-  int32_t bound = INT32_MIN;
-  if (by_count && k <= threads) {
+  int32_t bound = INT32_MIN, share = INT32_MIN;   // the bounds for n = k and n = k / CTAs
+  if (by_count && k <= p.split * threads) {
     for (int i = tid; i < BINS; i += threads) s.hist[i] = 0;
-    if (tid == 0) s.found = -1;
+    if (tid == 0) s.found = s.found_share = -1;
     __syncthreads();
     const int shift = max(0, bits_of((uint32_t)hi - (uint32_t)lo) - DIGIT);
     if (some) atomicAdd(&s.hist[((uint32_t)hi - (uint32_t)mine) >> shift], 1u);
@@ -424,29 +445,34 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     uint32_t sum = 0;
     for (int i = 0; i < per; ++i) sum += s.hist[bin0 + i];
     uint64_t total, before = block_scan(s, sum, total);
-    const uint64_t need = (uint64_t)k;
-    if (before < need && need <= before + sum)
+    const uint64_t need = (uint64_t)k, part = (uint64_t)((k + p.split - 1) / p.split);
+    if (sum)
       for (int i = 0; i < per; ++i) {
-        if (before < need && need <= before + s.hist[bin0 + i]) s.found = bin0 + i;
-        before += s.hist[bin0 + i];
+        const uint64_t after = before + s.hist[bin0 + i];
+        if (before < need && need <= after) s.found = bin0 + i;
+        if (before < part && part <= after) s.found_share = bin0 + i;
+        before = after;
       }
     __syncthreads();
-    if (s.found >= 0) {
-      const int64_t b = (int64_t)hi - ((((int64_t)s.found + 1) << shift) - 1);
-      bound = b > INT32_MIN ? (int32_t)b : INT32_MIN;
-    }
+    const auto least = [&](int bin) {   // what the maxima of this bin and of those before it are not below
+      const int64_t b = (int64_t)hi - ((((int64_t)bin + 1) << shift) - 1);
+      return bin >= 0 && b > INT32_MIN ? (int32_t)b : INT32_MIN;
+    };
+    bound = least(s.found);
+    share = least(s.found_share);
   }
-  if (tid == 0) { s.slice_lo = lo; s.slice_hi = hi; s.slice_bound = bound; s.late = landed ? 0u : 1u; }
+  if (tid == 0) { s.slice_lo = lo; s.slice_hi = hi; s.slice_bound = bound; s.slice_share = share; s.late = landed ? 0u : 1u; }
   r.sync();
   bool late = s.late != 0;
   if (p.split > 1) {   // (a lane for every CTA)
     const uint32_t c = (uint32_t)min(lane, p.split - 1);
     const uint32_t l = load32(remote(&s.late, c));
     const int32_t a = (int32_t)load32(remote(&s.slice_lo, c)), b = (int32_t)load32(remote(&s.slice_hi, c)), e = (int32_t)load32(remote(&s.slice_bound, c));
+    const int32_t f = (int32_t)load32(remote(&s.slice_share, c));
     late = __any_sync(FULL, l != 0);
     lo = __reduce_min_sync(FULL, a);
     hi = __reduce_max_sync(FULL, b);
-    bound = __reduce_max_sync(FULL, e);
+    bound = max(__reduce_max_sync(FULL, e), __reduce_min_sync(FULL, f));
   }
   if (late) {   // a copy that never came (its wait is bounded): no element is drawn
     if (rank == 0 && tid == 0) d.token[row] = -1;
@@ -556,32 +582,53 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   const bool beyond = cut.D == end;
   for (int b = warp; b < blocks; b += warps) {
     const bool whole = b * BLOCK >= r.first && (b + 1) * BLOCK <= r.last;
-    const int4* const at4 = reinterpret_cast<const int4*>(x) + b * (BLOCK / 4) + lane;
     uint64_t mass = 0;
     uint32_t ties = 0;
+    int4 v[GROUPS];
 #pragma unroll
-    for (int i = 0; i < BLOCK / 128; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
       const int j = b * BLOCK + 4 * (i * 32 + lane);
-      const int4 v = whole || j < r.last ? at4[i * 32] : make_int4(0, 0, 0, 0);
-      const int32_t e[4] = {v.x, v.y, v.z, v.w};
-      uint32_t dj[4];
-      bool in[4];
+      v[i] = j < r.last ? *reinterpret_cast<const int4*>(x + j) : make_int4(0, 0, 0, 0);
+    }
+    if (whole && beyond) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool valid = whole || (j + q >= r.first && j + q < r.last);
-        dj[q] = r.dist(e[q]);
-        in[q] = valid && (beyond || dj[q] < D32);
-        ties += valid && !beyond && dj[q] == D32;
+      for (int i = 0; i < GROUPS; ++i) {
+        const uint32_t w0 = r.weight(r.dist(v[i].x)), w1 = r.weight(r.dist(v[i].y)), w2 = r.weight(r.dist(v[i].z)), w3 = r.weight(r.dist(v[i].w));
+        mass += w0;
+        mass += w1;
+        mass += w2;
+        mass += w3;
+        kept += min(w0, 1u) + min(w1, 1u) + min(w2, 1u) + min(w3, 1u);
       }
-      if (__any_sync(FULL, in[0] || in[1] || in[2] || in[3])) {   // (behind a cut hardly any)
+    } else {
+      bool some_in = false;   // (behind a cut hardly any element is)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t w = in[q] ? r.weight(dj[q]) : 0u;
-          mass += w;
-          kept += min(w, 1u);
+      for (int i = 0; i < GROUPS; ++i) {
+        const int32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) some_in |= beyond || r.dist(e[q]) <= D32;
+      }
+      if (__any_sync(FULL, some_in)) {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+          const int j = b * BLOCK + 4 * (i * 32 + lane);
+          const int32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const bool valid = j + q >= r.first && j + q < r.last;
+            const uint32_t dj = r.dist(e[q]);
+            if (valid && (beyond || dj < D32)) {
+              const uint32_t w = r.weight(dj);
+              mass += w;
+              kept += min(w, 1u);
+            } else {
+              ties += valid && dj == D32;
+            }
+          }
         }
       }
     }
+    __syncwarp();
     // a lane's sum is below 2^35
     const uint32_t low = __reduce_add_sync(FULL, (uint32_t)mass & 0xfffffu), high = __reduce_add_sync(FULL, (uint32_t)(mass >> 20));
     ties = __reduce_add_sync(FULL, ties);
@@ -670,36 +717,53 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       const int b = __shfl_sync(FULL, hit, from);
       m = __shfl_sync(FULL, m, from);
       t = __shfl_sync(FULL, t, from);
-      // sixteen elements a lane
-      const int first = max(b * BLOCK + lane * (BLOCK / 32), r.first), last = min(b * BLOCK + (lane + 1) * (BLOCK / 32), r.last);
-      uint64_t mass = 0;
-      uint32_t ties = 0;
-      const auto each = [&](const auto& f) {   // f(place, weight, tie) for the lane's elements
-        for (int j = first; j < last; ++j) {
-          const uint32_t dj = r.dist(x[j]);
-          f(j, dj < cut.D ? r.weight(dj) : 0u, dj == cut.D ? 1u : 0u);
+      // its elements, four of every 128 a lane
+      uint32_t w[GROUPS][4], tie[GROUPS];
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        const int j = b * BLOCK + 4 * (i * 32 + lane);
+        const int4 v = j < r.last ? *reinterpret_cast<const int4*>(x + j) : make_int4(0, 0, 0, 0);
+        const int32_t e[4] = {v.x, v.y, v.z, v.w};
+        tie[i] = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool valid = j + q >= r.first && j + q < r.last;
+          const uint32_t dj = r.dist(e[q]);
+          w[i][q] = valid && dj < cut.D ? r.weight(dj) : 0u;
+          tie[i] |= (valid && dj == cut.D ? 1u : 0u) << q;
         }
-      };
-      each([&](int, uint32_t w, uint32_t tie) { mass += w; ties += tie; });
-      __syncwarp();
-      m += warp_scan(mass) - mass;
-      t += (uint32_t)(warp_scan(ties) - ties);
-      if (!passed(m, t) && passed(m + mass, t + ties)) {
-        int token = -1;
-        uint32_t weight = 0;
-        each([&](int j, uint32_t w, uint32_t tie) {
-          if (token >= 0) return;
-          m += w;
-          t += tie;
-          if (passed(m, t)) {
-            token = begin + j - skew;
-            weight = tie ? (all ? tie_weight : 0u) : w;
+      }
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        if (done) continue;
+        const uint64_t mine_mass = (uint64_t)w[i][0] + w[i][1] + w[i][2] + w[i][3];
+        const uint32_t mine_ties = (uint32_t)__popc(tie[i]);
+        const uint64_t mass_to = warp_scan(mine_mass);
+        const uint32_t ties_to = (uint32_t)warp_scan(mine_ties);
+        uint64_t m1 = m + mass_to - mine_mass;
+        uint32_t t1 = t + ties_to - mine_ties;
+        if (!passed(m1, t1) && passed(m1 + mine_mass, t1 + mine_ties)) {
+          int place = -1;
+          uint32_t weight = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t one_tie = tie[i] >> q & 1u;
+            m1 += w[i][q];
+            t1 += one_tie;
+            if (place < 0 && passed(m1, t1)) {
+              place = q;
+              weight = one_tie ? (all ? tie_weight : 0u) : w[i][q];
+            }
           }
-        });
-        d.token[row] = token;
-        if (d.weight) d.weight[row] = (int32_t)weight;
-        if (d.mass) d.mass[row] = (int64_t)all;
-        if (d.kept) d.kept[row] = (int32_t)all_kept;
+          d.token[row] = begin + b * BLOCK + 4 * (i * 32 + lane) + place - skew;
+          if (d.weight) d.weight[row] = (int32_t)weight;
+          if (d.mass) d.mass[row] = (int64_t)all;
+          if (d.kept) d.kept[row] = (int32_t)all_kept;
+        }
+        m += __shfl_sync(FULL, mass_to, 31);
+        t += __shfl_sync(FULL, ties_to, 31);
+        done = passed(m, t);
       }
     }
   }
