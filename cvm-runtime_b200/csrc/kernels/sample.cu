@@ -55,11 +55,6 @@ __device__ __forceinline__ uint32_t load32(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint64_t load64(uint32_t addr) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {   // inclusive
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -70,6 +65,10 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {   // inclusive
   return v;
 }
 
+__device__ __forceinline__ void store128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void store32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint4 load128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -117,11 +116,10 @@ struct Shared {
   alignas(16) int32_t list[LIST];
   alignas(16) int32_t all[ALL];
   uint32_t listed;
-  // read by the other CTAs
-  int32_t slice_lo, slice_hi, slice_bound, slice_share;
-  uint32_t late;               // the slice has not arrived
-  uint64_t cta_mass;
-  uint32_t cta_ties, cta_kept;
+  // what every CTA of the cluster says of its slice, sent here by it
+  alignas(16) int4 scores[MAX_SPLIT];     // smallest, largest, bounds
+  alignas(16) uint4 sums[MAX_SPLIT];      // weight (low, high), ties, kept
+  uint32_t late;                          // a slice has not arrived
   uint64_t found_before, found_size;
   int found, found_share;
   uint64_t bar;
@@ -137,6 +135,12 @@ struct Row {
   uint32_t min_weight;   // lighter elements are filtered out; 0 where the table has gone through that already
   uint32_t split;
   bool wide;             // the table lies in global memory
+  // entry() in fewer instructions where scale <= 2^16 and the table lies in shared memory: scores below floor_x have the last
+  // entry, as floor_x has, and above it (top - x) * scale is less than 2^31.
+  bool gentle;
+  int32_t floor_x;
+  uint32_t minus_scale, top_scaled;
+  __device__ __forceinline__ uint32_t entry_of(int32_t v) const { return ((uint32_t)max(v, floor_x) * minus_scale + top_scaled) >> 16; }
   __device__ __forceinline__ uint32_t dist(int32_t v) const { return (uint32_t)top - (uint32_t)v; }
   // min((d * scale) >> 16, last_entry): a table in shared memory has less than 2^15 entries, and every d above
   // saturated = (2^32 - 1) / scale has a product above 2^31.
@@ -367,9 +371,11 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 
   pdl_trigger();
   if (tid == 0) {
+    s.late = 0;
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&s.bar)));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for before anything is sent)
   pdl_wait();
   // (what the set-up needs of global memory is requested at once: a trip each would be longer than the slice takes)
   constexpr int EARLY = TABLE_SMEM_MAX / 512;
@@ -399,13 +405,15 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   r.min_weight = (uint32_t)((min_p * (uint64_t)max(d.table[0], 0) + ONE - 1) >> 30);
   r.wide = !p.table_smem;
   r.table = p.table_smem ? table_s : d.table;
+  bool plain = true;   // all entries are above 0 and below 2^27
 #pragma unroll
   for (int i = 0; i < EARLY; ++i)
     if (p.table_smem && tid + i * threads < d.table_len) {
-      const int32_t w = max(entry[i], 0);
-      table_s[tid + i * threads] = (uint32_t)w >= r.min_weight ? w : 0;
+      const int32_t w = (uint32_t)max(entry[i], 0) >= r.min_weight ? max(entry[i], 0) : 0;
+      table_s[tid + i * threads] = w;
+      plain = plain && w > 0 && w < 1 << 27;
     }
-  __syncthreads();
+  const bool plain_table = __syncthreads_and(plain) && p.table_smem;
   // (bounded: the copy is the only thing that is waited for)
   bool landed = false;
   for (uint32_t i = 0; !landed && i < (1u << 19); ++i) {
@@ -418,12 +426,20 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     landed = ok != 0;
   }
 
+  if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+
   // ---- the largest and the smallest score, and the bound of the k-th largest
   int32_t lo = INT32_MAX, hi = INT32_MIN;
-  r.each([&](int32_t v) {
-    lo = min(lo, v);
-    hi = max(hi, v);
-  });
+  const bool by_count = k >= 1 && k < vocab;
+  if (by_count || r.wide) {
+    r.each([&](int32_t v) {
+      lo = min(lo, v);
+      hi = max(hi, v);
+    });
+  } else {   // (the smallest is not asked for)
+    r.each([&](int32_t v) { hi = max(hi, v); });
+    lo = hi == INT32_MIN ? INT32_MAX : hi;
+  }
   const bool some = lo <= hi;   // the thread has seen an element
   const int32_t mine = hi;
   lo = __reduce_min_sync(FULL, lo);
@@ -432,7 +448,6 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   __syncthreads();
   lo = __reduce_min_sync(FULL, lane < warps ? s.lo[lane] : INT32_MAX);
   hi = __reduce_max_sync(FULL, lane < warps ? s.hi[lane] : INT32_MIN);
-  const bool by_count = k >= 1 && k < vocab;
   int32_t bound = INT32_MIN, share = INT32_MIN;   // the bounds for n = k and n = k / CTAs
   if (by_count && k <= p.split * threads) {
     for (int i = tid; i < BINS; i += threads) s.hist[i] = 0;
@@ -461,18 +476,17 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     bound = least(s.found);
     share = least(s.found_share);
   }
-  if (tid == 0) { s.slice_lo = lo; s.slice_hi = hi; s.slice_bound = bound; s.slice_share = share; s.late = landed ? 0u : 1u; }
+  if (warp == 0 && lane < p.split) {   // (a lane for every CTA)
+    store128(remote(&s.scores[rank], (uint32_t)lane), make_uint4((uint32_t)lo, (uint32_t)hi, (uint32_t)bound, (uint32_t)share));
+    if (!landed) store32(remote(&s.late, (uint32_t)lane), 1u);
+  }
   r.sync();
-  bool late = s.late != 0;
-  if (p.split > 1) {   // (a lane for every CTA)
-    const uint32_t c = (uint32_t)min(lane, p.split - 1);
-    const uint32_t l = load32(remote(&s.late, c));
-    const int32_t a = (int32_t)load32(remote(&s.slice_lo, c)), b = (int32_t)load32(remote(&s.slice_hi, c)), e = (int32_t)load32(remote(&s.slice_bound, c));
-    const int32_t f = (int32_t)load32(remote(&s.slice_share, c));
-    late = __any_sync(FULL, l != 0);
-    lo = __reduce_min_sync(FULL, a);
-    hi = __reduce_max_sync(FULL, b);
-    bound = max(__reduce_max_sync(FULL, e), __reduce_min_sync(FULL, f));
+  const bool late = s.late != 0;
+  {
+    const int4 v = s.scores[min(lane, p.split - 1)];
+    lo = __reduce_min_sync(FULL, v.x);
+    hi = __reduce_max_sync(FULL, v.y);
+    bound = max(__reduce_max_sync(FULL, v.z), __reduce_min_sync(FULL, v.w));
   }
   if (late) {   // a copy that never came (its wait is bounded): no element is drawn
     if (rank == 0 && tid == 0) d.token[row] = -1;
@@ -482,6 +496,10 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     return;
   }
   r.top = hi;
+  r.gentle = !r.wide && r.scale <= 65536;
+  r.floor_x = (int32_t)max((int64_t)hi - (int64_t)min(r.first_of(r.last_entry), (uint64_t)1 << 32), (int64_t)INT32_MIN);
+  r.minus_scale = 0u - r.scale;
+  r.top_scaled = (uint32_t)hi * r.scale;
   const int range_bits = bits_of((uint32_t)hi - (uint32_t)lo);
 
   // ---- the cuts
@@ -517,13 +535,21 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       uint32_t last = 0;   // (of the last entry, which elements far behind the first one share: counted in registers)
       const uint32_t left = (uint32_t)min(cut.D, end - 1);
       const bool beyond = cut.D == end;
-      list.each([&](int32_t v) {
-        const uint32_t dj = list.dist(v), e = list.entry(dj);
-        if (beyond || dj < left) {
+      if (beyond && list.gentle) {
+        list.each([&](int32_t v) {
+          const uint32_t e = list.entry_of(v);
           if (e == list.last_entry) ++last;
           else atomicAdd(&hist[e], 1u);
-        }
-      });
+        });
+      } else {
+        list.each([&](int32_t v) {
+          const uint32_t dj = list.dist(v), e = list.entry(dj);
+          if (beyond || dj < left) {
+            if (e == list.last_entry) ++last;
+            else atomicAdd(&hist[e], 1u);
+          }
+        });
+      }
       last = __reduce_add_sync(FULL, last);
       if (lane == 0 && last) atomicAdd(&hist[list.last_entry], last);
       if (tid == 0 && cut.ties && (list.split == 1 || rank == 0)) atomicAdd(&hist[list.entry((uint32_t)cut.D)], cut.ties);
@@ -590,7 +616,14 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       const int j = b * BLOCK + 4 * (i * 32 + lane);
       v[i] = j < r.last ? *reinterpret_cast<const int4*>(x + j) : make_int4(0, 0, 0, 0);
     }
-    if (whole && beyond) {
+    if (whole && beyond && r.gentle && plain_table) {   // (sixteen weights below 2^27 fit 32 bits)
+      uint32_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i)
+        sum += (uint32_t)(r.table[r.entry_of(v[i].x)] + r.table[r.entry_of(v[i].y)]) + (uint32_t)(r.table[r.entry_of(v[i].z)] + r.table[r.entry_of(v[i].w)]);
+      mass = sum;
+      kept += BLOCK / 32;
+    } else if (whole && beyond) {
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
         const uint32_t w0 = r.weight(r.dist(v[i].x)), w1 = r.weight(r.dist(v[i].y)), w2 = r.weight(r.dist(v[i].z)), w3 = r.weight(r.dist(v[i].w));
@@ -651,27 +684,26 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     const uint64_t mi = warp_scan(m), ti = warp_scan(t);
     mass_in_front = mi - m;
     ties_in_front = (uint32_t)(ti - t);
-    if (lane == 31) { s.cta_mass = mi; s.cta_ties = (uint32_t)ti; }
+    const uint64_t mass = __shfl_sync(FULL, mi, 31);
+    const uint32_t ties = __shfl_sync(FULL, (uint32_t)ti, 31);
+    if (lane < p.split) store128(remote(&s.sums[rank], (uint32_t)lane), make_uint4((uint32_t)mass, (uint32_t)(mass >> 32), ties, kept));
   };
   if (warp == 0) {
-    scan_blocks();
     kept = __reduce_add_sync(FULL, lane < warps ? s.kept[lane] : 0u);
-    if (lane == 0) s.cta_kept = kept;
+    scan_blocks();
   }
   r.sync();
-  uint64_t all = s.cta_mass, front_mass = 0;
-  uint32_t front_ties = 0, all_kept = s.cta_kept;
-  if (p.split > 1) {   // (a lane for every CTA)
-    const uint32_t c = (uint32_t)min(lane, p.split - 1);
-    const uint64_t m = load64(remote(&s.cta_mass, c));
-    const uint32_t t = load32(remote(&s.cta_ties, c)), n = load32(remote(&s.cta_kept, c));
-    const uint64_t sums = warp_scan(lane < p.split ? m : 0);
-    const uint32_t tie_sums = (uint32_t)warp_scan(lane < p.split ? t : 0);
-    all = __shfl_sync(FULL, sums, 31);
-    all_kept = __reduce_add_sync(FULL, lane < p.split ? n : 0u);
-    front_mass = __shfl_sync(FULL, sums - (lane < p.split ? m : 0), rank);
-    front_ties = __shfl_sync(FULL, tie_sums - (lane < p.split ? t : 0), rank);
-  }
+  uint64_t all, front_mass;
+  uint32_t front_ties, all_kept;
+  auto add_up = [&]() {   // over the CTAs, and over those in front of this one
+    const uint4 v = lane < p.split ? s.sums[lane] : make_uint4(0, 0, 0, 0);
+    const uint64_t m = v.x | (uint64_t)v.y << 32, mass = warp_scan(m), ties = warp_scan(v.z);
+    all = __shfl_sync(FULL, mass, 31);
+    all_kept = __reduce_add_sync(FULL, v.w);
+    front_mass = __shfl_sync(FULL, mass - m, rank);
+    front_ties = (uint32_t)__shfl_sync(FULL, ties - v.z, rank);
+  };
+  add_up();
   if (cut.ties && tie_weight) all_kept += cut.ties;
   all += (uint64_t)cut.ties * tie_weight;
   const uint64_t target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
@@ -691,9 +723,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     __syncthreads();
     if (warp == 0) scan_blocks();
     r.sync();
-    front_mass = 0;
-    front_ties = 0;
-    for (int c = 0; c < rank; ++c) front_ties += load32(remote(&s.cta_ties, (uint32_t)c));
+    add_up();
   }
   if (warp == 0) {
     // the lane and the block of it in which the running weight passes the target
