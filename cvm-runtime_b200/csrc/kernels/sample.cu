@@ -215,21 +215,22 @@ __device__ __forceinline__ void clear(const Row& r, uint32_t* hist) {
 }
 // The cut that leaves `need` of the elements with from <= d < to (there are as many), and all in front of them.
 __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t from, uint64_t to) {
-  const uint32_t span = (uint32_t)(to - 1 - from), base = (uint32_t)from;   // (distances are 32 bits wide, `to` may be 2^32)
-  const int all_bits = max(1, 32 - __clz((int)span));
-  int bits = min(all_bits, DIGIT), shift = all_bits - bits;
-  uint32_t prefix = 0;
+  uint32_t base = (uint32_t)from, span = (uint32_t)(to - 1 - from);   // the elements with d - base <= span (distances are 32 bits wide)
   while (true) {
+    const int all_bits = max(1, 32 - __clz((int)span)), bits = min(all_bits, DIGIT), shift = all_bits - bits;
     uint32_t* const hist = s.hist;
     clear(r, hist);
+    const uint32_t top = (uint32_t)r.top - base;
     r.each([&](int32_t v) {
-      const uint32_t d = r.dist(v) - base;
-      if (r.dist(v) >= base && d <= span && (uint64_t)d >> (shift + bits) == prefix) atomicAdd(&hist[(d >> shift) & (BINS - 1)], 1u);
+      const uint32_t t = top - (uint32_t)v;
+      if (t <= span) atomicAdd(&hist[t >> shift], 1u);
     });
     r.sync();
     const int per = BINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // four or eight bins a thread
     uint32_t own[8];
-    const uint4 a = sum_of_cluster(hist + bin0, r.split), b = per > 4 ? sum_of_cluster(hist + bin0 + 4, r.split) : make_uint4(0, 0, 0, 0);
+    const uint4 none = make_uint4(0, 0, 0, 0);   // (the last digit has fewer bits)
+    const uint4 a = bin0 < 1 << bits ? sum_of_cluster(hist + bin0, r.split) : none;
+    const uint4 b = per > 4 && bin0 + 4 < 1 << bits ? sum_of_cluster(hist + bin0 + 4, r.split) : none;
     own[0] = a.x; own[1] = a.y; own[2] = a.z; own[3] = a.w; own[4] = b.x; own[5] = b.y; own[6] = b.z; own[7] = b.w;
     uint64_t sum = 0, total;
 #pragma unroll
@@ -248,11 +249,11 @@ __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t fro
     }
     __syncthreads();
     need -= s.found_before;
-    prefix = (prefix << bits) | (uint32_t)s.found;
-    if (need == s.found_size) return {min(from + (((uint64_t)prefix + 1) << shift), to), 0};   // all of the bin
-    if (shift == 0) return {from + prefix, (uint32_t)need};
-    bits = min(shift, DIGIT);
-    shift -= bits;
+    const uint64_t at = (uint64_t)base + ((uint64_t)(uint32_t)s.found << shift), behind = min(at + ((uint64_t)1 << shift), (uint64_t)base + span + 1);
+    if (need == s.found_size) return {behind, 0};   // all of the bin
+    if (shift == 0) return {at, (uint32_t)need};
+    base = (uint32_t)at;
+    span = (uint32_t)(behind - 1 - at);
   }
 }
 
@@ -323,7 +324,7 @@ __device__ int collect(const Row& r, Shared& s, uint64_t from, uint64_t to) {
   __syncthreads();
   r.each([&](int32_t v) {
     const uint32_t d = r.dist(v);
-    if (d >= base && d - base <= span) {
+    if (d >= base && d - base <= span && *reinterpret_cast<volatile uint32_t*>(&s.listed) <= LIST) {   // (not one after the other when there are too many)
       const uint32_t at = atomicAdd(&s.listed, 1u);
       if (at < LIST) s.list[at] = v;
     }
@@ -431,14 +432,14 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   // ---- the largest and the smallest score, and the bound of the k-th largest
   int32_t lo = INT32_MAX, hi = INT32_MIN;
   const bool by_count = k >= 1 && k < vocab;
-  if (by_count || r.wide) {
+  if (by_count || top_p < ONE) {
     r.each([&](int32_t v) {
       lo = min(lo, v);
       hi = max(hi, v);
     });
   } else {   // (the smallest is not asked for)
     r.each([&](int32_t v) { hi = max(hi, v); });
-    lo = hi == INT32_MIN ? INT32_MAX : hi;
+    lo = INT32_MIN;
   }
   const bool some = lo <= hi;   // the thread has seen an element
   const int32_t mine = hi;
@@ -588,11 +589,8 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
         if (wanted < size && to - from == 1) {
           cut = {from, (uint32_t)wanted};
         } else if (wanted < size) {
-          if (list.split > 1 || !by_count) {
-            const int m = collect(r, s, from, to);
-            if (m >= 0) look_at_list(m);
-          }
-          cut = cut_by_count(list, s, wanted, from, to);
+          // (one digit, mostly: an entry is 2^16 / scale distances wide)
+          cut = cut_by_count(list, s, wanted, from, min(to, max((uint64_t)r.dist(lo) + 1, from + 1)));
         } else if (to <= cut.D) {   // (all of the entry; the cut that was there may lie in it)
           cut = {to, 0};
         }
