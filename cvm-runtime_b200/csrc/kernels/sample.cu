@@ -118,6 +118,7 @@ struct Shared {
   uint32_t listed;
   // what every CTA of the cluster says of its slice, sent here by it
   alignas(16) int4 scores[MAX_SPLIT];     // smallest, largest, bounds
+  alignas(16) uint4 answer;
   alignas(16) uint4 sums[MAX_SPLIT];      // weight (low, high), ties, kept
   uint32_t late;                          // a slice has not arrived
   uint64_t found_before, found_size;
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       // the elements that are left, by table entry
       uint32_t* const hist = s.hist;
       clear(list, hist);
-      if (tid == 0) s.found = -1;
+      if (tid == 0) s.answer = make_uint4(0xffffffffu, 0, 0, 0);
       uint32_t last = 0;   // (of the last entry, which elements far behind the first one share: counted in registers)
       const uint32_t left = (uint32_t)min(cut.D, end - 1);
       const bool beyond = cut.D == end;
@@ -555,34 +556,43 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       if (lane == 0 && last) atomicAdd(&hist[list.last_entry], last);
       if (tid == 0 && cut.ties && (list.split == 1 || rank == 0)) atomicAdd(&hist[list.entry((uint32_t)cut.D)], cut.ties);
       list.sync();
-      const int per = BINS / threads;   // four or eight entries a thread
-      const uint32_t e0 = (uint32_t)(per * tid);
-      const uint4 a = sum_of_cluster(hist + e0, list.split), b = per > 4 ? sum_of_cluster(hist + e0 + 4, list.split) : make_uint4(0, 0, 0, 0);
+      // Every CTA adds up its share of the entries (a cluster's counts of all of them are 128 KB to fetch: 4 us), tells the
+      // others its weight, and the one in whose share the target lies finds the entry for all.
+      const int parts = (int)list.split, part = parts > 1 ? rank : 0, share = BINS / parts, per = max(4, share / threads);
+      const uint32_t e0 = (uint32_t)(part * share + per * tid);
+      const bool here = per * tid < share;
+      const uint4 none = make_uint4(0, 0, 0, 0), a = here ? sum_of_cluster(hist + e0, list.split) : none;
+      const uint4 b = here && per > 4 ? sum_of_cluster(hist + e0 + 4, list.split) : none;
       const uint32_t n[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
       uint64_t mass = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 8; ++i)
         if (n[i]) mass += (uint64_t)n[i] * (uint32_t)table_s[e0 + i];   // (entries behind the table are not counted)
-      }
       uint64_t all, before = block_scan(s, mass, all);
+      if (parts > 1) {
+        if (warp == 0 && lane < parts) store128(remote(&s.sums[rank], (uint32_t)lane), make_uint4((uint32_t)all, (uint32_t)(all >> 32), 0, 0));
+        list.sync();
+        const uint4 v = lane < parts ? s.sums[lane] : none;
+        const uint64_t m = v.x | (uint64_t)v.y << 32, sums = warp_scan(m);
+        before += __shfl_sync(FULL, sums - m, rank);
+        all = __shfl_sync(FULL, sums, 31);
+      }
       const uint64_t need = share_of(all);
       if (before < need && need <= before + mass) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (!n[i]) continue;
-          const uint64_t w = (uint32_t)table_s[e0 + i], here = n[i] * w;
-          if (before < need && need <= before + here) {
-            s.found = (int)(e0 + i);
-            s.found_before = (need - before + w - 1) / w;   // elements of this entry that are needed
-            s.found_size = n[i];
+          const uint64_t w = (uint32_t)table_s[e0 + i], weight = n[i] * w;
+          if (before < need && need <= before + weight) {   // the entry, the elements of it that are needed, and that it has
+            const uint4 answer = make_uint4(e0 + i, (uint32_t)((need - before + w - 1) / w), n[i], 0);
+            for (int c = 0; c < parts; ++c) store128(parts > 1 ? remote(&s.answer, (uint32_t)c) : smem_addr(&s.answer), answer);
           }
-          before += here;
+          before += weight;
         }
       }
-      __syncthreads();
-      const int e = s.found;
-      const uint64_t wanted = s.found_before, size = s.found_size;
-      __syncthreads();
+      list.sync();
+      const int e = (int)s.answer.x;
+      const uint64_t wanted = s.answer.y, size = s.answer.z;
       if (e >= 0) {   // (else nothing weighs anything, and no cut is needed)
         const uint64_t from = r.first_of((uint32_t)e);
         const uint64_t to = min((uint32_t)e == r.last_entry ? end : r.first_of((uint32_t)e + 1), cut.D + (cut.ties ? 1 : 0));
