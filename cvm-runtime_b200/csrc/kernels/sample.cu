@@ -5,9 +5,9 @@
 // d = max - x < D and the first `ties` ones, in index order, with d = D: the filters only look for that cut, and neither sort
 // nor list the row.
 //   top_k   In a CTA, the n-th largest of the maxima of its threads is a lower bound of its n-th largest element (that many
-//           threads have one as large).  So the row's k-th is not below any CTA's bound for n = k, nor below the least of the
-//           bounds for n = k / CTAs.  The elements that are not below these are few more than k; they are put on a list, and
-//           the cut is found on it.
+//           threads have one as large).  So the row's k-th is not below the least of the CTAs' bounds for n = k / CTAs.  The
+//           elements that are not below it are few more than k; they are put on a list, and the cuts of top_k and top_p are
+//           found on it by bisection: a thread holds an element, and a count over the CTA is one barrier.
 //   top_p   An element's weight is a function of its table index, so the elements of every index are counted; the running
 //           sum of count * weight gives the index in which the share is reached and how many of its elements are needed, and
 //           the cut among those is one by count again.
@@ -26,7 +26,7 @@ constexpr int MAX_WARPS = 32;
 constexpr int DIGIT = 12, BINS = 1 << DIGIT;       // of counts
 constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bin
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
-constexpr int LIST = 1024, ALL = 2048;  // elements on a CTA's list, on a cluster's
+constexpr int LIST = 1024;              // elements on a list
 constexpr int MAX_SPLIT = 8;
 constexpr int BLOCK = 512, GROUPS = BLOCK / 128, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / 8 / BLOCK + 2;
 constexpr uint32_t FULL = 0xffffffffu;
@@ -108,21 +108,22 @@ struct Cut {
 
 struct Shared {
   alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 16 bits, and the rest
-  uint64_t scan[MAX_WARPS];
+  uint64_t scan[MAX_WARPS], warp_sums[2][MAX_WARPS];
   int32_t lo[MAX_WARPS], hi[MAX_WARPS];
   uint32_t kept[MAX_WARPS];
   uint64_t block_mass[MAX_BLOCKS];
   uint32_t block_ties[MAX_BLOCKS];
-  alignas(16) int32_t list[LIST];
-  alignas(16) int32_t all[ALL];
+  alignas(16) int32_t list[LIST];    // of the slice's elements
+  alignas(16) int32_t all[LIST];     // of the row's
   uint32_t listed;
   // what every CTA of the cluster says of its slice, sent here by it
-  alignas(16) int4 scores[MAX_SPLIT];     // smallest, largest, bounds
+  alignas(16) int4 scores[MAX_SPLIT];     // smallest, largest, bound
   alignas(16) uint4 answer;
   alignas(16) uint4 sums[MAX_SPLIT];      // weight (low, high), ties, kept
   uint32_t late;                          // a slice has not arrived
   uint64_t found_before, found_size;
-  int found, found_share;
+  int found;
+  uint32_t counts[MAX_SPLIT];             // elements on the CTAs' lists
   uint64_t bar;
 };
 
@@ -318,36 +319,71 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
   }
 }
 
-// Puts the elements with from <= d < to, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are too many.
-__device__ int collect(const Row& r, Shared& s, uint64_t from, uint64_t to) {
-  const uint32_t span = (uint32_t)(to - 1 - from), base = (uint32_t)from;
+// Puts the elements with d <= last, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are more than threads.
+__device__ int collect(const Row& r, Shared& s, uint32_t last, int rank) {
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
   r.each([&](int32_t v) {
-    const uint32_t d = r.dist(v);
-    if (d >= base && d - base <= span && *reinterpret_cast<volatile uint32_t*>(&s.listed) <= LIST) {   // (not one after the other when there are too many)
+    if (r.dist(v) <= last && *reinterpret_cast<volatile uint32_t*>(&s.listed) <= LIST) {   // (not one after the other when there are too many)
       const uint32_t at = atomicAdd(&s.listed, 1u);
       if (at < LIST) s.list[at] = v;
     }
   });
-  r.sync();
-  if (r.split == 1) {
-    const int n = (int)s.listed;
-    if (n <= LIST)
-      for (int i = threadIdx.x; i < n; i += blockDim.x) s.all[i] = s.list[i];
-    __syncthreads();
-    return n <= LIST ? n : -1;
-  }
-  // (a warp for every CTA's list)
+  __syncthreads();
   const int lane = threadIdx.x & 31;
-  const uint32_t mine = lane < (int)r.split ? load32(remote(&s.listed, (uint32_t)lane)) : 0u;
+  if (threadIdx.x < r.split) store32(remote(&s.counts[rank], threadIdx.x), s.listed);
+  r.sync();
+  const uint32_t mine = lane < (int)r.split ? s.counts[lane] : 0u;
+  const bool fits = !__any_sync(FULL, mine > LIST) && __reduce_add_sync(FULL, mine) <= blockDim.x;
   const uint32_t sums = (uint32_t)warp_scan(mine), n = __shfl_sync(FULL, sums, 31);
-  const bool fits = !__any_sync(FULL, mine > LIST) && n <= ALL;
+  // (a warp for every CTA's list)
   const uint32_t c = threadIdx.x >> 5, count = __shfl_sync(FULL, mine, (int)(c & 31)), at = __shfl_sync(FULL, sums - mine, (int)(c & 31));
   if (fits && c < r.split)
     for (uint32_t i = lane; i < count; i += 32) s.all[at + i] = (int32_t)load32(remote(&s.list[i], c));
   __syncthreads();
   return fits ? (int)n : -1;
+}
+
+// The cut that leaves `need` elements of a list, one a thread (`mine`: the thread has one, at distance d <= last).
+__device__ Cut cut_list_by_count(uint64_t need, bool mine, uint32_t d, uint32_t last) {
+  uint32_t from = 0, to = last;
+  while (from < to) {
+    const uint32_t mid = from + (to - from) / 2;
+    if ((uint64_t)__syncthreads_count(mine && d <= mid) >= need) to = mid;
+    else from = mid + 1;
+  }
+  return {from, (uint32_t)(need - (uint64_t)__syncthreads_count(mine && d < from))};
+}
+// Sum of w over the CTA.  `turn` alternates, so that one barrier a sum is enough.
+__device__ __forceinline__ uint64_t block_sum(Shared& s, uint32_t w, int turn) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  uint64_t* const sums = s.warp_sums[turn & 1];
+  const uint64_t sum = __reduce_add_sync(FULL, w & 0xffffu) + ((uint64_t)__reduce_add_sync(FULL, w >> 16) << 16);   // below 2^36
+  if (lane == 0) sums[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  const uint64_t v = lane < warps ? sums[lane] : 0;
+  return __reduce_add_sync(FULL, (uint32_t)v & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(v >> 20)) << 20);
+}
+// Where the weight of a list's elements in front of `cut` reaches need(total).
+template <typename Need>
+__device__ Cut cut_list_by_weight(const Row& r, Shared& s, const Cut& cut, bool mine, uint32_t d, const Need& need_of) {
+  const uint32_t w = mine && d < cut.D ? r.weight(d) : 0u;
+  const uint64_t tie_weight = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
+  int turn = 0;
+  const uint64_t strict = block_sum(s, w, turn++), need = need_of(strict + cut.ties * tie_weight);
+  if (need > strict) {   // the cut lies among the ties, or nothing weighs anything
+    Cut c = cut;
+    if (tie_weight) c.ties = (uint32_t)min((uint64_t)cut.ties, (need - strict + tie_weight - 1) / tie_weight);
+    return c;
+  }
+  uint32_t from = 0, to = (uint32_t)(cut.D - 1);   // (something lies in front of the cut)
+  while (from < to) {
+    const uint32_t mid = from + (to - from) / 2;
+    if (block_sum(s, d <= mid ? w : 0u, turn++) >= need) to = mid;
+    else from = mid + 1;
+  }
+  const uint64_t rest = need - block_sum(s, d < from ? w : 0u, turn++), each = r.weight(from);
+  return {from, (uint32_t)((rest + each - 1) / each)};
 }
 
 __device__ __forceinline__ int bits_of(uint64_t range) { return max(1, 64 - __clzll((long long)range)); }   // of the largest distance
@@ -450,36 +486,20 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   __syncthreads();
   lo = __reduce_min_sync(FULL, lane < warps ? s.lo[lane] : INT32_MAX);
   hi = __reduce_max_sync(FULL, lane < warps ? s.hi[lane] : INT32_MIN);
-  int32_t bound = INT32_MIN, share = INT32_MIN;   // the bounds for n = k and n = k / CTAs
-  if (by_count && k <= p.split * threads) {
-    for (int i = tid; i < BINS; i += threads) s.hist[i] = 0;
-    if (tid == 0) s.found = s.found_share = -1;
-    __syncthreads();
-    const int shift = max(0, bits_of((uint32_t)hi - (uint32_t)lo) - DIGIT);
-    if (some) atomicAdd(&s.hist[((uint32_t)hi - (uint32_t)mine) >> shift], 1u);
-    __syncthreads();
-    const int per = BINS / threads, bin0 = per * tid;
-    uint32_t sum = 0;
-    for (int i = 0; i < per; ++i) sum += s.hist[bin0 + i];
-    uint64_t total, before = block_scan(s, sum, total);
-    const uint64_t need = (uint64_t)k, part = (uint64_t)((k + p.split - 1) / p.split);
-    if (sum)
-      for (int i = 0; i < per; ++i) {
-        const uint64_t after = before + s.hist[bin0 + i];
-        if (before < need && need <= after) s.found = bin0 + i;
-        if (before < part && part <= after) s.found_share = bin0 + i;
-        before = after;
-      }
-    __syncthreads();
-    const auto least = [&](int bin) {   // what the maxima of this bin and of those before it are not below
-      const int64_t b = (int64_t)hi - ((((int64_t)bin + 1) << shift) - 1);
-      return bin >= 0 && b > INT32_MIN ? (int32_t)b : INT32_MIN;
-    };
-    bound = least(s.found);
-    share = least(s.found_share);
+  int32_t bound = INT32_MIN;
+  const int part = (k - 1) / p.split + 1;   // of k, for a CTA
+  if (by_count && part <= threads && __syncthreads_count(some) >= part) {
+    const uint32_t far = (uint32_t)hi - (uint32_t)mine;
+    uint32_t from = 0, to = (uint32_t)hi - (uint32_t)lo;
+    for (int i = 0; i < 14 && from < to; ++i) {   // (to some ten-thousandth of the range)
+      const uint32_t mid = from + (to - from) / 2;
+      if (__syncthreads_count(some && far <= mid) >= part) to = mid;
+      else from = mid + 1;
+    }
+    bound = (int32_t)((uint32_t)hi - to);
   }
   if (warp == 0 && lane < p.split) {   // (a lane for every CTA)
-    store128(remote(&s.scores[rank], (uint32_t)lane), make_uint4((uint32_t)lo, (uint32_t)hi, (uint32_t)bound, (uint32_t)share));
+    store128(remote(&s.scores[rank], (uint32_t)lane), make_uint4((uint32_t)lo, (uint32_t)hi, (uint32_t)bound, 0));
     if (!landed) store32(remote(&s.late, (uint32_t)lane), 1u);
   }
   r.sync();
@@ -488,7 +508,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     const int4 v = s.scores[min(lane, p.split - 1)];
     lo = __reduce_min_sync(FULL, v.x);
     hi = __reduce_max_sync(FULL, v.y);
-    bound = max(__reduce_max_sync(FULL, v.z), __reduce_min_sync(FULL, v.w));
+    bound = __reduce_min_sync(FULL, v.z);
   }
   if (late) {   // a copy that never came (its wait is bounded): no element is drawn
     if (rank == 0 && tid == 0) d.token[row] = -1;
@@ -507,62 +527,61 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   // ---- the cuts
   const uint64_t end = (uint64_t)1 << 32;
   Cut cut = {end, 0};   // everything
-  // What the cuts look at instead of the row: a list that holds all that the last one has left, and more.
-  Row list = r;
-  auto look_at_list = [&](int n) {
-    list.x = s.all;
-    list.first = 0;
-    list.last = n;
-    list.split = 1;
+  const auto share_of = [=](uint64_t all) {
+    const uint64_t need = top_p * (all >> 30) + ((top_p * (all & (ONE - 1)) + ONE - 1) >> 30);
+    return need > 1 ? need : (uint64_t)1;
   };
+  bool listed = false;
   if (by_count) {
-    const uint64_t to = (uint64_t)r.dist(bound) + 1;
-    const int n = collect(r, s, 0, to);
-    if (n >= 0) look_at_list(n);
-    cut = cut_by_count(list, s, (uint64_t)k, 0, n >= 0 ? to : (uint64_t)r.dist(lo) + 1);
+    const int n = collect(r, s, r.dist(bound), rank);
+    if (n >= 0) {
+      listed = true;
+      const bool mine = tid < n;
+      const uint32_t dj = mine ? r.dist(s.all[tid]) : 0u;
+      cut = cut_list_by_count((uint64_t)k, mine, dj, r.dist(bound));
+      if (top_p < ONE) cut = cut_list_by_weight(r, s, cut, mine, dj, share_of);
+    } else {   // (hundreds of equal scores, or a large k)
+      cut = cut_by_count(r, s, (uint64_t)k, 0, (uint64_t)r.dist(lo) + 1);
+    }
   }
-  if (top_p < ONE) {
-    const auto share_of = [=](uint64_t all) {
-      const uint64_t need = top_p * (all >> 30) + ((top_p * (all & (ONE - 1)) + ONE - 1) >> 30);
-      return need > 1 ? need : (uint64_t)1;
-    };
+  if (top_p < ONE && !listed) {
     if (r.wide) {
       const uint32_t w = cut.ties ? r.weight((uint32_t)cut.D) : 0u, ties = cut.ties;
-      cut = cut_by_weight(list, s, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
+      cut = cut_by_weight(r, s, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
     } else {
       // the elements that are left, by table entry
       uint32_t* const hist = s.hist;
-      clear(list, hist);
+      clear(r, hist);
       if (tid == 0) s.answer = make_uint4(0xffffffffu, 0, 0, 0);
       uint32_t last = 0;   // (of the last entry, which elements far behind the first one share: counted in registers)
       const uint32_t left = (uint32_t)min(cut.D, end - 1);
       const bool beyond = cut.D == end;
-      if (beyond && list.gentle) {
-        list.each([&](int32_t v) {
-          const uint32_t e = list.entry_of(v);
-          if (e == list.last_entry) ++last;
+      if (beyond && r.gentle) {
+        r.each([&](int32_t v) {
+          const uint32_t e = r.entry_of(v);
+          if (e == r.last_entry) ++last;
           else atomicAdd(&hist[e], 1u);
         });
       } else {
-        list.each([&](int32_t v) {
-          const uint32_t dj = list.dist(v), e = list.entry(dj);
+        r.each([&](int32_t v) {
+          const uint32_t dj = r.dist(v), e = r.entry(dj);
           if (beyond || dj < left) {
-            if (e == list.last_entry) ++last;
+            if (e == r.last_entry) ++last;
             else atomicAdd(&hist[e], 1u);
           }
         });
       }
       last = __reduce_add_sync(FULL, last);
-      if (lane == 0 && last) atomicAdd(&hist[list.last_entry], last);
-      if (tid == 0 && cut.ties && (list.split == 1 || rank == 0)) atomicAdd(&hist[list.entry((uint32_t)cut.D)], cut.ties);
-      list.sync();
+      if (lane == 0 && last) atomicAdd(&hist[r.last_entry], last);
+      if (tid == 0 && cut.ties && rank == 0) atomicAdd(&hist[r.entry((uint32_t)cut.D)], cut.ties);
+      r.sync();
       // Every CTA adds up its share of the entries (a cluster's counts of all of them are 128 KB to fetch: 4 us), tells the
       // others its weight, and the one in whose share the target lies finds the entry for all.
-      const int parts = (int)list.split, part = parts > 1 ? rank : 0, share = BINS / parts, per = max(4, share / threads);
+      const int parts = (int)r.split, part = parts > 1 ? rank : 0, share = BINS / parts, per = max(4, share / threads);
       const uint32_t e0 = (uint32_t)(part * share + per * tid);
       const bool here = per * tid < share;
-      const uint4 none = make_uint4(0, 0, 0, 0), a = here ? sum_of_cluster(hist + e0, list.split) : none;
-      const uint4 b = here && per > 4 ? sum_of_cluster(hist + e0 + 4, list.split) : none;
+      const uint4 none = make_uint4(0, 0, 0, 0), a = here ? sum_of_cluster(hist + e0, r.split) : none;
+      const uint4 b = here && per > 4 ? sum_of_cluster(hist + e0 + 4, r.split) : none;
       const uint32_t n[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
       uint64_t mass = 0;
 #pragma unroll
@@ -571,7 +590,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       uint64_t all, before = block_scan(s, mass, all);
       if (parts > 1) {
         if (warp == 0 && lane < parts) store128(remote(&s.sums[rank], (uint32_t)lane), make_uint4((uint32_t)all, (uint32_t)(all >> 32), 0, 0));
-        list.sync();
+        r.sync();
         const uint4 v = lane < parts ? s.sums[lane] : none;
         const uint64_t m = v.x | (uint64_t)v.y << 32, sums = warp_scan(m);
         before += __shfl_sync(FULL, sums - m, rank);
@@ -590,7 +609,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
           before += weight;
         }
       }
-      list.sync();
+      r.sync();
       const int e = (int)s.answer.x;
       const uint64_t wanted = s.answer.y, size = s.answer.z;
       if (e >= 0) {   // (else nothing weighs anything, and no cut is needed)
@@ -600,7 +619,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
           cut = {from, (uint32_t)wanted};
         } else if (wanted < size) {
           // (one digit, mostly: an entry is 2^16 / scale distances wide)
-          cut = cut_by_count(list, s, wanted, from, min(to, max((uint64_t)r.dist(lo) + 1, from + 1)));
+          cut = cut_by_count(r, s, wanted, from, min(to, max((uint64_t)r.dist(lo) + 1, from + 1)));
         } else if (to <= cut.D) {   // (all of the entry; the cut that was there may lie in it)
           cut = {to, 0};
         }
@@ -689,9 +708,9 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (lane * PER + i < blocks) { m += s.block_mass[lane * PER + i]; t += s.block_ties[lane * PER + i]; }
-    const uint64_t mi = warp_scan(m), ti = warp_scan(t);
+    const uint64_t mi = warp_scan(m), ti = cut.ties ? warp_scan(t) : 0;
     mass_in_front = mi - m;
-    ties_in_front = (uint32_t)(ti - t);
+    ties_in_front = cut.ties ? (uint32_t)(ti - t) : 0u;
     const uint64_t mass = __shfl_sync(FULL, mi, 31);
     const uint32_t ties = __shfl_sync(FULL, (uint32_t)ti, 31);
     if (lane < p.split) store128(remote(&s.sums[rank], (uint32_t)lane), make_uint4((uint32_t)mass, (uint32_t)(mass >> 32), ties, kept));
@@ -704,12 +723,17 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   uint64_t all, front_mass;
   uint32_t front_ties, all_kept;
   auto add_up = [&]() {   // over the CTAs, and over those in front of this one
-    const uint4 v = lane < p.split ? s.sums[lane] : make_uint4(0, 0, 0, 0);
-    const uint64_t m = v.x | (uint64_t)v.y << 32, mass = warp_scan(m), ties = warp_scan(v.z);
-    all = __shfl_sync(FULL, mass, 31);
-    all_kept = __reduce_add_sync(FULL, v.w);
-    front_mass = __shfl_sync(FULL, mass - m, rank);
-    front_ties = (uint32_t)__shfl_sync(FULL, ties - v.z, rank);
+    all = front_mass = 0;
+    front_ties = all_kept = 0;
+#pragma unroll
+    for (int c = 0; c < MAX_SPLIT; ++c) {
+      if (c >= p.split) break;
+      const uint4 v = s.sums[c];
+      const uint64_t m = v.x | (uint64_t)v.y << 32;
+      all += m;
+      all_kept += v.w;
+      if (c < rank) { front_mass += m; front_ties += v.z; }
+    }
   };
   add_up();
   if (cut.ties && tie_weight) all_kept += cut.ties;
