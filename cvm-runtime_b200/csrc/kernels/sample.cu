@@ -28,7 +28,7 @@ constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bi
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
 constexpr int LIST = 1024;              // elements on a list
 constexpr int MAX_SPLIT = 8;
-constexpr int BLOCK = 512, GROUPS = BLOCK / 128, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / 8 / BLOCK + 2;
+constexpr int BLOCK = 512, GROUPS = BLOCK / 128, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / BLOCK + 2;
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr uint64_t ONE = 1u << 30;
 
@@ -107,14 +107,24 @@ struct Cut {
 };
 
 struct Shared {
-  alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 16 bits, and the rest
-  uint64_t scan[MAX_WARPS], warp_sums[2][MAX_WARPS];
+  union {
+    alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 16 bits, and the rest
+    struct {                           // (a row whose cuts are found on its list needs no histogram behind it)
+      alignas(16) int2 list[LIST];     // of the slice's elements: score and index
+      alignas(16) uint2 all[LIST];     // of the row's: distance and index
+    };
+  };
+  union {
+    struct {
+      uint64_t block_mass[MAX_BLOCKS];
+      uint32_t block_ties[MAX_BLOCKS];
+    };
+    uint32_t all_weight[LIST];
+  };
+  uint64_t scan[MAX_WARPS];
+  uint32_t reached[2][MAX_WARPS];
   int32_t lo[MAX_WARPS], hi[MAX_WARPS];
   uint32_t kept[MAX_WARPS];
-  uint64_t block_mass[MAX_BLOCKS];
-  uint32_t block_ties[MAX_BLOCKS];
-  alignas(16) int32_t list[LIST];    // of the slice's elements
-  alignas(16) int32_t all[LIST];     // of the row's
   uint32_t listed;
   // what every CTA of the cluster says of its slice, sent here by it
   alignas(16) int4 scores[MAX_SPLIT];     // smallest, largest, bound
@@ -127,7 +137,10 @@ struct Shared {
   uint64_t bar;
 };
 
-// What a thread knows of its row, or (find_cut) of a list of some of its elements.
+extern __shared__ __align__(16) uint8_t dynamic_smem[];   // the slice, if it is resident, and the table
+__device__ __forceinline__ const int32_t* resident() { return reinterpret_cast<const int32_t*>(dynamic_smem); }
+
+// What a thread knows of its row.
 struct Row {
   const int32_t* x;
   const int32_t* table;
@@ -163,37 +176,46 @@ struct Row {
     if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
   }
-  // Calls f(value) for the thread's share of the valid elements: whole groups of four, and the ragged ends by a few threads.
-  template <typename F>
+  // The values at places j .. j + 3, j a multiple of 4 (zeros, or what lies there in shared memory, outside the valid ones).
+  template <bool RESIDENT>
+  __device__ __forceinline__ int4 four(int j, bool all_valid) const {
+    if (RESIDENT) return all_valid || j < last ? *reinterpret_cast<const int4*>(resident() + j) : make_int4(0, 0, 0, 0);
+    if (all_valid || (j >= first && j + 4 <= last)) return *reinterpret_cast<const int4*>(x + j);
+    int4 v = make_int4(0, 0, 0, 0);   // (nothing outside the row is read)
+    if (j >= first && j < last) v.x = x[j];
+    if (j + 1 >= first && j + 1 < last) v.y = x[j + 1];
+    if (j + 2 >= first && j + 2 < last) v.z = x[j + 2];
+    if (j + 3 >= first && j + 3 < last) v.w = x[j + 3];
+    return v;
+  }
+  // Calls f(value, place) for the thread's share of the valid elements: whole groups of four, and the ragged ends by a few threads.
+  template <bool RESIDENT, typename F>
   __device__ __forceinline__ void each(const F& f) const {
     const int g0 = (first + 3) >> 2, g1 = last >> 2, tid = threadIdx.x;
+    const int32_t* const at = RESIDENT ? resident() : x;
     if (g0 > g1) {   // (less than a group)
-      if (first + tid < last) f(x[first + tid]);
+      if (first + tid < last) f(at[first + tid], first + tid);
       return;
     }
+    const auto four = [&](const int4& v, int g) {
+      f(v.x, 4 * g);
+      f(v.y, 4 * g + 1);
+      f(v.z, 4 * g + 2);
+      f(v.w, 4 * g + 3);
+    };
+    constexpr int UNDER_WAY = RESIDENT ? 4 : 8;
     const int step = blockDim.x;
     int g = g0 + tid;
-    for (; g + 3 * step < g1; g += 4 * step) {   // (four requests under way)
-      int4 v[4];
+    for (; g + (UNDER_WAY - 1) * step < g1; g += UNDER_WAY * step) {
+      int4 v[UNDER_WAY];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const int4*>(x)[g + i * step];
+      for (int i = 0; i < UNDER_WAY; ++i) v[i] = reinterpret_cast<const int4*>(at)[g + i * step];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f(v[i].x);
-        f(v[i].y);
-        f(v[i].z);
-        f(v[i].w);
-      }
+      for (int i = 0; i < UNDER_WAY; ++i) four(v[i], g + i * step);
     }
-    for (; g < g1; g += step) {
-      const int4 v = reinterpret_cast<const int4*>(x)[g];
-      f(v.x);
-      f(v.y);
-      f(v.z);
-      f(v.w);
-    }
-    if (first + tid < 4 * g0) f(x[first + tid]);
-    if (4 * g1 + tid < last) f(x[4 * g1 + tid]);
+    for (; g < g1; g += step) four(reinterpret_cast<const int4*>(at)[g], g);
+    if (first + tid < 4 * g0) f(at[first + tid], first + tid);
+    if (4 * g1 + tid < last) f(at[4 * g1 + tid], 4 * g1 + tid);
   }
 };
 
@@ -216,6 +238,7 @@ __device__ __forceinline__ void clear(const Row& r, uint32_t* hist) {
   __syncthreads();
 }
 // The cut that leaves `need` of the elements with from <= d < to (there are as many), and all in front of them.
+template <bool RESIDENT>
 __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t from, uint64_t to) {
   uint32_t base = (uint32_t)from, span = (uint32_t)(to - 1 - from);   // the elements with d - base <= span (distances are 32 bits wide)
   while (true) {
@@ -223,7 +246,7 @@ __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t fro
     uint32_t* const hist = s.hist;
     clear(r, hist);
     const uint32_t top = (uint32_t)r.top - base;
-    r.each([&](int32_t v) {
+    r.each<RESIDENT>([&](int32_t v, int) {
       const uint32_t t = top - (uint32_t)v;
       if (t <= span) atomicAdd(&hist[t >> shift], 1u);
     });
@@ -261,7 +284,7 @@ __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t fro
 
 // Where, in the order of d, the weight of the elements with d < limit reaches need(total); if the total is less than that, a
 // cut among the ties of `whole`, of tie_weight each.
-template <typename Need>
+template <bool RESIDENT, typename Need>
 __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need& need_of, const Cut& whole, uint32_t tie_weight) {
   int bits = min(range_bits, WDIGIT), shift = range_bits - bits;
   uint32_t prefix = 0;
@@ -269,7 +292,7 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
   for (bool first = true;; first = false) {
     uint32_t* const hist = s.hist;
     clear(r, hist);
-    r.each([&](int32_t v) {
+    r.each<RESIDENT>([&](int32_t v, int) {
       const uint32_t d = r.dist(v);
       if (d < whole.D && (uint64_t)d >> (shift + bits) == prefix) {
         const uint32_t w = r.weight(d), bin = (d >> shift) & ((1u << bits) - 1u);
@@ -319,14 +342,16 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
   }
 }
 
-// Puts the elements with d <= last, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are more than threads.
-__device__ int collect(const Row& r, Shared& s, uint32_t last, int rank) {
+// Puts the elements with d <= last, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are more than
+// threads.  `index0`: the index of place 0.
+template <bool RESIDENT>
+__device__ int collect(const Row& r, Shared& s, uint32_t last, int rank, int index0) {
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  r.each([&](int32_t v) {
+  r.each<RESIDENT>([&](int32_t v, int j) {
     if (r.dist(v) <= last && *reinterpret_cast<volatile uint32_t*>(&s.listed) <= LIST) {   // (not one after the other when there are too many)
       const uint32_t at = atomicAdd(&s.listed, 1u);
-      if (at < LIST) s.list[at] = v;
+      if (at < LIST) s.list[at] = make_int2(v, index0 + j);
     }
   });
   __syncthreads();
@@ -339,7 +364,10 @@ __device__ int collect(const Row& r, Shared& s, uint32_t last, int rank) {
   // (a warp for every CTA's list)
   const uint32_t c = threadIdx.x >> 5, count = __shfl_sync(FULL, mine, (int)(c & 31)), at = __shfl_sync(FULL, sums - mine, (int)(c & 31));
   if (fits && c < r.split)
-    for (uint32_t i = lane; i < count; i += 32) s.all[at + i] = (int32_t)load32(remote(&s.list[i], c));
+    for (uint32_t i = lane; i < count; i += 32) {
+      const uint32_t from = remote(&s.list[i], c), v = load32(from), index = load32(from + 4);
+      s.all[at + i] = make_uint2(r.dist((int32_t)v), index);
+    }
   __syncthreads();
   return fits ? (int)n : -1;
 }
@@ -354,47 +382,45 @@ __device__ Cut cut_list_by_count(uint64_t need, bool mine, uint32_t d, uint32_t 
   }
   return {from, (uint32_t)(need - (uint64_t)__syncthreads_count(mine && d < from))};
 }
-// Sum of w over the CTA.  `turn` alternates, so that one barrier a sum is enough.
-__device__ __forceinline__ uint64_t block_sum(Shared& s, uint32_t w, int turn) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  uint64_t* const sums = s.warp_sums[turn & 1];
-  const uint64_t sum = __reduce_add_sync(FULL, w & 0xffffu) + ((uint64_t)__reduce_add_sync(FULL, w >> 16) << 16);   // below 2^36
-  if (lane == 0) sums[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  const uint64_t v = lane < warps ? sums[lane] : 0;
-  return __reduce_add_sync(FULL, (uint32_t)v & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(v >> 20)) << 20);
+// The smallest K in [from, to] for which the weights of the list's elements with key <= K sum to `need` or more (those up to
+// `to` do).  Every warp adds up the list for a place of its own between `from` and `to`, so a turn cuts what is left to a 17th
+// (512 threads): five turns for any index, where halving takes eighteen.
+template <typename Key>
+__device__ uint32_t search_list(Shared& s, int n, uint32_t from, uint32_t to, uint64_t need, const Key& key) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  for (int turn = 0; from < to; ++turn) {
+    const uint64_t range = to - from;
+    const auto place = [&](int i) { return from + (uint32_t)(range * (uint32_t)(i + 1) / (uint32_t)(warps + 1)); };
+    const uint32_t at = place(warp);
+    uint64_t sum = 0;
+    for (int i = lane; i < n; i += 32) sum += key(s.all[i]) <= at ? s.all_weight[i] : 0u;   // (below 2^36)
+    sum = __reduce_add_sync(FULL, (uint32_t)sum & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(sum >> 20)) << 20);
+    if (lane == 0) s.reached[turn & 1][warp] = sum >= need;
+    __syncthreads();
+    const uint32_t mask = __ballot_sync(FULL, lane < warps && s.reached[turn & 1][lane]);
+    const int first = mask ? __ffs(mask) - 1 : warps;
+    const uint32_t lower = first > 0 ? place(first - 1) + 1 : from;
+    if (mask) to = place(first);
+    from = lower;
+  }
+  return from;
 }
-// Where the weight of a list's elements in front of `cut` reaches need(total).
-template <typename Need>
-__device__ Cut cut_list_by_weight(const Row& r, Shared& s, const Cut& cut, bool mine, uint32_t d, const Need& need_of) {
-  const uint32_t w = mine && d < cut.D ? r.weight(d) : 0u;
-  const uint64_t tie_weight = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
-  int turn = 0;
-  const uint64_t strict = block_sum(s, w, turn++), need = need_of(strict + cut.ties * tie_weight);
-  if (need > strict) {   // the cut lies among the ties, or nothing weighs anything
-    Cut c = cut;
-    if (tie_weight) c.ties = (uint32_t)min((uint64_t)cut.ties, (need - strict + tie_weight - 1) / tie_weight);
-    return c;
-  }
-  uint32_t from = 0, to = (uint32_t)(cut.D - 1);   // (something lies in front of the cut)
-  while (from < to) {
-    const uint32_t mid = from + (to - from) / 2;
-    if (block_sum(s, d <= mid ? w : 0u, turn++) >= need) to = mid;
-    else from = mid + 1;
-  }
-  const uint64_t rest = need - block_sum(s, d < from ? w : 0u, turn++), each = r.weight(from);
-  return {from, (uint32_t)((rest + each - 1) / each)};
+// Sum of the list's weights (every warp for itself).
+__device__ __forceinline__ uint64_t sum_of_list(const Shared& s, int n) {
+  uint64_t sum = 0;
+  for (int i = threadIdx.x & 31; i < n; i += 32) sum += s.all_weight[i];
+  return __reduce_add_sync(FULL, (uint32_t)sum & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(sum >> 20)) << 20);
 }
 
 __device__ __forceinline__ int bits_of(uint64_t range) { return max(1, 64 - __clzll((long long)range)); }   // of the largest distance
 
+template <bool RESIDENT>
 __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__ Params p) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
   const int rank = p.split > 1 ? (int)cluster_rank() : 0, row = (int)blockIdx.x / p.split;
-  int32_t* const x = reinterpret_cast<int32_t*>(smem_raw);
-  int32_t* const table_s = x + p.slice;
+  int32_t* const slice_s = reinterpret_cast<int32_t*>(dynamic_smem);
+  int32_t* const table_s = slice_s + (RESIDENT ? p.slice : 0);
   const cvmk_sample_desc& d = p.d;
   const int vocab = d.vocab;
   const int32_t* src = d.logits + (size_t)row * (size_t)d.pitch;
@@ -402,6 +428,8 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   const int skew = (int)((reinterpret_cast<uintptr_t>(src) >> 2) & 3);
   const int begin = rank * p.slice;                       // this slice's place 0
   Row r;
+  const int32_t* const at = src - skew + begin;           // of place 0
+  const int32_t* const x = RESIDENT ? slice_s : at;
   r.x = x;
   r.first = min(max(skew - begin, 0), p.slice);
   r.last = min(max(skew + vocab - begin, r.first), p.slice);
@@ -422,17 +450,16 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   for (int i = 0; i < EARLY; ++i) entry[i] = p.table_smem && tid + i * threads < d.table_len ? d.table[tid + i * threads] : 0;
   // whole 16-byte words by the bulk engine, the ragged ends by threads
   const int b0 = min((r.first + 3) & ~3, r.last), b1 = max(b0, r.last & ~3);
-  const int32_t* at = src - skew + begin;                 // of place 0
-  if (tid == 0) {
+  if (RESIDENT && tid == 0) {
     const uint32_t bytes = (uint32_t)(b1 - b0) * 4u;
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(&s.bar)), "r"(bytes) : "memory");
     if (bytes)
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(x + b0)),
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(slice_s + b0)),
                    "l"(at + b0), "r"(bytes), "r"(smem_addr(&s.bar))
                    : "memory");
   }
-  if (tid >= 32 && tid < 35 && r.first + tid - 32 < b0) x[r.first + tid - 32] = at[r.first + tid - 32];
-  if (tid >= 35 && tid < 38 && b1 + tid - 35 < r.last) x[b1 + tid - 35] = at[b1 + tid - 35];
+  if (RESIDENT && tid >= 32 && tid < 35 && r.first + tid - 32 < b0) slice_s[r.first + tid - 32] = at[r.first + tid - 32];
+  if (RESIDENT && tid >= 35 && tid < 38 && b1 + tid - 35 < r.last) slice_s[b1 + tid - 35] = at[b1 + tid - 35];
   const int k = d.top_k ? d.top_k[row] : 0;
   const uint64_t top_p = d.top_p ? (uint64_t)min(max(d.top_p[row], 0), (int)ONE) : ONE;
   const uint64_t min_p = d.min_p ? (uint64_t)min(max(d.min_p[row], 0), (int)ONE) : 0;
@@ -453,7 +480,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     }
   const bool plain_table = __syncthreads_and(plain) && p.table_smem;
   // (bounded: the copy is the only thing that is waited for)
-  bool landed = false;
+  bool landed = !RESIDENT;
   for (uint32_t i = 0; !landed && i < (1u << 19); ++i) {
     uint32_t ok;
     asm volatile(
@@ -470,12 +497,12 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   int32_t lo = INT32_MAX, hi = INT32_MIN;
   const bool by_count = k >= 1 && k < vocab;
   if (by_count || top_p < ONE) {
-    r.each([&](int32_t v) {
+    r.each<RESIDENT>([&](int32_t v, int) {
       lo = min(lo, v);
       hi = max(hi, v);
     });
   } else {   // (the smallest is not asked for)
-    r.each([&](int32_t v) { hi = max(hi, v); });
+    r.each<RESIDENT>([&](int32_t v, int) { hi = max(hi, v); });
     lo = INT32_MIN;
   }
   const bool some = lo <= hi;   // the thread has seen an element
@@ -531,23 +558,73 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     const uint64_t need = top_p * (all >> 30) + ((top_p * (all & (ONE - 1)) + ONE - 1) >> 30);
     return need > 1 ? need : (uint64_t)1;
   };
-  bool listed = false;
   if (by_count) {
-    const int n = collect(r, s, r.dist(bound), rank);
+    const uint32_t last = r.dist(bound);
+    const int n = collect<RESIDENT>(r, s, last, rank, begin - skew);
     if (n >= 0) {
-      listed = true;
+      // Everything else is done on the list, by every CTA for itself.
       const bool mine = tid < n;
-      const uint32_t dj = mine ? r.dist(s.all[tid]) : 0u;
-      cut = cut_list_by_count((uint64_t)k, mine, dj, r.dist(bound));
-      if (top_p < ONE) cut = cut_list_by_weight(r, s, cut, mine, dj, share_of);
-    } else {   // (hundreds of equal scores, or a large k)
-      cut = cut_by_count(r, s, (uint64_t)k, 0, (uint64_t)r.dist(lo) + 1);
+      const uint2 e = mine ? s.all[tid] : make_uint2(0, 0);
+      cut = cut_list_by_count((uint64_t)k, mine, e.x, last);
+      // of the elements at the cut the first ones by index: those up to `tie_index`
+      auto tie_index = [&]() {
+        uint32_t from = 0, to = (uint32_t)vocab - 1u;
+        if ((uint32_t)__syncthreads_count(mine && e.x == cut.D) <= cut.ties) return to;
+        while (from < to) {
+          const uint32_t mid = from + (to - from) / 2;
+          if ((uint32_t)__syncthreads_count(mine && e.x == cut.D && e.y <= mid) >= cut.ties) to = mid;
+          else from = mid + 1;
+        }
+        return from;
+      };
+      uint32_t ties_to = tie_index();
+      const uint32_t weight = mine ? r.weight(e.x) : 0u;
+      uint32_t w = e.x < cut.D || (e.x == cut.D && e.y <= ties_to) ? weight : 0u;
+      if (mine) s.all_weight[tid] = w;
+      __syncthreads();
+      uint64_t all = sum_of_list(s, n);
+      if (top_p < ONE && all) {
+        const uint64_t need = share_of(all);
+        const uint32_t at_d = search_list(s, n, 0, last, need, [](const uint2& v) { return v.x; });
+        // the elements in front of at_d, and of those at it as many as it takes
+        const uint32_t each = r.weight(at_d);
+        uint64_t before = 0;
+        for (int i = lane; i < n; i += 32) before += s.all[i].x < at_d ? s.all_weight[i] : 0u;
+        before = __reduce_add_sync(FULL, (uint32_t)before & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(before >> 20)) << 20);
+        const uint32_t taken = (uint32_t)((need - before + each - 1) / each);
+        if (at_d < cut.D || taken < cut.ties) {   // (else the cut of top_k stays)
+          cut = {at_d, taken};
+          ties_to = tie_index();
+          w = e.x < cut.D || (e.x == cut.D && e.y <= ties_to) ? weight : 0u;
+        }
+        __syncthreads();   // (the weights have been read)
+        if (mine) s.all_weight[tid] = w;
+        __syncthreads();
+        all = sum_of_list(s, n);
+      }
+      const uint32_t kept = (uint32_t)__syncthreads_count(mine && w > 0);
+      const uint64_t target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
+      if (all == 0) {   // nothing weighs anything: the first element with d = 0
+        if (mine) s.all_weight[tid] = e.x == 0;
+        __syncthreads();
+      }
+      const uint32_t token = search_list(s, n, 0, (uint32_t)vocab - 1u, target + 1, [](const uint2& v) { return v.y; });
+      if (rank == 0 && mine && e.y == token) {
+        d.token[row] = (int32_t)token;
+        if (d.weight) d.weight[row] = (int32_t)(all ? w : 0u);
+        if (d.mass) d.mass[row] = (int64_t)all;
+        if (d.kept) d.kept[row] = (int32_t)kept;
+      }
+      __syncwarp();
+      if (p.split > 1) r.sync();   // nobody still reads this CTA's list
+      return;
     }
+    cut = cut_by_count<RESIDENT>(r, s, (uint64_t)k, 0, (uint64_t)r.dist(lo) + 1);   // (hundreds of equal scores, or a large k)
   }
-  if (top_p < ONE && !listed) {
+  if (top_p < ONE) {
     if (r.wide) {
       const uint32_t w = cut.ties ? r.weight((uint32_t)cut.D) : 0u, ties = cut.ties;
-      cut = cut_by_weight(r, s, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
+      cut = cut_by_weight<RESIDENT>(r, s, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
     } else {
       // the elements that are left, by table entry
       uint32_t* const hist = s.hist;
@@ -557,13 +634,13 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       const uint32_t left = (uint32_t)min(cut.D, end - 1);
       const bool beyond = cut.D == end;
       if (beyond && r.gentle) {
-        r.each([&](int32_t v) {
+        r.each<RESIDENT>([&](int32_t v, int) {
           const uint32_t e = r.entry_of(v);
           if (e == r.last_entry) ++last;
           else atomicAdd(&hist[e], 1u);
         });
       } else {
-        r.each([&](int32_t v) {
+        r.each<RESIDENT>([&](int32_t v, int) {
           const uint32_t dj = r.dist(v), e = r.entry(dj);
           if (beyond || dj < left) {
             if (e == r.last_entry) ++last;
@@ -619,7 +696,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
           cut = {from, (uint32_t)wanted};
         } else if (wanted < size) {
           // (one digit, mostly: an entry is 2^16 / scale distances wide)
-          cut = cut_by_count(r, s, wanted, from, min(to, max((uint64_t)r.dist(lo) + 1, from + 1)));
+          cut = cut_by_count<RESIDENT>(r, s, wanted, from, min(to, max((uint64_t)r.dist(lo) + 1, from + 1)));
         } else if (to <= cut.D) {   // (all of the entry; the cut that was there may lie in it)
           cut = {to, 0};
         }
@@ -641,7 +718,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
       const int j = b * BLOCK + 4 * (i * 32 + lane);
-      v[i] = j < r.last ? *reinterpret_cast<const int4*>(x + j) : make_int4(0, 0, 0, 0);
+      v[i] = r.four<RESIDENT>(j, whole);
     }
     if (whole && beyond && r.gentle && plain_table) {   // (sixteen weights below 2^27 fit 32 bits)
       uint32_t sum = 0;
@@ -700,14 +777,12 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   kept = __reduce_add_sync(FULL, kept);
   if (lane == 0) s.kept[warp] = kept;
   __syncthreads();
-  constexpr int PER = (MAX_BLOCKS + 31) / 32;   // blocks a lane of warp 0
+  const int per_lane = (blocks + 31) / 32;      // blocks of a lane of warp 0
   uint64_t mass_in_front = 0;
   uint32_t ties_in_front = 0;                   // of the lane's blocks
   auto scan_blocks = [&]() {
     uint64_t m = 0, t = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane * PER + i < blocks) { m += s.block_mass[lane * PER + i]; t += s.block_ties[lane * PER + i]; }
+    for (int b = lane * per_lane; b < min((lane + 1) * per_lane, blocks); ++b) { m += s.block_mass[b]; t += s.block_ties[b]; }
     const uint64_t mi = warp_scan(m), ti = cut.ties ? warp_scan(t) : 0;
     mass_in_front = mi - m;
     ties_in_front = cut.ties ? (uint32_t)(ti - t) : 0u;
@@ -764,15 +839,13 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     uint32_t t = front_ties + ties_in_front;
     int hit = -1;
     if (!passed(m, t)) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int b = lane * PER + i;
-        if (hit >= 0 || b >= blocks) continue;
-        if (passed(m + s.block_mass[b], t + s.block_ties[b])) { hit = b; continue; }
+      for (int b = lane * per_lane; b < min((lane + 1) * per_lane, blocks); ++b) {
+        if (passed(m + s.block_mass[b], t + s.block_ties[b])) { hit = b; break; }
         m += s.block_mass[b];
         t += s.block_ties[b];
       }
     }
+    __syncwarp();
     const uint32_t who = __ballot_sync(FULL, hit >= 0);   // one lane of one CTA
     if (who) {
       const int from = __ffs(who) - 1;
@@ -784,7 +857,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
         const int j = b * BLOCK + 4 * (i * 32 + lane);
-        const int4 v = j < r.last ? *reinterpret_cast<const int4*>(x + j) : make_int4(0, 0, 0, 0);
+        const int4 v = r.four<RESIDENT>(j, false);
         const int32_t e[4] = {v.x, v.y, v.z, v.w};
         tie[i] = 0;
 #pragma unroll
@@ -864,17 +937,21 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   p.split = 1;
   while (p.split < 8 && (smem_of(p.split) > half || ((int64_t)d->rows * p.split * 2 <= 2 * sms && slice_of(p.split) > 2048))) p.split *= 2;
   if (const char* e = dev_env("CVM_B200_SAMPLE_SPLIT")) p.split = atoi(e);
+  bool resident = true;
+  if (const char* e = dev_env("CVM_B200_SAMPLE_STREAM")) resident = atoi(e) == 0;
   p.slice = slice_of(p.split);
-  const int smem = smem_of(p.split);
+  const int smem = resident ? smem_of(p.split) : (p.table_smem ? d->table_len * 4 : 0);
   int threads = smem > half ? 1024 : 512;
   if (const char* e = dev_env("CVM_B200_SAMPLE_THREADS")) threads = atoi(e);
   if (smem > room) { set_error("sample: too large"); return CVMK_ERR_ARG; }
 
   static bool attr_of_device[64] = {false};
   if (!attr_of_device[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (check_cuda(e, "cudaFuncSetAttribute(sample_kernel)")) return CVMK_ERR_CUDA;
+    for (auto k : {sample_kernel<true>, sample_kernel<false>}) {
+      cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+      if (check_cuda(e, "cudaFuncSetAttribute(sample_kernel)")) return CVMK_ERR_CUDA;
+    }
     attr_of_device[dev & 63] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -890,5 +967,5 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, sample_kernel, p), "sample_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, resident ? sample_kernel<true> : sample_kernel<false>, p), "sample_kernel launch");
 }
