@@ -150,6 +150,8 @@ struct Row {
   uint32_t min_weight;   // lighter elements are filtered out; 0 where the table has gone through that already
   uint32_t split;
   bool wide;             // the table lies in global memory
+  int table_at;          // else at this place of the dynamic shared memory (known to be that: a look-up in a pointer's memory is twice as slow)
+  __device__ __forceinline__ const int32_t* in_smem() const { return reinterpret_cast<const int32_t*>(dynamic_smem) + table_at; }
   // entry() in fewer instructions where scale <= 2^16 and the table lies in shared memory: scores below floor_x have the last
   // entry, as floor_x has, and above it (top - x) * scale is less than 2^31.
   bool gentle;
@@ -161,7 +163,7 @@ struct Row {
   // saturated = (2^32 - 1) / scale has a product above 2^31.
   __device__ __forceinline__ uint32_t entry(uint32_t d) const { return min(min(d, saturated) * scale >> 16, last_entry); }
   __device__ __forceinline__ uint32_t weight(uint32_t d) const {   // 0 where min_p filters it out
-    if (!wide) return (uint32_t)table[entry(d)];
+    if (!wide) return (uint32_t)in_smem()[entry(d)];
     const uint64_t q = (uint64_t)d * scale >> 16;
     const int32_t w = table[q < last_entry ? (uint32_t)q : last_entry];
     return w > 0 && (uint32_t)w >= min_weight ? (uint32_t)w : 0u;
@@ -218,6 +220,11 @@ struct Row {
     if (4 * g1 + tid < last) f(at[4 * g1 + tid], 4 * g1 + tid);
   }
 };
+
+// Sum over the warp of numbers below 2^45.
+__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
+  return __reduce_add_sync(FULL, (uint32_t)v & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(v >> 20)) << 20);
+}
 
 // Exclusive sum of v over the threads of the CTA, and the sum of all.
 __device__ __forceinline__ uint64_t block_scan(Shared& s, uint64_t v, uint64_t& total) {
@@ -394,7 +401,7 @@ __device__ uint32_t search_list(Shared& s, int n, uint32_t from, uint32_t to, ui
     const uint32_t at = place(warp);
     uint64_t sum = 0;
     for (int i = lane; i < n; i += 32) sum += key(s.all[i]) <= at ? s.all_weight[i] : 0u;   // (below 2^36)
-    sum = __reduce_add_sync(FULL, (uint32_t)sum & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(sum >> 20)) << 20);
+    sum = warp_sum(sum);
     if (lane == 0) s.reached[turn & 1][warp] = sum >= need;
     __syncthreads();
     const uint32_t mask = __ballot_sync(FULL, lane < warps && s.reached[turn & 1][lane]);
@@ -409,7 +416,42 @@ __device__ uint32_t search_list(Shared& s, int n, uint32_t from, uint32_t to, ui
 __device__ __forceinline__ uint64_t sum_of_list(const Shared& s, int n) {
   uint64_t sum = 0;
   for (int i = threadIdx.x & 31; i < n; i += 32) sum += s.all_weight[i];
-  return __reduce_add_sync(FULL, (uint32_t)sum & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(sum >> 20)) << 20);
+  return warp_sum(sum);
+}
+
+// The weights of the blocks b0, b0 + warps, .. < end of a row without a cut, all of whose places are valid, with a table of
+// weights below 2^27 (sixteen of them fit 32 bits) and above 0; returns how many elements the lane has seen.  A function of its
+// own, so that the registers hold the next block, on its way from global memory, and not what the kernel needs later.
+template <bool RESIDENT>
+__device__ __noinline__ uint32_t sum_blocks(const Row r, Shared& s, int b0, int end) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int4* const at = reinterpret_cast<const int4*>(RESIDENT ? resident() : r.x);
+  const int32_t* const table = r.in_smem();
+  int4 next[GROUPS];
+  const auto request = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) next[i] = at[b * (BLOCK / 4) + i * 32 + lane];
+  };
+  uint32_t seen = 0;
+  if (b0 < end) request(b0);
+  for (int b = b0; b < end; b += warps) {
+    int4 v[GROUPS];
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) v[i] = next[i];
+    if (b + warps < end) request(b + warps);
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i)
+      sum += (uint32_t)(table[r.entry_of(v[i].x)] + table[r.entry_of(v[i].y)]) + (uint32_t)(table[r.entry_of(v[i].z)] + table[r.entry_of(v[i].w)]);
+    const uint64_t mass = warp_sum(sum);
+    if (lane == 0) {
+      s.block_mass[b] = mass;
+      s.block_ties[b] = 0;
+    }
+    seen += BLOCK / 32;
+  }
+  __syncwarp();
+  return seen;
 }
 
 __device__ __forceinline__ int bits_of(uint64_t range) { return max(1, 64 - __clzll((long long)range)); }   // of the largest distance
@@ -469,7 +511,8 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   r.last_entry = (uint32_t)d.table_len - 1u;
   r.min_weight = (uint32_t)((min_p * (uint64_t)max(d.table[0], 0) + ONE - 1) >> 30);
   r.wide = !p.table_smem;
-  r.table = p.table_smem ? table_s : d.table;
+  r.table = d.table;
+  r.table_at = RESIDENT ? p.slice : 0;
   bool plain = true;   // all entries are above 0 and below 2^27
 #pragma unroll
   for (int i = 0; i < EARLY; ++i)
@@ -590,7 +633,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
         const uint32_t each = r.weight(at_d);
         uint64_t before = 0;
         for (int i = lane; i < n; i += 32) before += s.all[i].x < at_d ? s.all_weight[i] : 0u;
-        before = __reduce_add_sync(FULL, (uint32_t)before & 0xfffffu) + ((uint64_t)__reduce_add_sync(FULL, (uint32_t)(before >> 20)) << 20);
+        before = warp_sum(before);
         const uint32_t taken = (uint32_t)((need - before + each - 1) / each);
         if (at_d < cut.D || taken < cut.ties) {   // (else the cut of top_k stays)
           cut = {at_d, taken};
@@ -710,24 +753,22 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   uint32_t kept = 0;
   const uint32_t D32 = (uint32_t)min(cut.D, end - 1);
   const bool beyond = cut.D == end;
+  // (whole blocks from `whole0` to `whole1`)
+  const int whole0 = (r.first + BLOCK - 1) / BLOCK, whole1 = r.last / BLOCK;
+  const bool straight = beyond && r.gentle && plain_table;
+  if (straight) {
+    const int b0 = whole0 + (warp - whole0 % warps + warps) % warps;   // the warp's first of them
+    kept += sum_blocks<RESIDENT>(r, s, b0, whole1);
+  }
   for (int b = warp; b < blocks; b += warps) {
-    const bool whole = b * BLOCK >= r.first && (b + 1) * BLOCK <= r.last;
+    const bool whole = b >= whole0 && b < whole1;
+    if (straight && whole) continue;
     uint64_t mass = 0;
     uint32_t ties = 0;
     int4 v[GROUPS];
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-      const int j = b * BLOCK + 4 * (i * 32 + lane);
-      v[i] = r.four<RESIDENT>(j, whole);
-    }
-    if (whole && beyond && r.gentle && plain_table) {   // (sixteen weights below 2^27 fit 32 bits)
-      uint32_t sum = 0;
-#pragma unroll
-      for (int i = 0; i < GROUPS; ++i)
-        sum += (uint32_t)(r.table[r.entry_of(v[i].x)] + r.table[r.entry_of(v[i].y)]) + (uint32_t)(r.table[r.entry_of(v[i].z)] + r.table[r.entry_of(v[i].w)]);
-      mass = sum;
-      kept += BLOCK / 32;
-    } else if (whole && beyond) {
+    for (int i = 0; i < GROUPS; ++i) v[i] = r.four<RESIDENT>(b * BLOCK + 4 * (i * 32 + lane), whole);
+    if (whole && beyond) {
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
         const uint32_t w0 = r.weight(r.dist(v[i].x)), w1 = r.weight(r.dist(v[i].y)), w2 = r.weight(r.dist(v[i].z)), w3 = r.weight(r.dist(v[i].w));
@@ -766,11 +807,10 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       }
     }
     __syncwarp();
-    // a lane's sum is below 2^35
-    const uint32_t low = __reduce_add_sync(FULL, (uint32_t)mass & 0xfffffu), high = __reduce_add_sync(FULL, (uint32_t)(mass >> 20));
-    ties = __reduce_add_sync(FULL, ties);
+    mass = warp_sum(mass);
+    ties = cut.ties ? __reduce_add_sync(FULL, ties) : 0u;
     if (lane == 0) {
-      s.block_mass[b] = low + ((uint64_t)high << 20);
+      s.block_mass[b] = mass;
       s.block_ties[b] = ties;
     }
   }
@@ -868,16 +908,23 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
           tie[i] |= (valid && dj == cut.D ? 1u : 0u) << q;
         }
       }
+      // the 128 of them, and among these the lane
       bool done = false;
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
         if (done) continue;
         const uint64_t mine_mass = (uint64_t)w[i][0] + w[i][1] + w[i][2] + w[i][3];
         const uint32_t mine_ties = (uint32_t)__popc(tie[i]);
-        const uint64_t mass_to = warp_scan(mine_mass);
-        const uint32_t ties_to = (uint32_t)warp_scan(mine_ties);
-        uint64_t m1 = m + mass_to - mine_mass;
-        uint32_t t1 = t + ties_to - mine_ties;
+        const uint64_t mass_to = m + warp_sum(mine_mass);
+        const uint32_t ties_to = t + (cut.ties ? __reduce_add_sync(FULL, mine_ties) : 0u);
+        done = passed(mass_to, ties_to);
+        if (!done) {
+          m = mass_to;
+          t = ties_to;
+          continue;
+        }
+        uint64_t m1 = m + warp_scan(mine_mass) - mine_mass;
+        uint32_t t1 = t + (cut.ties ? (uint32_t)warp_scan(mine_ties) - mine_ties : 0u);
         if (!passed(m1, t1) && passed(m1 + mine_mass, t1 + mine_ties)) {
           int place = -1;
           uint32_t weight = 0;
@@ -896,9 +943,6 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
           if (d.mass) d.mass[row] = (int64_t)all;
           if (d.kept) d.kept[row] = (int32_t)all_kept;
         }
-        m += __shfl_sync(FULL, mass_to, 31);
-        t += __shfl_sync(FULL, ties_to, 31);
-        done = passed(m, t);
       }
     }
   }
