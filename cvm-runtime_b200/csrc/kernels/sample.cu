@@ -1,7 +1,8 @@
 // Sampling with temperature, top-k, min-p and top-p from given random numbers, in whole numbers (cvmk_sample).
 //
 // A row belongs to one CTA, or to a cluster of them with a contiguous slice each.  A slice is read once, by a bulk copy into
-// shared memory; every later pass over it reads it there.  What is left of a row after its filters is all elements with
+// shared memory, and every later pass reads it there; or, where there are so many rows that more of them at work are worth more
+// than that, each pass reads it from global memory (L2).  What is left of a row after its filters is all elements with
 // d = max - x < D and the first `ties` ones, in index order, with d = D: the filters only look for that cut, and neither sort
 // nor list the row.
 //   top_k   In a CTA, the n-th largest of the maxima of its threads is a lower bound of its n-th largest element (that many
@@ -977,17 +978,32 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   auto slice_of = [&](int split) { return ((d->vocab + 3 + split - 1) / split + 3) & ~3; };
   auto smem_of = [&](int split) { return slice_of(split) * 4 + (p.table_smem ? d->table_len * 4 : 0); };
+  // How many CTAs a row is cut over, and whether its slices are kept in shared memory.  The choice is by sizes, and by whether
+  // rows may be cut (top_k or top_p given); us of one call in a chain of calls, kept (k) or read again from L2 (g), CTAs a row:
+  //   - as many CTAs a row as are resident at once, two an SM (of clusters of eight 33, not 37: GPCs have 16 to 20 SMs), each with
+  //     4000 elements or more.  50021 elements, 64 rows, with cuts: k4 28, k8 44, g2 37; 150 rows without: g1 21, g2 30, k4 33.
+  //   - kept where two slices fit an SM.  131072 elements, 8 rows with cuts: k8 29, g8 35.  A CTA an SM, of 1024 threads, only
+  //     for the few rows of which all are resident then: 262144 elements, 8 rows with cuts: k8 31, g8 41; 37 rows 61 and 48.
+  //   - with cuts rows differ in how long they take, and more and shorter CTAs even that out: slices of 65536 at most.
+  //     262144 elements, 256 rows: g1 239, g2 207, g4 193, g8 260; 131072, 150 rows: g1 88, g2 66, g4 83.
   const int room = 226 * 1024 - (int)sizeof(Shared), half = 113 * 1024 - (int)sizeof(Shared) - 1024;
-  p.split = 1;
-  while (p.split < 8 && (smem_of(p.split) > half || ((int64_t)d->rows * p.split * 2 <= 2 * sms && slice_of(p.split) > 2048))) p.split *= 2;
+  const bool cuts = d->top_k || d->top_p;
+  static const int at_once[4] = {296, 148, 71, 33};   // clusters of 1, 2, 4 and 8 CTAs, two an SM; 148 SMs
+  int log2 = 0;
+  while (log2 < 3 && (int64_t)d->rows * 148 <= (int64_t)at_once[log2 + 1] * sms && slice_of(2 << log2) >= 4000) ++log2;
+  while (cuts && log2 < 3 && slice_of(1 << log2) > 65536 + 4) ++log2;
+  p.split = 1 << log2;
+  bool resident = smem_of(p.split) <= half;
+  int threads = 512;
+  if (!resident && p.split == 8 && d->rows <= 14 * sms / 148 && smem_of(8) <= room) {
+    resident = true;
+    threads = 1024;
+  }
   if (const char* e = dev_env("CVM_B200_SAMPLE_SPLIT")) p.split = atoi(e);
-  bool resident = true;
   if (const char* e = dev_env("CVM_B200_SAMPLE_STREAM")) resident = atoi(e) == 0;
+  if (const char* e = dev_env("CVM_B200_SAMPLE_THREADS")) threads = atoi(e);
   p.slice = slice_of(p.split);
   const int smem = resident ? smem_of(p.split) : (p.table_smem ? d->table_len * 4 : 0);
-  int threads = smem > half ? 1024 : 512;
-  if (const char* e = dev_env("CVM_B200_SAMPLE_THREADS")) threads = atoi(e);
-  if (smem > room) { set_error("sample: too large"); return CVMK_ERR_ARG; }
 
   static bool attr_of_device[64] = {false};
   if (!attr_of_device[dev & 63]) {

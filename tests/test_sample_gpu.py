@@ -82,7 +82,7 @@ def test_counts_of_rows(kn, rows):
     run(kn, logits(rng, rows, 3001, "normal"), EXP, rng.randint(10000, 60000, rows), rng.randint(0, 2**31, rows), **settings(rng, rows))
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 327680), (2, 300000), (2, 131072), (1, 50021), (30, 32000), (160, 70003)])
+@pytest.mark.parametrize("rows,vocab", [(1, 327680), (2, 300000), (2, 131072), (1, 50021), (30, 32000), (160, 70003), (40, 300000), (80, 150001)])
 def test_large_vocabularies(kn, rows, vocab):
     rng = np.random.RandomState(vocab)
     few = min(rows, 6)   # (the definition in Python takes a second a row: the rows behind are the first ones again)
@@ -92,6 +92,23 @@ def test_large_vocabularies(kn, rows, vocab):
     got = run(kn, x[again], EXP, 30000, 987654321, **{n: v[again] for n, v in s.items()}, check=False)
     for r in range(few):
         want = ref.sample_row(x[r], EXP, 30000, int(s["top_k"][r]), int(s["top_p"][r]), int(s["min_p"][r]), 987654321)
+        for i in range(r, rows, few):
+            assert tuple(int(g[i]) for g in got) == want
+
+
+# So many rows that slices are not kept in shared memory, at every place of a row against 16 bytes
+@pytest.mark.parametrize("skew", [0, 1, 2, 3])
+@pytest.mark.parametrize("filters", [False, True])
+def test_many_rows(kn, skew, filters):
+    rng = np.random.RandomState(skew)
+    few, rows, vocab = 5, 300, 20009
+    x = logits(rng, few, vocab, "normal")
+    s = settings(rng, few) if filters else dict(top_k=np.zeros(few), top_p=np.full(few, ONE), min_p=np.zeros(few))
+    scale, u, again = rng.randint(10000, 90000, few), rng.randint(0, 2**31, few), np.arange(rows) % few
+    given = {n: v[again] for n, v in s.items()} if filters else {}
+    got = run(kn, x[again], EXP, scale[again], u[again], **given, pad=skew, skew=skew, check=False)
+    for r in range(few):
+        want = ref.sample_row(x[r], EXP, int(scale[r]), int(s["top_k"][r]), int(s["top_p"][r]), int(s["min_p"][r]), int(u[r]))
         for i in range(r, rows, few):
             assert tuple(int(g[i]) for g in got) == want
 
