@@ -59,7 +59,7 @@ struct Params {
   int table_s_dtype;               // of the copy in shared memory
   DevChain cw, cv, cy;
   int straight;                    // 1: straight_part() takes the chains and the table, and the tensor operand if there is one
-  int io;                          // 1: and y, and that operand, go through shared memory by TMA
+  int io;                          // and y, and that operand, go through shared memory by TMA: 1 y in int8, 2 y in int32
   int tail;                        // 1: chain_y ends with an int8 tensor and a clip, which run on packed 16-bit words
   uint32_t tail_lo, tail_hi;       // the clip's bounds in both halves
   DevChain head;                   // chain_y without those two steps
@@ -463,39 +463,127 @@ __device__ __noinline__ void general_part(const Params& p, const Part t, bool fa
   __syncwarp();
 }
 
-// Both sides in the three-instruction form and an int8 table in shared memory.  IO: `staged` is the warp's piece of the tile as
-// it will lie in memory, 32 rows of t.columns bytes in the TMA swizzle of that width; RES: there the int8 operand of the tensor
-// step lies already.  Little code: what a tile's loop holds has to come to the SM's instruction cache.
-template <bool GATED, bool RES, bool IO>
-__device__ __forceinline__ void straight_part(const Params& p, const Part& t, const int8_t* table_s, uint8_t* staged) {
+// Both sides in the three-instruction form, and the table in shared memory (T32: in int32): the product of a chunk's sides.
+template <bool GATED, bool T32>
+__device__ __forceinline__ void straight_chunk(const Params& p, const Part& t, const uint8_t* table_s, int c, int32_t (&a)[16], int32_t (&b)[16]) {
+  if (GATED) tmem_ld_two(t.t0 + (uint32_t)c, t.t0 + 128u + (uint32_t)c, a, b);
+  else tmem_ld16(t.t0 + (uint32_t)c, a);
+  if (c + 16 >= t.columns) hand_back(t.acc_free);
+  requant(t.bias + c, p.qw, a);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) a[j] = T32 ? reinterpret_cast<const int32_t*>(table_s)[a[j]] : (int32_t) reinterpret_cast<const int8_t*>(table_s)[a[j]];
+  if (GATED) {
+    requant(t.bias + 32 + c, p.qv, b);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+  }
+}
+// `staged` is the warp's piece of the tile as it will lie in memory, 32 rows of t.columns bytes in the TMA swizzle of that width;
+// RES: there the int8 operand of the tensor step lies already.
+// Little code: what a tile's loop holds has to come to the SM's instruction cache.
+template <bool GATED, bool RES, bool T32>
+__device__ __forceinline__ void straight_part(const Params& p, const Part& t, const uint8_t* table_s, uint8_t* staged) {
   const int lane = threadIdx.x & 31;
   constexpr int COLUMNS = GATED ? 32 : 64;
 #pragma unroll 1
   for (int c = 0; c < COLUMNS; c += 16) {
     int32_t a[16], b[16];
-    if (GATED) tmem_ld_two(t.t0 + (uint32_t)c, t.t0 + 128u + (uint32_t)c, a, b);
-    else tmem_ld16(t.t0 + (uint32_t)c, a);
-    if (c + 16 >= COLUMNS) hand_back(t.acc_free);
-    requant(t.bias + c, p.qw, a);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) a[j] = table_s[a[j]];
-    if (GATED) {
-      requant(t.bias + 32 + c, p.qv, b);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
-    }
+    straight_chunk<GATED, T32>(p, t, table_s, c, a, b);
     apply_chain<16>(RES ? p.head : p.cy, a, 0, 0, 0);
-    if (IO) {
-      uint4* at = reinterpret_cast<uint4*>(staged + panel_offset(lane, c >> 4, COLUMNS));
-      *at = RES ? packed_tail(p, *at, a) : packed(a);
-    } else if (t.row < p.rows) {
-      const int unit = t.unit0 + c;
-      store_run(p.y, p.y_dtype, (long long)t.row * p.y_pitch + unit, min(16, p.units - unit), a);
+    uint4* at = reinterpret_cast<uint4*>(staged + panel_offset(lane, c >> 4, COLUMNS));
+    *at = RES ? packed_tail(p, *at, a) : packed(a);
+    __syncwarp();
+  }
+}
+// Results in int32: 16 columns at a time leave through `out`, 32 rows of 64 bytes in the TMA swizzle of that width, two
+// buffers in turn; `operand`: the int8 operand of the tensor step, as above.
+template <bool GATED, bool RES, bool T32>
+__device__ __noinline__ void wide_part(const Params& p, const Part t, const CUtensorMap* tmap_y, const uint8_t* table_s, const uint8_t* operand, uint8_t* out, bool live) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < t.columns; c += 16) {
+    int32_t a[16], b[16];
+    straight_chunk<GATED, T32>(p, t, table_s, c, a, b);
+    if (RES) {
+      const uint4 r = *reinterpret_cast<const uint4*>(operand + panel_offset(lane, c >> 4, GATED ? 32 : 64));
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) b[j] = (int32_t)(int8_t)(w[j >> 2] >> ((j & 3) * 8));
+    }
+    apply_chain<16, true>(p.cy, a, 0, 0, 0, b, p.res_step);
+    uint8_t* const to = out + ((c >> 4) & 1) * 2048;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // (what lay there has left)
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<int4*>(to + panel_offset(lane, q, 64)) = make_int4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0 && live && t.unit0 + c < p.units) tma_store_2d(tmap_y, to, t.unit0 + c, t.row);
+    if (lane == 0) tma_store_commit();
+  }
+}
+// The same where rows of y do not begin on 16 bytes, or the operand is int32: 16 columns at a time are turned through
+// `turn`, so that lanes read and write along rows, two rows a time (a lane that stores its own row touches 32 rows a time).
+constexpr int TURN_PITCH = 17;   // words of a row of 16
+template <bool GATED, bool RES, bool T32>
+__device__ __noinline__ void turned_part(const Params& p, const Part t, const uint8_t* table_s, int32_t* turn) {
+  const int lane = threadIdx.x & 31, col = lane & 15, half = lane >> 4, rows = p.rows - (t.row - lane) - half;   // left, from the lane's first on
+  const size_t step = 2 * (size_t)p.y_pitch;
+#pragma unroll 1
+  for (int c = 0; c < t.columns; c += 16) {
+    const int unit = t.unit0 + c + col;
+    const size_t lin = (size_t)(t.row - lane + half) * (size_t)p.y_pitch + unit;
+    const int mine = unit < p.units ? rows : 0;
+    int32_t a[16], b[16];
+    if (RES) {   // (the operand travels while the sums are waited for)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        b[i] = 2 * i < mine ? (p.res_dtype == CVMK_I8 ? (int32_t) reinterpret_cast<const int8_t*>(p.res)[lin + i * step]
+                                                      : reinterpret_cast<const int32_t*>(p.res)[lin + i * step]) : 0;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) turn[(2 * i + half) * TURN_PITCH + col] = b[i];
+    }
+    __syncwarp();
+    straight_chunk<GATED, T32>(p, t, table_s, c, a, b);
+    if (RES) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) b[j] = turn[lane * TURN_PITCH + j];
+      __syncwarp();
+    }
+    apply_chain<16, true>(p.cy, a, 0, 0, 0, b, p.res_step);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) turn[lane * TURN_PITCH + j] = a[j];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int32_t v = turn[(2 * i + half) * TURN_PITCH + col];
+      if (2 * i >= mine) continue;
+      if (p.y_dtype == CVMK_I8) reinterpret_cast<int8_t*>(p.y)[lin + i * step] = (int8_t)v;
+      else reinterpret_cast<int32_t*>(p.y)[lin + i * step] = v;
     }
     __syncwarp();
   }
 }
+template <bool T32>
+__device__ __forceinline__ void other_parts(const Params& p, const Part& t, const CUtensorMap* tmap_y, const uint8_t* table_s, uint8_t* staged, bool live) {
+  if (p.io == 2) {
+    uint8_t* const out = p.res ? staged + 2048 : staged;
+    if (p.res) p.gated ? wide_part<true, true, T32>(p, t, tmap_y, table_s, staged, out, live) : wide_part<false, true, T32>(p, t, tmap_y, table_s, staged, out, live);
+    else p.gated ? wide_part<true, false, T32>(p, t, tmap_y, table_s, staged, out, live) : wide_part<false, false, T32>(p, t, tmap_y, table_s, staged, out, live);
+  } else if (T32 && p.io) {
+    if (p.res) p.gated ? straight_part<true, true, true>(p, t, table_s, staged) : straight_part<false, true, true>(p, t, table_s, staged);
+    else p.gated ? straight_part<true, false, true>(p, t, table_s, staged) : straight_part<false, false, true>(p, t, table_s, staged);
+  } else {
+    int32_t* const turn = reinterpret_cast<int32_t*>(staged);
+    if (p.res) p.gated ? turned_part<true, true, T32>(p, t, table_s, turn) : turned_part<false, true, T32>(p, t, table_s, turn);
+    else p.gated ? turned_part<true, false, T32>(p, t, table_s, turn) : turned_part<false, false, T32>(p, t, table_s, turn);
+  }
+}
 
+// USUAL: results in int8 by TMA, a table of int8 in shared memory; the other forms are a kernel of their own, so that what they
+// need (calls, registers) costs the usual one nothing (ungated 6000 rows 2048 -> 8192 77.6 -> 73 us, gated 4096 rows 334 -> 321).
+template <bool USUAL>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_y,
@@ -600,13 +688,14 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue: a row a lane, a quarter of the columns a group of four warps
+    const int io = USUAL ? 1 : p.io;
     const int quarter = warp & 3, group = (warp - 2) >> 2, columns = tile_units / 4;   // 32 units, ungated 64
     const uint32_t acc_empty0 = map_rank(smem_u32(&bar_acc_empty[0]), 0);
     int32_t* const bias = bias_s[warp - 2];   // of w's columns, gated: 32 of w's and 32 of v's
     const int32_t* const bias2 = p.gated ? p.bias_v : p.bias_w;
     // the warp's piece of a tile on its way, in one buffer or (tensor operands, which come a tile early) two
     const int piece = 32 * columns;
-    uint8_t* const staged0 = smem + p.stages * PAIR_STAGE + (warp - 2) * piece * (p.res ? 2 : 1);
+    uint8_t* const staged0 = smem + p.stages * PAIR_STAGE + (warp - 2) * (io == 1 ? piece * (p.res ? 2 : 1) : (io ? (p.res ? 6144 : 4096) : 32 * TURN_PITCH * 4));
     uint32_t res_phase = 0;
     auto request = [&](int tile, int buffer) {   // (one lane)
       const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
@@ -615,7 +704,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
       mbar_expect_tx(&bar_res[warp - 2][buffer], (uint32_t)piece);
       tma_load_2d(staged0 + buffer * piece, &tmap_r, &bar_res[warp - 2][buffer], unit, row);
     };
-    if (p.io && p.res && lane == 0 && first < tiles) request(first, 0);
+    if (io && p.res && lane == 0 && first < tiles) request(first, 0);
     int i = 0;
     for (int tile = first; tile < tiles; tile += step, ++i) {
       const int acc = i & 1;
@@ -625,9 +714,9 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
       // what the tile needs beside the sums travels while the products are computed: the biases, and an int8 residual
       const int u1 = unit0 + lane, u2 = p.gated ? u1 : u1 + 32;
       const int32_t b1 = p.bias_w && u1 < p.units ? p.bias_w[u1] : 0, b2 = bias2 && u2 < p.units ? bias2[u2] : 0;
-      // (p.io: the operand of the next tile sets out into the buffer that the last tile's results have left)
+      // (p.io == 1: the operand of the next tile sets out into the buffer that the last tile's results have left)
       const bool live = warp_row < p.rows && unit0 < p.units;
-      if (p.io && lane == 0) {
+      if (io == 1 && lane == 0) {
         tma_store_wait_read();
         if (p.res && tile + step < tiles) request(tile + step, (i + 1) & 1);
       }
@@ -641,19 +730,23 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
       if (!__all_sync(FULL_MASK, mbar_wait(&bar_acc_full[acc], (uint32_t)((i >> 1) & 1), &abort_flag, 4))) break;
       tc_fence_after();
       const Part part = {row, unit0, columns, t0, acc_empty0 + 8u * (uint32_t)acc, bias, table_s};
-      const int buffer = p.res ? acc : 0;
+      const int buffer = io == 1 && p.res ? acc : 0;
       uint8_t* const staged = staged0 + buffer * piece;
-      const int8_t* const table8 = reinterpret_cast<const int8_t*>(table_s);
-      if (p.io && p.res && live) {
+      if (io && p.res && live) {
         if (!__all_sync(FULL_MASK, mbar_wait(&bar_res[warp - 2][buffer], (res_phase >> buffer) & 1u, &abort_flag, 5))) break;
         res_phase ^= 1u << buffer;
       }
       const bool straight = fast1 && fast2 && p.straight;
       if (!straight) general_part(p, part, fast1, fast2);
-      else if (p.io && p.res) p.gated ? straight_part<true, true, true>(p, part, table8, staged) : straight_part<false, true, true>(p, part, table8, staged);
-      else if (p.io) p.gated ? straight_part<true, false, true>(p, part, table8, staged) : straight_part<false, false, true>(p, part, table8, staged);
-      else p.gated ? straight_part<true, false, false>(p, part, table8, staged) : straight_part<false, false, false>(p, part, table8, staged);
-      if (straight && p.io) {
+      else if (USUAL && p.res) p.gated ? straight_part<true, true, false>(p, part, table_s, staged) : straight_part<false, true, false>(p, part, table_s, staged);
+      else if (USUAL) p.gated ? straight_part<true, false, false>(p, part, table_s, staged) : straight_part<false, false, false>(p, part, table_s, staged);
+      else if (p.table_s_dtype == CVMK_I8) other_parts<false>(p, part, &tmap_y, table_s, staged, live);
+      else other_parts<true>(p, part, &tmap_y, table_s, staged, live);
+      if (!USUAL && io == 2 && p.res) {   // (one buffer: the next operand may come once this one has been read)
+        __syncwarp();
+        if (lane == 0 && tile + step < tiles) request(tile + step, 0);
+      }
+      if (straight && io == 1) {
         fence_async_smem();
         __syncwarp();
         if (lane == 0 && live) {
@@ -662,7 +755,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         }
       }
     }
-    if (p.io && lane == 0) tma_store_wait_all();   // (shared memory goes with the CTA)
+    if (io && lane == 0) tma_store_wait_all();   // (shared memory goes with the CTA)
     __syncwarp();
   }
   if (abort_flag) {
@@ -701,13 +794,13 @@ int sm_count() {
   return sms;
 }
 
-// A row-major int8 matrix, in boxes of `box_cols` bytes of `box_rows` rows; zeros outside.
+// A row-major matrix of int8 (wide: int32), rows `pitch` elements apart, in boxes of `box_bytes` of `box_rows` rows; zeros outside.
 CUresult encode_matrix(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows, CUtensorMapL2promotion promo,
-                       int box_cols = BLOCK_K) {
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-  return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B), promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                       int box_bytes = BLOCK_K, bool wide = false) {
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * (wide ? 4 : 1)};
+  cuuint32_t box[2] = {(cuuint32_t)box_bytes / (wide ? 4 : 1), (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  return encoder()(map, wide ? CU_TENSOR_MAP_DATA_TYPE_INT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B), promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // The three-instruction form of a lowered chain from step `first` on, in front of a table of `len` entries or not (0).
@@ -814,14 +907,16 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
     plan->split = 1;
     // y in int8 leaves, and an int8 tensor operand comes, by TMA; a warp's piece of the tile waits in shared memory, twice with
     // an operand, for which the ring gives up two of its six stages
-    plan->io = p.y_dtype == CVMK_I8 && !((uintptr_t)p.y & 15) && p.y_pitch % 16 == 0;
+    const int wide = p.y_dtype == CVMK_I32;
+    plan->io = !((uintptr_t)p.y & 15) && p.y_pitch * p.y_dtype % 16 == 0 ? 1 + wide : 0;
     const void* operand = nullptr;
     for (int i = 0; i < p.chain_y.n; ++i)
       if (is_tensor_step(p.chain_y.s[i])) {
         operand = p.chain_y.s[i].ptr;
-        if (p.chain_y.s[i].ptr_dtype != CVMK_I8 || ((uintptr_t)operand & 15)) plan->io = 0;
+        if (p.chain_y.s[i].ptr_dtype != CVMK_I8 || ((uintptr_t)operand & 15) || p.y_pitch % 16) plan->io = 0;
       }
-    const int staged = plan->io ? 128 * (p.v ? 128 : 256) * (operand ? 2 : 1) : 0;
+    // (without it: room to turn 16 columns of a warp's rows)
+    const int staged = std::max(plan->io == 1 ? 128 * (p.v ? 128 : 256) * (operand ? 2 : 1) : (plan->io ? EPI_WARPS * (operand ? 6144 : 4096) : 0), EPI_WARPS * 32 * TURN_PITCH * 4);
     plan->stages = std::min(6, (PAIR_SMEM_MAX - 1024 - staged) / PAIR_STAGE);
     // (no other kernel's CTAs fit beside a pair: they could hold TMEM columns and wait for its end)
     plan->smem_bytes = std::max(1024 + plan->stages * PAIR_STAGE + staged, 206 * 1024);
@@ -829,7 +924,7 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
     plan->grid = 2 * (int)std::min<int64_t>(tiles, sms / 2);
     if (plan->io) {
       const int columns = p.v ? 32 : 64;
-      CUresult r = encode_matrix((CUtensorMap*)plan->tmap_y, p.y, p.rows, p.units, p.y_pitch, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE, columns);
+      CUresult r = encode_matrix((CUtensorMap*)plan->tmap_y, p.y, p.rows, p.units, p.y_pitch, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE, wide ? 64 : columns, wide);
       if (r == CUDA_SUCCESS && operand)
         r = encode_matrix((CUtensorMap*)plan->tmap_r, operand, p.rows, p.units, p.y_pitch, 32, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, columns);
       if (r != CUDA_SUCCESS) { set_error("dense_lut_prepare: tensor map rejected (CUresult %d)", (int)r); return CVMK_ERR_CUDA; }
@@ -908,9 +1003,10 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
       p.res = p.cy.s[i].ptr; p.res_dtype = p.cy.s[i].dt; p.res_step = i;
     }
 
-  p.straight = p.qw.on && (!p.gated || p.qv.on) && p.table_smem && p.table_s_dtype == CVMK_I8 && (!p.res || p.tail);
-  p.io = plan->io && p.straight;
-  if (p.res && !p.io) p.straight = 0;
+  p.straight = p.qw.on && (!p.gated || p.qv.on) && p.table_smem;
+  p.io = p.straight && (plan->io == 2 || (plan->io == 1 && (!p.res || p.tail))) ? plan->io : 0;
+
+  const bool usual = p.io == 1 && p.table_s_dtype == CVMK_I8;
 
   static bool attr_of_device[64] = {false};
   int dev = 0;
@@ -921,7 +1017,8 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
       return e == cudaSuccess ? cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100) : e;
     };
     if (check_cuda(allow(dense_lut_small_kernel, SMALL_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_small_kernel)") ||
-        check_cuda(allow(dense_lut_pair_kernel, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)"))
+        check_cuda(allow(dense_lut_pair_kernel<true>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
+        check_cuda(allow(dense_lut_pair_kernel<false>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)"))
       return CVMK_ERR_CUDA;
     attr_of_device[dev & 63] = true;
   }
@@ -944,6 +1041,6 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pair || plan->split > 1 ? 2 : 1;
-  if (pair) return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_pair_kernel, tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
+  if (pair) return check_cuda(cudaLaunchKernelEx(&cfg, usual ? dense_lut_pair_kernel<true> : dense_lut_pair_kernel<false>, tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
   return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_small_kernel, tx, tw, tv, p), "dense_lut_small_kernel launch");
 }

@@ -517,7 +517,7 @@ typedef struct __attribute__((aligned(64))) {
   int32_t split;        /* CTAs of a cluster that share a tile's reduction */
   int32_t row_tile;     /* rows of x a tile */
   int32_t table_smem;   /* bytes of the table kept in shared memory, 0: read where it lies */
-  int32_t io;           /* 1: y and an int8 tensor operand go through shared memory by TMA */
+  int32_t io;           /* y and an int8 tensor operand go through shared memory by TMA: 1 y in int8, 2 in int32 */
   int32_t reserved[4];
 } cvmk_dense_lut_plan;
 
