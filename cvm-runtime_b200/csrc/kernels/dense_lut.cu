@@ -427,8 +427,8 @@ __device__ __forceinline__ void hand_back(uint32_t acc_free) {
   if ((threadIdx.x & 31) == 0) arrive_at(acc_free);
 }
 
-// Everything that the straight form below does not take: step by step.
-__device__ __noinline__ void general_part(const Params& p, const Part t, bool fast_w, bool fast_v) {
+// Everything that the straight forms below do not take: step by step.
+__device__ __forceinline__ void general_part(const Params& p, const Part& t, bool fast_w, bool fast_v) {
 #pragma unroll 1
   for (int c = 0; c < t.columns; c += 16) {
     const int unit = t.unit0 + c, n = min(16, p.units - unit);
@@ -462,6 +462,10 @@ __device__ __noinline__ void general_part(const Params& p, const Part t, bool fa
   }
   __syncwarp();
 }
+
+// The same as a function of its own, for the kernels that need it only where a bias is so large that its sum might overflow.
+// (The launch's parameters are then read as memory, not as constants: a third of the speed.)
+__device__ __noinline__ void rare_part(const Params& p, const Part t, bool fast_w, bool fast_v) { general_part(p, t, fast_w, fast_v); }
 
 // Both sides in the three-instruction form, and the table in shared memory (T32: in int32): the product of a chunk's sides.
 template <bool GATED, bool T32>
@@ -498,7 +502,7 @@ __device__ __forceinline__ void straight_part(const Params& p, const Part& t, co
 // Results in int32: 16 columns at a time leave through `out`, 32 rows of 64 bytes in the TMA swizzle of that width, two
 // buffers in turn; `operand`: the int8 operand of the tensor step, as above.
 template <bool GATED, bool RES, bool T32>
-__device__ __noinline__ void wide_part(const Params& p, const Part t, const CUtensorMap* tmap_y, const uint8_t* table_s, const uint8_t* operand, uint8_t* out, bool live) {
+__device__ __forceinline__ void wide_part(const Params& p, const Part& t, const CUtensorMap* tmap_y, const uint8_t* table_s, const uint8_t* operand, uint8_t* out, bool live) {
   const int lane = threadIdx.x & 31;
 #pragma unroll 1
   for (int c = 0; c < t.columns; c += 16) {
@@ -526,7 +530,7 @@ __device__ __noinline__ void wide_part(const Params& p, const Part t, const CUte
 // `turn`, so that lanes read and write along rows, two rows a time (a lane that stores its own row touches 32 rows a time).
 constexpr int TURN_PITCH = 17;   // words of a row of 16
 template <bool GATED, bool RES, bool T32>
-__device__ __noinline__ void turned_part(const Params& p, const Part t, const uint8_t* table_s, int32_t* turn) {
+__device__ __forceinline__ void turned_part(const Params& p, const Part& t, const uint8_t* table_s, int32_t* turn) {
   const int lane = threadIdx.x & 31, col = lane & 15, half = lane >> 4, rows = p.rows - (t.row - lane) - half;   // left, from the lane's first on
   const size_t step = 2 * (size_t)p.y_pitch;
 #pragma unroll 1
@@ -565,25 +569,26 @@ __device__ __noinline__ void turned_part(const Params& p, const Part t, const ui
     __syncwarp();
   }
 }
-template <bool T32>
-__device__ __forceinline__ void other_parts(const Params& p, const Part& t, const CUtensorMap* tmap_y, const uint8_t* table_s, uint8_t* staged, bool live) {
-  if (p.io == 2) {
-    uint8_t* const out = p.res ? staged + 2048 : staged;
-    if (p.res) p.gated ? wide_part<true, true, T32>(p, t, tmap_y, table_s, staged, out, live) : wide_part<false, true, T32>(p, t, tmap_y, table_s, staged, out, live);
-    else p.gated ? wide_part<true, false, T32>(p, t, tmap_y, table_s, staged, out, live) : wide_part<false, false, T32>(p, t, tmap_y, table_s, staged, out, live);
-  } else if (T32 && p.io) {
-    if (p.res) p.gated ? straight_part<true, true, true>(p, t, table_s, staged) : straight_part<false, true, true>(p, t, table_s, staged);
-    else p.gated ? straight_part<true, false, true>(p, t, table_s, staged) : straight_part<false, false, true>(p, t, table_s, staged);
+// Which of these a kernel runs.  They are kernels of their own: together they need more registers than there are, and as functions
+// they read the launch's parameters as memory (6000 rows 2048 -> 8192 with a residual to int32: 192 us).
+enum Kind { USUAL, WIDE, TURNED, GENERAL };   // straight_part() with a table of int8; wide_part(), or straight_part() with a table of int32
+template <int KIND, bool GATED, bool RES>
+__device__ __forceinline__ void run_part(const Params& p, const Part& t, const CUtensorMap* tmap_y, const uint8_t* table_s, uint8_t* staged, bool live) {
+  if (KIND == USUAL) {
+    straight_part<GATED, RES, false>(p, t, table_s, staged);
+  } else if (KIND == WIDE) {
+    uint8_t* const out = RES ? staged + 2048 : staged;
+    if (p.io == 1) straight_part<GATED, RES, true>(p, t, table_s, staged);
+    else if (p.table_s_dtype == CVMK_I8) wide_part<GATED, RES, false>(p, t, tmap_y, table_s, staged, out, live);
+    else wide_part<GATED, RES, true>(p, t, tmap_y, table_s, staged, out, live);
+  } else if (p.table_s_dtype == CVMK_I8) {
+    turned_part<GATED, RES, false>(p, t, table_s, reinterpret_cast<int32_t*>(staged));
   } else {
-    int32_t* const turn = reinterpret_cast<int32_t*>(staged);
-    if (p.res) p.gated ? turned_part<true, true, T32>(p, t, table_s, turn) : turned_part<false, true, T32>(p, t, table_s, turn);
-    else p.gated ? turned_part<true, false, T32>(p, t, table_s, turn) : turned_part<false, false, T32>(p, t, table_s, turn);
+    turned_part<GATED, RES, true>(p, t, table_s, reinterpret_cast<int32_t*>(staged));
   }
 }
 
-// USUAL: results in int8 by TMA, a table of int8 in shared memory; the other forms are a kernel of their own, so that what they
-// need (calls, registers) costs the usual one nothing (ungated 6000 rows 2048 -> 8192 77.6 -> 73 us, gated 4096 rows 334 -> 321).
-template <bool USUAL>
+template <int KIND>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_y,
@@ -688,7 +693,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue: a row a lane, a quarter of the columns a group of four warps
-    const int io = USUAL ? 1 : p.io;
+    const int io = KIND == USUAL ? 1 : (KIND == WIDE ? p.io : 0);
     const int quarter = warp & 3, group = (warp - 2) >> 2, columns = tile_units / 4;   // 32 units, ungated 64
     const uint32_t acc_empty0 = map_rank(smem_u32(&bar_acc_empty[0]), 0);
     int32_t* const bias = bias_s[warp - 2];   // of w's columns, gated: 32 of w's and 32 of v's
@@ -737,12 +742,11 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         res_phase ^= 1u << buffer;
       }
       const bool straight = fast1 && fast2 && p.straight;
-      if (!straight) general_part(p, part, fast1, fast2);
-      else if (USUAL && p.res) p.gated ? straight_part<true, true, false>(p, part, table_s, staged) : straight_part<false, true, false>(p, part, table_s, staged);
-      else if (USUAL) p.gated ? straight_part<true, false, false>(p, part, table_s, staged) : straight_part<false, false, false>(p, part, table_s, staged);
-      else if (p.table_s_dtype == CVMK_I8) other_parts<false>(p, part, &tmap_y, table_s, staged, live);
-      else other_parts<true>(p, part, &tmap_y, table_s, staged, live);
-      if (!USUAL && io == 2 && p.res) {   // (one buffer: the next operand may come once this one has been read)
+      if (KIND == GENERAL) general_part(p, part, fast1, fast2);
+      else if (!straight) rare_part(p, part, fast1, fast2);
+      else if (p.res) p.gated ? run_part<KIND, true, true>(p, part, &tmap_y, table_s, staged, live) : run_part<KIND, false, true>(p, part, &tmap_y, table_s, staged, live);
+      else p.gated ? run_part<KIND, true, false>(p, part, &tmap_y, table_s, staged, live) : run_part<KIND, false, false>(p, part, &tmap_y, table_s, staged, live);
+      if (KIND == WIDE && io == 2 && p.res) {   // (one buffer: the next operand may come once this one has been read)
         __syncwarp();
         if (lane == 0 && tile + step < tiles) request(tile + step, 0);
       }
@@ -1006,7 +1010,7 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   p.straight = p.qw.on && (!p.gated || p.qv.on) && p.table_smem;
   p.io = p.straight && (plan->io == 2 || (plan->io == 1 && (!p.res || p.tail))) ? plan->io : 0;
 
-  const bool usual = p.io == 1 && p.table_s_dtype == CVMK_I8;
+  const int kind = !p.straight ? GENERAL : (!p.io ? TURNED : (p.io == 1 && p.table_s_dtype == CVMK_I8 ? USUAL : WIDE));
 
   static bool attr_of_device[64] = {false};
   int dev = 0;
@@ -1017,8 +1021,10 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
       return e == cudaSuccess ? cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100) : e;
     };
     if (check_cuda(allow(dense_lut_small_kernel, SMALL_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_small_kernel)") ||
-        check_cuda(allow(dense_lut_pair_kernel<true>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
-        check_cuda(allow(dense_lut_pair_kernel<false>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)"))
+        check_cuda(allow(dense_lut_pair_kernel<USUAL>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
+        check_cuda(allow(dense_lut_pair_kernel<WIDE>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
+        check_cuda(allow(dense_lut_pair_kernel<TURNED>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
+        check_cuda(allow(dense_lut_pair_kernel<GENERAL>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)"))
       return CVMK_ERR_CUDA;
     attr_of_device[dev & 63] = true;
   }
@@ -1041,6 +1047,10 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pair || plan->split > 1 ? 2 : 1;
-  if (pair) return check_cuda(cudaLaunchKernelEx(&cfg, usual ? dense_lut_pair_kernel<true> : dense_lut_pair_kernel<false>, tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
+  if (pair) {
+    static void (*const kernels[])(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Params) = {
+        dense_lut_pair_kernel<USUAL>, dense_lut_pair_kernel<WIDE>, dense_lut_pair_kernel<TURNED>, dense_lut_pair_kernel<GENERAL>};
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernels[kind], tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
+  }
   return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_small_kernel, tx, tw, tv, p), "dense_lut_small_kernel launch");
 }
