@@ -2,7 +2,7 @@
 // products of int8 operands whose int32 sums never leave the chip.
 //
 // dense_lut_small_kernel: the weights are the 128-row operand of the tensor instructions and the rows of x
-// (up to 256 of them) its columns, so a launch is one stream of weights whatever the batch.  A gated tile is
+// (up to 128 of them) its columns, so a launch is one stream of weights whatever the batch.  A gated tile is
 // 64 units: 64 rows of w and under them the same 64 of v, so that one accumulator holds both products of a
 // unit; ungated, 128 units of w.  The reduction of a tile can be cut over a cluster of CTAs: every CTA
 // writes its partial sums (int32: exact in any order) to its shared memory and each finishes its share of the
@@ -123,6 +123,44 @@ __device__ __forceinline__ void copy_table(const Params& p, uint8_t* table_s, in
   }
 }
 
+// Whether the bias leaves room for the sum (see Requant).
+__device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) {
+  const long long b = (long long)bias + q.add;
+  return b <= q.room && b >= -(long long)q.room;
+}
+// One channel's sums; `bias` has q.add in it.
+template <int V>
+__device__ __forceinline__ void requant_one(int32_t bias, const Requant& q, int32_t (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = max(__viaddmin_s32(v[j], bias, q.hi), q.lo) >> q.shift;
+}
+// V sums at `at` of every CTA of the cluster, added up.  (A word of another CTA takes a fifth of a microsecond to come: the
+// requests go out together.)
+template <int V>
+__device__ __forceinline__ void sum_ranks(const Params& p, uint32_t at, int32_t (&a)[V]) {
+  constexpr int AT_ONCE = 16 / V;   // CTAs
+#pragma unroll
+  for (int j = 0; j < V; ++j) a[j] = 0;
+#pragma unroll
+  for (int s0 = 0; s0 < 8; s0 += AT_ONCE) {
+    if (s0 >= p.split) break;
+    int4 g[AT_ONCE][V / 4];
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s)
+      if (s0 + s < p.split) {
+        const uint32_t from = p.split > 1 ? map_rank(at, (uint32_t)(s0 + s)) : at;
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) g[s][q] = load_remote(from + 16 * q);
+      }
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s)
+      if (s0 + s < p.split) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) { a[4 * q] += g[s][q].x; a[4 * q + 1] += g[s][q].y; a[4 * q + 2] += g[s][q].z; a[4 * q + 3] += g[s][q].w; }
+      }
+  }
+}
+
 // bytes of one row of partial sums: 16 more than the sums, so that eight rows of one column lie in different banks
 __host__ __device__ inline int sums_pitch(int row_tile) { return row_tile * 4 + 16; }
 __host__ __device__ inline int small_ring_bytes(int row_tile, int stages) {
@@ -130,6 +168,9 @@ __host__ __device__ inline int small_ring_bytes(int row_tile, int stages) {
   return ring > sums ? ring : sums;
 }
 
+// JOB: rows of x that a thread finishes at a time, 4 or 8 (few rows: more threads at work; many: fewer instructions an element:
+// 256 rows 256 -> 8192 21.6 us with 4, 13.2 with 8; 8 rows 4096 -> 4096 7.7 and 8.7).
+template <int JOB>
 __global__ void __launch_bounds__(THREADS)
 dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                        const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Params p) {
@@ -145,8 +186,7 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int rank = uniform(p.split > 1 ? (int)cluster_rank() : 0);
   const int tile = (int)blockIdx.x >> p.split_log2;
-  const int ut = tile / p.row_tiles, row0 = (tile - ut * p.row_tiles) * p.row_tile;
-  const int tile_units = p.gated ? 64 : 128, unit0 = ut * tile_units;
+  const int tile_units = p.gated ? 64 : 128, unit0 = tile * tile_units;
   const int kb0 = (rank * p.kblocks) >> p.split_log2, mine = (((rank + 1) * p.kblocks) >> p.split_log2) - kb0;
   const int stage_bytes = W_BYTES + p.row_tile * BLOCK_K;
   uint8_t* const table_s = smem + small_ring_bytes(p.row_tile, p.stages);
@@ -160,7 +200,7 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
     tma_load_2d(smem + s * stage_bytes, &tmap_w, &bar_full[s], col, unit0);
     tma_load_2d(smem + s * stage_bytes + W_BYTES / 2, p.gated ? &tmap_v : &tmap_w, &bar_full[s], col, p.gated ? unit0 : unit0 + 64);
   };
-  auto load_x = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + W_BYTES, &tmap_x, &bar_full[s], (kb0 + kb) * BLOCK_K, row0); };
+  auto load_x = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + W_BYTES, &tmap_x, &bar_full[s], (kb0 + kb) * BLOCK_K, 0); };
   const int first = min(p.stages, mine);
   if (warp == 0) {
     if (leader) {
@@ -252,44 +292,48 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
     tc_fence_after();
     tmem_dealloc(tmem_base, (uint32_t)p.tmem_cols);
   }
-  // This CTA's share of the units, four rows of x a thread and turn.
+  // This CTA's share of the units, JOB rows of x a thread and turn.
   if (!abort_flag) {
     pdl_wait();
-    const int share = tile_units >> p.split_log2, jobs = share * (p.row_tile >> 2);
+    const int share = tile_units >> p.split_log2, jobs = share * ((p.row_tile + JOB - 1) / JOB);
     for (int k = (int)threadIdx.x; k < jobs; k += THREADS) {
-      const int q = k / share, ul = rank * share + k - q * share, unit = unit0 + ul, r0 = row0 + 4 * q;
+      const int q = k / share, ul = rank * share + k - q * share, unit = unit0 + ul, r0 = JOB * q;
       if (unit >= p.units || r0 >= p.rows) continue;
-      int32_t a[4], b[4];
-      const uint32_t at = ring + (uint32_t)(ul * pitch + 16 * q), at_v = at + (uint32_t)(64 * pitch);
-      const int32_t ba = bias_s[ul], bb = bias_s[p.gated ? ul + 64 : ul];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { a[j] = ba; b[j] = bb; }
-      for (int s = 0; s < p.split; ++s) {
-        const int4 g = load_remote(p.split > 1 ? map_rank(at, (uint32_t)s) : at);
-        a[0] += g.x; a[1] += g.y; a[2] += g.z; a[3] += g.w;
-        if (p.gated) {
-          const int4 h = load_remote(p.split > 1 ? map_rank(at_v, (uint32_t)s) : at_v);
-          b[0] += h.x; b[1] += h.y; b[2] += h.z; b[3] += h.w;
-        }
-      }
-      const int n = min(4, p.rows - r0);
+      const int n = min(JOB, p.rows - r0);
       const long long lin = (long long)r0 * p.y_pitch + unit;
-      int32_t pre[4] = {0, 0, 0, 0};
+      int32_t a[JOB], b[JOB], pre[JOB] = {};
       if (p.res) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < JOB; ++j)
           if (j < n) pre[j] = p.res_dtype == CVMK_I8 ? reinterpret_cast<const int8_t*>(p.res)[lin + j * p.y_pitch]
                                                      : reinterpret_cast<const int32_t*>(p.res)[lin + j * p.y_pitch];
       }
-      activate<4>(p, table_s, a);
-      if (p.gated) {
-        apply_chain<4>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+      const uint32_t at = ring + (uint32_t)(ul * pitch + 4 * JOB * q), at_v = at + (uint32_t)(64 * pitch);
+      const int32_t ba = bias_s[ul], bb = bias_s[p.gated ? ul + 64 : ul];
+      sum_ranks(p, at, a);
+      if (p.gated) sum_ranks(p, at_v, b);
+      if (p.qw.on && in_room(ba, p.qw)) {
+        requant_one(ba + p.qw.add, p.qw, a);
+        look_up<JOB>(p, table_s, a);
+      } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+        for (int j = 0; j < JOB; ++j) a[j] += ba;
+        activate<JOB>(p, table_s, a);
       }
-      apply_chain<4, true>(p.cy, a, 0, 0, 0, pre, p.res_step);
+      if (p.gated) {
+        if (p.qv.on && in_room(bb, p.qv)) {
+          requant_one(bb + p.qv.add, p.qv, b);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < JOB; ++j) b[j] += bb;
+          apply_chain<JOB>(p.cv, b, 0, 0, 0, nullptr, -1, p.first_v);
+        }
+#pragma unroll
+        for (int j = 0; j < JOB; ++j) a[j] = (int32_t)((uint32_t)a[j] * (uint32_t)b[j]);
+      }
+      apply_chain<JOB, true>(p.cy, a, 0, 0, 0, pre, p.res_step);
+#pragma unroll
+      for (int j = 0; j < JOB; ++j)
         if (j < n) {
           if (p.y_dtype == CVMK_I8) reinterpret_cast<int8_t*>(p.y)[lin + j * p.y_pitch] = (int8_t)a[j];
           else reinterpret_cast<int32_t*>(p.y)[lin + j * p.y_pitch] = a[j];
@@ -392,10 +436,6 @@ __device__ __forceinline__ void add_bias(const int32_t* bias_s, int32_t (&v)[16]
   }
 }
 
-__device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) {
-  const long long b = (long long)bias + q.add;
-  return b <= q.room && b >= -(long long)q.room;
-}
 __device__ __forceinline__ void requant(const int32_t* bias_s, const Requant& q, int32_t (&v)[16]) {   // biases with q.add in them
   const int hi = q.hi, lo = q.lo, sh = q.shift;
 #pragma unroll
@@ -526,15 +566,19 @@ __device__ __forceinline__ void wide_part(const Params& p, const Part& t, const 
     if (lane == 0) tma_store_commit();
   }
 }
-// The same where rows of y do not begin on 16 bytes, or the operand is int32: 16 columns at a time are turned through
-// `turn`, so that lanes read and write along rows, two rows a time (a lane that stores its own row touches 32 rows a time).
-constexpr int TURN_PITCH = 17;   // words of a row of 16
+// The same where rows of y do not begin on 16 bytes, or the operand is int32.  Lanes read and write along rows (a lane that works
+// on its own row touches 32 rows a time): 16 columns of the operand, and of results in int32, are turned through `turn`, two rows
+// a time; results in int8 wait in `piece` and leave as whole words, wherever a row begins against four bytes, and a few bytes.
+constexpr int TURN_PITCH = 17;   // words of a row of 16, or of 64 bytes
+constexpr int TURN_BYTES = 32 * TURN_PITCH * 4;
 template <bool GATED, bool RES, bool T32>
-__device__ __forceinline__ void turned_part(const Params& p, const Part& t, const uint8_t* table_s, int32_t* turn) {
+__device__ __forceinline__ void turned_part(const Params& p, const Part& t, const uint8_t* table_s, uint32_t* piece, int32_t* turn) {
+  constexpr int COLUMNS = GATED ? 32 : 64;
   const int lane = threadIdx.x & 31, col = lane & 15, half = lane >> 4, rows = p.rows - (t.row - lane) - half;   // left, from the lane's first on
   const size_t step = 2 * (size_t)p.y_pitch;
+  const bool narrow = p.y_dtype == CVMK_I8;
 #pragma unroll 1
-  for (int c = 0; c < t.columns; c += 16) {
+  for (int c = 0; c < COLUMNS; c += 16) {
     const int unit = t.unit0 + c + col;
     const size_t lin = (size_t)(t.row - lane + half) * (size_t)p.y_pitch + unit;
     const int mine = unit < p.units ? rows : 0;
@@ -556,19 +600,45 @@ __device__ __forceinline__ void turned_part(const Params& p, const Part& t, cons
       __syncwarp();
     }
     apply_chain<16, true>(p.cy, a, 0, 0, 0, b, p.res_step);
+    if (narrow) {
+      const uint4 w = packed(a);
+      uint32_t* const to = piece + lane * TURN_PITCH + (c >> 2);
+      to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
+      continue;
+    }
 #pragma unroll
     for (int j = 0; j < 16; ++j) turn[lane * TURN_PITCH + j] = a[j];
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int32_t v = turn[(2 * i + half) * TURN_PITCH + col];
-      if (2 * i >= mine) continue;
-      if (p.y_dtype == CVMK_I8) reinterpret_cast<int8_t*>(p.y)[lin + i * step] = (int8_t)v;
-      else reinterpret_cast<int32_t*>(p.y)[lin + i * step] = v;
-    }
+    for (int i = 0; i < 16; ++i)
+      if (2 * i < mine) reinterpret_cast<int32_t*>(p.y)[lin + i * step] = turn[(2 * i + half) * TURN_PITCH + col];
     __syncwarp();
   }
+  __syncwarp();
+  const int n = min(COLUMNS, p.units - t.unit0);   // bytes of a row
+  if (!narrow || n <= 0) return;
+  uint8_t* const y0 = reinterpret_cast<uint8_t*>(p.y) + (size_t)(t.row - lane) * (size_t)p.y_pitch + t.unit0;
+  auto bytes_in_front = [](const uint8_t* at) { return (int)(-reinterpret_cast<uintptr_t>(at) & 3); };   // of the first whole word
+  uint8_t* at = y0 + (size_t)half * (size_t)p.y_pitch;
+  for (int i = 0; i < 16; ++i, at += step) {
+    const int head = bytes_in_front(at);
+    if (2 * i < rows && 4 * col + 4 <= n - head) {
+      const uint32_t* const from = piece + (2 * i + half) * TURN_PITCH + col;
+      *reinterpret_cast<uint32_t*>(at + head + 4 * col) = __funnelshift_r(from[0], from[1], 8 * head);
+    }
+  }
+  if (t.row < p.rows) {   // what is left at the ends of the lane's row
+    uint8_t* const mine = y0 + (size_t)lane * (size_t)p.y_pitch;
+    const uint8_t* const from = reinterpret_cast<const uint8_t*>(piece + lane * TURN_PITCH);
+    const int head = min(bytes_in_front(mine), n), tail = head + ((n - head) & ~3);
+    for (int e = 0; e < 3; ++e) {
+      if (e < head) mine[e] = from[e];
+      if (tail + e < n) mine[tail + e] = from[tail + e];
+    }
+  }
+  __syncwarp();
 }
+
 // Which of these a kernel runs.  They are kernels of their own: together they need more registers than there are, and as functions
 // they read the launch's parameters as memory (6000 rows 2048 -> 8192 with a residual to int32: 192 us).
 enum Kind { USUAL, WIDE, TURNED, GENERAL };   // straight_part() with a table of int8; wide_part(), or straight_part() with a table of int32
@@ -582,9 +652,9 @@ __device__ __forceinline__ void run_part(const Params& p, const Part& t, const C
     else if (p.table_s_dtype == CVMK_I8) wide_part<GATED, RES, false>(p, t, tmap_y, table_s, staged, out, live);
     else wide_part<GATED, RES, true>(p, t, tmap_y, table_s, staged, out, live);
   } else if (p.table_s_dtype == CVMK_I8) {
-    turned_part<GATED, RES, false>(p, t, table_s, reinterpret_cast<int32_t*>(staged));
+    turned_part<GATED, RES, false>(p, t, table_s, reinterpret_cast<uint32_t*>(staged), reinterpret_cast<int32_t*>(staged + TURN_BYTES));
   } else {
-    turned_part<GATED, RES, true>(p, t, table_s, reinterpret_cast<int32_t*>(staged));
+    turned_part<GATED, RES, true>(p, t, table_s, reinterpret_cast<uint32_t*>(staged), reinterpret_cast<int32_t*>(staged + TURN_BYTES));
   }
 }
 
@@ -700,7 +770,7 @@ dense_lut_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     const int32_t* const bias2 = p.gated ? p.bias_v : p.bias_w;
     // the warp's piece of a tile on its way, in one buffer or (tensor operands, which come a tile early) two
     const int piece = 32 * columns;
-    uint8_t* const staged0 = smem + p.stages * PAIR_STAGE + (warp - 2) * (io == 1 ? piece * (p.res ? 2 : 1) : (io ? (p.res ? 6144 : 4096) : 32 * TURN_PITCH * 4));
+    uint8_t* const staged0 = smem + p.stages * PAIR_STAGE + (warp - 2) * (io == 1 ? piece * (p.res ? 2 : 1) : (io ? (p.res ? 6144 : 4096) : 2 * TURN_BYTES));
     uint32_t res_phase = 0;
     auto request = [&](int tile, int buffer) {   // (one lane)
       const int ut = tile / p.row_tiles, rt = tile - ut * p.row_tiles;
@@ -866,6 +936,70 @@ const char* refusal(const cvmk_dense_lut_desc& d) {
   return nullptr;
 }
 
+// What the kernels are given, from a plan whose tile sizes, table_smem and io are set.
+int make_params(const cvmk_dense_lut_plan& plan, Params* out) {
+  Params& p = *out;
+  memset(&p, 0, sizeof(p));
+  const cvmk_dense_lut_desc& d = plan.d;
+  p.y = d.y; p.y_pitch = d.y_pitch; p.y_dtype = d.y_dtype;
+  p.rows = d.rows; p.units = d.units;
+  p.kblocks = (d.K + BLOCK_K - 1) / BLOCK_K;
+  p.gated = d.v != nullptr;
+  p.params_static = d.params_static;
+  const bool pair = plan.kernel == 1;
+  const int tile_units = (p.gated ? 64 : 128) * (pair ? 2 : 1);
+  p.unit_tiles = (d.units + tile_units - 1) / tile_units;
+  p.row_tile = plan.row_tile;
+  p.row_tiles = (d.rows + p.row_tile - 1) / p.row_tile;
+  p.stages = plan.stages;
+  p.split = plan.split;
+  while ((1 << p.split_log2) < p.split) ++p.split_log2;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.row_tile) p.tmem_cols *= 2;
+  p.table = d.table; p.table_len = d.table_len; p.table_dtype = d.table_dtype; p.table_smem = plan.table_smem;
+  p.status = d.status;
+  int rc = lower_chain(d.chain_w, &p.cw);
+  if (!rc) rc = lower_chain(d.chain_v, &p.cv);
+  if (!rc) rc = lower_chain(d.chain_y, &p.cy);
+  if (rc) return rc;
+  if (p.cw.n && p.cw.s[0].op == K_ADD_C) { p.bias_w = (const int32_t*)p.cw.s[0].ptr; p.first_w = 1; }
+  if (p.cv.n && p.cv.s[0].op == K_ADD_C) { p.bias_v = (const int32_t*)p.cv.s[0].ptr; p.first_v = 1; }
+  p.qw = requant_of(p.cw, p.first_w, d.table_len, d.K);
+  p.qv = requant_of(p.cv, p.first_v, 0, d.K);
+  // Ungated, the first steps of chain_y are functions of a table entry: the copy of the table goes through them.
+  p.table_s_dtype = d.table_dtype;
+  if (!p.gated && p.table_smem) {
+    while (p.ct.n < p.cy.n && !is_tensor_op(p.cy.s[p.ct.n].op)) { p.ct.s[p.ct.n] = p.cy.s[p.ct.n]; ++p.ct.n; }
+    if (p.ct.n) p.table_s_dtype = to_int8(p.ct.s[p.ct.n - 1]) ? CVMK_I8 : CVMK_I32;
+    if (p.table_s_dtype * (int64_t)d.table_len > p.table_smem) {   // (wider than the room the plan has for it)
+      p.ct.n = 0;
+      p.table_s_dtype = d.table_dtype;
+    }
+    for (int i = p.ct.n; i < p.cy.n; ++i) p.cy.s[i - p.ct.n] = p.cy.s[i];
+    p.cy.n -= p.ct.n;
+  }
+  const int at = p.cy.n - 2;
+  if (at >= 0 && is_tensor_op(p.cy.s[at].op) && p.cy.s[at].dt == CVMK_I8 && p.cy.s[at + 1].op == K_CLIP && d.y_dtype == CVMK_I8 &&
+      p.cy.s[at + 1].a >= -32767 && p.cy.s[at + 1].b <= 32767 &&
+      (at ? to_int8(p.cy.s[at - 1]) : !p.gated && p.table_s_dtype == CVMK_I8)) {
+    p.tail = 1;
+    p.head = p.cy;
+    p.head.n = at;
+    p.tail_lo = both_halves(p.cy.s[at + 1].a);
+    p.tail_hi = both_halves(p.cy.s[at + 1].b);
+  }
+  p.res_step = -1;
+  for (int i = 0; i < p.cy.n; ++i)
+    if (is_tensor_op(p.cy.s[i].op)) {
+      p.res = p.cy.s[i].ptr; p.res_dtype = p.cy.s[i].dt; p.res_step = i;
+    }
+
+  p.straight = p.qw.on && (!p.gated || p.qv.on) && p.table_smem;
+  p.io = p.straight && (plan.io == 2 || (plan.io == 1 && (!p.res || p.tail))) ? plan.io : 0;
+
+  return CVMK_OK;
+}
+
 }  // namespace
 }  // namespace cvmk
 
@@ -905,7 +1039,11 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   const int64_t table_bytes = (int64_t)p.table_len * p.table_dtype;
   plan->table_smem = table_bytes <= TABLE_SMEM_MAX ? (int)table_bytes : 0;
   const int table_room = (plan->table_smem + 15) & ~15;
-  plan->kernel = p.rows > 256 ? 1 : 0;
+  // More than 128 rows go to pairs of CTAs (us, small kernel | pairs, gated: 256 -> 8192 64 rows 6.7 | 7.7, 130 rows 10.3 | 8.0;
+  // 1024 -> 2777 64 rows 12.8 | 12.0, 130 rows 12.4 | 12.2; 4096 -> 500, where the small one cuts the reduction, 130 rows
+  // 13.1 | 18.6, 256 rows 19.5 | 18.7; 4096 -> 8192 130 rows 21.0 | 20.0, 256 rows 29.7 | 20.3).
+  plan->kernel = p.rows > 128 ? 1 : 0;
+  if (const char* e = dev_env("CVM_B200_DL_KERNEL")) plan->kernel = atoi(e);
   if (plan->kernel == 1) {
     plan->row_tile = 256;
     plan->split = 1;
@@ -919,8 +1057,11 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
         operand = p.chain_y.s[i].ptr;
         if (p.chain_y.s[i].ptr_dtype != CVMK_I8 || ((uintptr_t)operand & 15) || p.y_pitch % 16) plan->io = 0;
       }
-    // (without it: room to turn 16 columns of a warp's rows)
-    const int staged = std::max(plan->io == 1 ? 128 * (p.v ? 128 : 256) * (operand ? 2 : 1) : (plan->io ? EPI_WARPS * (operand ? 6144 : 4096) : 0), EPI_WARPS * 32 * TURN_PITCH * 4);
+    Params q;
+    if (const int rc = make_params(*plan, &q)) return rc;
+    plan->io = q.io;
+    const int staged = plan->io == 1 ? 128 * (p.v ? 128 : 256) * (operand ? 2 : 1)
+                     : EPI_WARPS * (plan->io ? (operand ? 6144 : 4096) : (q.straight ? 2 * TURN_BYTES : 0));
     plan->stages = std::min(6, (PAIR_SMEM_MAX - 1024 - staged) / PAIR_STAGE);
     // (no other kernel's CTAs fit beside a pair: they could hold TMEM columns and wait for its end)
     plan->smem_bytes = std::max(1024 + plan->stages * PAIR_STAGE + staged, 206 * 1024);
@@ -935,13 +1076,19 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
     }
     return encode_operands(plan, 128, 128);
   }
-  const int row_tiles = (p.rows + 255) / 256;
-  plan->row_tile = ((p.rows + row_tiles - 1) / row_tiles + 15) & ~15;
-  const int64_t unit_tiles = (p.units + tile_units - 1) / tile_units, tiles = unit_tiles * row_tiles;
-  const int per_sm = plan->row_tile <= 64 ? 2 : 1, limit = per_sm == 2 ? 112 * 1024 : SMALL_SMEM_MAX;
+  plan->row_tile = (p.rows + 15) & ~15;
+  const int64_t tiles = (p.units + tile_units - 1) / tile_units;
+  // Two CTAs an SM for few rows, whose loads then overlap the other one's last steps; one with all of its memory for more (64 rows
+  // 4096 -> 4096 gated 15.4 and 12.7 us).  A tile's reduction is cut while three quarters of the SMs have no tile and every part is
+  // left 16 blocks of K: the exchange takes 2 to 3 us (8 rows 4096 -> 4096: whole 11.1, in two 9.5, in four 8.7; 64 rows 1024 ->
+  // 4096: whole 7.2, in two 9.5; 1 row 2048 -> 8192 gated: whole 9.3, in two 10.2).
+  int per_sm = plan->row_tile <= 32 ? 2 : 1;
+  if (const char* e = dev_env("CVM_B200_DL_PERSM")) per_sm = atoi(e);
+  const int limit = per_sm == 2 ? 112 * 1024 : SMALL_SMEM_MAX;
   plan->split = 1;
-  while (plan->split < 8 && kblocks >= 4 * plan->split && tiles * 2 * plan->split <= (int64_t)per_sm * sms) plan->split *= 2;
+  while (plan->split < 8 && kblocks >= 16 * plan->split && tiles * plan->split * 4 <= (int64_t)3 * sms) plan->split *= 2;
   auto smem_of = [&](int stages) { return 1024 + small_ring_bytes(plan->row_tile, stages) + table_room; };
+  if (const char* e = dev_env("CVM_B200_DL_SPLIT")) plan->split = atoi(e);
   plan->stages = std::min((kblocks + plan->split - 1) / plan->split, MAX_STAGES);
   while (plan->stages > 2 && smem_of(plan->stages) > limit) --plan->stages;
   // (26 KB and more: beside a pair of CTAs of conv_tc_kernel, which takes its TMEM columns on two SMs, nothing of this kernel fits)
@@ -956,60 +1103,8 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   const cvmk_dense_lut_desc& d = plan->d;
   if (d.rows == 0) return CVMK_OK;
   Params p;
-  memset(&p, 0, sizeof(p));
-  p.y = d.y; p.y_pitch = d.y_pitch; p.y_dtype = d.y_dtype;
-  p.rows = d.rows; p.units = d.units;
-  p.kblocks = (d.K + BLOCK_K - 1) / BLOCK_K;
-  p.gated = d.v != nullptr;
-  p.params_static = d.params_static;
+  if (const int rc = make_params(*plan, &p)) return rc;
   const bool pair = plan->kernel == 1;
-  const int tile_units = (p.gated ? 64 : 128) * (pair ? 2 : 1);
-  p.unit_tiles = (d.units + tile_units - 1) / tile_units;
-  p.row_tile = plan->row_tile;
-  p.row_tiles = (d.rows + p.row_tile - 1) / p.row_tile;
-  p.stages = plan->stages;
-  p.split = plan->split;
-  while ((1 << p.split_log2) < p.split) ++p.split_log2;
-  p.tmem_cols = 32;
-  while (p.tmem_cols < p.row_tile) p.tmem_cols *= 2;
-  p.table = d.table; p.table_len = d.table_len; p.table_dtype = d.table_dtype; p.table_smem = plan->table_smem;
-  p.status = d.status;
-  if (lower_chain(d.chain_w, &p.cw) || lower_chain(d.chain_v, &p.cv) || lower_chain(d.chain_y, &p.cy)) return CVMK_ERR_ARG;
-  if (p.cw.n && p.cw.s[0].op == K_ADD_C) { p.bias_w = (const int32_t*)p.cw.s[0].ptr; p.first_w = 1; }
-  if (p.cv.n && p.cv.s[0].op == K_ADD_C) { p.bias_v = (const int32_t*)p.cv.s[0].ptr; p.first_v = 1; }
-  p.qw = requant_of(p.cw, p.first_w, d.table_len, d.K);
-  p.qv = requant_of(p.cv, p.first_v, 0, d.K);
-  // Ungated, the first steps of chain_y are functions of a table entry: the copy of the table goes through them.
-  p.table_s_dtype = d.table_dtype;
-  if (!p.gated && p.table_smem) {
-    while (p.ct.n < p.cy.n && !is_tensor_op(p.cy.s[p.ct.n].op)) { p.ct.s[p.ct.n] = p.cy.s[p.ct.n]; ++p.ct.n; }
-    if (p.ct.n) p.table_s_dtype = to_int8(p.ct.s[p.ct.n - 1]) ? CVMK_I8 : CVMK_I32;
-    if (p.table_s_dtype * (int64_t)d.table_len > p.table_smem) {   // (wider than the room the plan has for it)
-      p.ct.n = 0;
-      p.table_s_dtype = d.table_dtype;
-    }
-    for (int i = p.ct.n; i < p.cy.n; ++i) p.cy.s[i - p.ct.n] = p.cy.s[i];
-    p.cy.n -= p.ct.n;
-  }
-  const int at = p.cy.n - 2;
-  if (at >= 0 && is_tensor_op(p.cy.s[at].op) && p.cy.s[at].dt == CVMK_I8 && p.cy.s[at + 1].op == K_CLIP && d.y_dtype == CVMK_I8 &&
-      p.cy.s[at + 1].a >= -32767 && p.cy.s[at + 1].b <= 32767 &&
-      (at ? to_int8(p.cy.s[at - 1]) : !p.gated && p.table_s_dtype == CVMK_I8)) {
-    p.tail = 1;
-    p.head = p.cy;
-    p.head.n = at;
-    p.tail_lo = both_halves(p.cy.s[at + 1].a);
-    p.tail_hi = both_halves(p.cy.s[at + 1].b);
-  }
-  p.res_step = -1;
-  for (int i = 0; i < p.cy.n; ++i)
-    if (is_tensor_op(p.cy.s[i].op)) {
-      p.res = p.cy.s[i].ptr; p.res_dtype = p.cy.s[i].dt; p.res_step = i;
-    }
-
-  p.straight = p.qw.on && (!p.gated || p.qv.on) && p.table_smem;
-  p.io = p.straight && (plan->io == 2 || (plan->io == 1 && (!p.res || p.tail))) ? plan->io : 0;
-
   const int kind = !p.straight ? GENERAL : (!p.io ? TURNED : (p.io == 1 && p.table_s_dtype == CVMK_I8 ? USUAL : WIDE));
 
   static bool attr_of_device[64] = {false};
@@ -1020,7 +1115,8 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
       const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
       return e == cudaSuccess ? cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100) : e;
     };
-    if (check_cuda(allow(dense_lut_small_kernel, SMALL_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_small_kernel)") ||
+    if (check_cuda(allow(dense_lut_small_kernel<4>, SMALL_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_small_kernel)") ||
+        check_cuda(allow(dense_lut_small_kernel<8>, SMALL_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_small_kernel)") ||
         check_cuda(allow(dense_lut_pair_kernel<USUAL>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
         check_cuda(allow(dense_lut_pair_kernel<WIDE>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
         check_cuda(allow(dense_lut_pair_kernel<TURNED>, PAIR_SMEM_MAX), "cudaFuncSetAttribute(dense_lut_pair_kernel)") ||
@@ -1052,5 +1148,5 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
         dense_lut_pair_kernel<USUAL>, dense_lut_pair_kernel<WIDE>, dense_lut_pair_kernel<TURNED>, dense_lut_pair_kernel<GENERAL>};
     return check_cuda(cudaLaunchKernelEx(&cfg, kernels[kind], tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
   }
-  return check_cuda(cudaLaunchKernelEx(&cfg, dense_lut_small_kernel, tx, tw, tv, p), "dense_lut_small_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, plan->row_tile <= 32 ? dense_lut_small_kernel<4> : dense_lut_small_kernel<8>, tx, tw, tv, p), "dense_lut_small_kernel launch");
 }
