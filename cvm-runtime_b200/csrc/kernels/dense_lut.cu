@@ -186,7 +186,8 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int rank = uniform(p.split > 1 ? (int)cluster_rank() : 0);
   const int tile = (int)blockIdx.x >> p.split_log2;
-  const int tile_units = p.gated ? 64 : 128, unit0 = tile * tile_units;
+  const int ut = tile / p.row_tiles, row0 = (tile - ut * p.row_tiles) * p.row_tile;
+  const int tile_units = p.gated ? 64 : 128, unit0 = ut * tile_units;
   const int kb0 = (rank * p.kblocks) >> p.split_log2, mine = (((rank + 1) * p.kblocks) >> p.split_log2) - kb0;
   const int stage_bytes = W_BYTES + p.row_tile * BLOCK_K;
   uint8_t* const table_s = smem + small_ring_bytes(p.row_tile, p.stages);
@@ -200,7 +201,7 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
     tma_load_2d(smem + s * stage_bytes, &tmap_w, &bar_full[s], col, unit0);
     tma_load_2d(smem + s * stage_bytes + W_BYTES / 2, p.gated ? &tmap_v : &tmap_w, &bar_full[s], col, p.gated ? unit0 : unit0 + 64);
   };
-  auto load_x = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + W_BYTES, &tmap_x, &bar_full[s], (kb0 + kb) * BLOCK_K, 0); };
+  auto load_x = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + W_BYTES, &tmap_x, &bar_full[s], (kb0 + kb) * BLOCK_K, row0); };
   const int first = min(p.stages, mine);
   if (warp == 0) {
     if (leader) {
@@ -297,7 +298,7 @@ dense_lut_small_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
     pdl_wait();
     const int share = tile_units >> p.split_log2, jobs = share * ((p.row_tile + JOB - 1) / JOB);
     for (int k = (int)threadIdx.x; k < jobs; k += THREADS) {
-      const int q = k / share, ul = rank * share + k - q * share, unit = unit0 + ul, r0 = JOB * q;
+      const int q = k / share, ul = rank * share + k - q * share, unit = unit0 + ul, r0 = row0 + JOB * q;
       if (unit >= p.units || r0 >= p.rows) continue;
       const int n = min(JOB, p.rows - r0);
       const long long lin = (long long)r0 * p.y_pitch + unit;
@@ -894,6 +895,46 @@ Requant requant_of(const DevChain& c, int first, int len, int K) {
   return {1, (int)add, (int)lo, (int)hi, rs.d, (int)room};
 }
 
+// Which kernel runs a layer, and how the small one cuts it (rows of x a tile, CTAs that share its reduction): every cut, and the
+// pairs of CTAs, are given a time, and the least of them is taken.  The terms, in microseconds of a launch in a chain of launches
+// (of 40 shapes, 1 to 2000 rows, 176 to 8192 long, 35 to 16384 units, each cut timed; most are within 10 %):
+//   small   4 for the launch, 0.045 a row of the tile for its last steps, 0.19 a block of K (a load's latency, a ring of several
+//           in flight), all operands at 8 MB a microsecond out of L2 and the weights at 6 out of memory, 1.1 for the exchange
+//           of partial sums; times the rounds of CTAs, two an SM up to 32 rows and one beyond, and of clusters as many as
+//           are resident at once (GPCs have 16 to 20 SMs).
+//   pairs   5.3 for the launch (6.8 where rows of y do not begin on 16 bytes), 0.1 a block of K to fill the ring, and a round of
+//           tiles the longer of 0.28 a block and 2.7 for its last steps.
+// Cut over rows, a layer of few units uses the whole GPU: 128 rows 176 -> 122 14.8 us in one tile of rows and 5.4 in eight, 1000
+// rows 1024 -> 250 gated 6.2 in 63 (pairs 11.1).  Cut in K: 8 rows 4096 -> 4096 whole 10.6, in four 7.5.
+struct Cut { int row_tile, split; };   // split 0: pairs
+Cut choose(const cvmk_dense_lut_desc& d, int kblocks, int sms) {
+  const double weights = (double)d.units * d.K * (d.v ? 2 : 1);
+  const int64_t pair_tiles = (int64_t)((d.rows + 255) / 256) * ((d.units + (d.v ? 127 : 255)) / (d.v ? 128 : 256)), pairs = sms / 2;
+  const bool aligned = !((uintptr_t)d.y & 15) && d.y_pitch * d.y_dtype % 16 == 0;
+  Cut best = {256, 0};
+  double least = (aligned ? 5.3 : 6.8) + 0.1 * kblocks + std::max((pair_tiles + pairs - 1) / pairs * std::max(0.28 * kblocks, 2.7), weights / 6e6);
+  static const int at_once[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};   // clusters of 1, 2, 4 and 8 CTAs, one and two an SM; 148 SMs
+  for (int row_tile = 16; row_tile <= 128; row_tile *= 2) {
+    const int rt = std::min(row_tile, (std::min(d.rows, 128) + 15) & ~15);
+    const int64_t tiles = (int64_t)((d.units + (d.v ? 63 : 127)) / (d.v ? 64 : 128)) * ((d.rows + rt - 1) / rt);
+    for (int log2 = 0; log2 < 4 && (log2 == 0 || kblocks >= 4 << log2); ++log2) {
+      const int split = 1 << log2, per = (kblocks + split - 1) / split;
+      const int64_t room = std::max<int64_t>((int64_t)at_once[rt <= 32][log2] * sms / 148, 1), rounds = (tiles + room - 1) / room;
+      const double bytes = (double)tiles * split * per * (W_BYTES + rt * BLOCK_K);
+      const double us = 4.0 + 0.045 * rt * rounds + std::max({0.19 * per * rounds, bytes / 8e6, weights / 6e6}) + (split > 1 ? 1.1 : 0.0);
+      if (us < least) {
+        least = us;
+        best = {rt, split};
+      }
+    }
+    if (rt < row_tile) break;
+  }
+  if (const char* e = dev_env("CVM_B200_DL_KERNEL")) best = atoi(e) ? Cut{256, 0} : (best.split ? best : Cut{128, 1});
+  if (const char* e = dev_env("CVM_B200_DL_ROWTILE")) best.row_tile = atoi(e);
+  if (const char* e = dev_env("CVM_B200_DL_SPLIT")) best.split = atoi(e);
+  return best;
+}
+
 // Values that a step leaves within 8 bits, whatever it is given.
 bool to_int8(const DevStep& s) {
   if (s.op == K_CLIP) return s.a >= -128 && s.b <= 127;
@@ -1039,11 +1080,8 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   const int64_t table_bytes = (int64_t)p.table_len * p.table_dtype;
   plan->table_smem = table_bytes <= TABLE_SMEM_MAX ? (int)table_bytes : 0;
   const int table_room = (plan->table_smem + 15) & ~15;
-  // More than 128 rows go to pairs of CTAs (us, small kernel | pairs, gated: 256 -> 8192 64 rows 6.7 | 7.7, 130 rows 10.3 | 8.0;
-  // 1024 -> 2777 64 rows 12.8 | 12.0, 130 rows 12.4 | 12.2; 4096 -> 500, where the small one cuts the reduction, 130 rows
-  // 13.1 | 18.6, 256 rows 19.5 | 18.7; 4096 -> 8192 130 rows 21.0 | 20.0, 256 rows 29.7 | 20.3).
-  plan->kernel = p.rows > 128 ? 1 : 0;
-  if (const char* e = dev_env("CVM_B200_DL_KERNEL")) plan->kernel = atoi(e);
+  const Cut cut = choose(p, kblocks, sms);
+  plan->kernel = cut.split == 0;
   if (plan->kernel == 1) {
     plan->row_tile = 256;
     plan->split = 1;
@@ -1076,19 +1114,11 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
     }
     return encode_operands(plan, 128, 128);
   }
-  plan->row_tile = (p.rows + 15) & ~15;
-  const int64_t tiles = (p.units + tile_units - 1) / tile_units;
-  // Two CTAs an SM for few rows, whose loads then overlap the other one's last steps; one with all of its memory for more (64 rows
-  // 4096 -> 4096 gated 15.4 and 12.7 us).  A tile's reduction is cut while three quarters of the SMs have no tile and every part is
-  // left 16 blocks of K: the exchange takes 2 to 3 us (8 rows 4096 -> 4096: whole 11.1, in two 9.5, in four 8.7; 64 rows 1024 ->
-  // 4096: whole 7.2, in two 9.5; 1 row 2048 -> 8192 gated: whole 9.3, in two 10.2).
-  int per_sm = plan->row_tile <= 32 ? 2 : 1;
-  if (const char* e = dev_env("CVM_B200_DL_PERSM")) per_sm = atoi(e);
-  const int limit = per_sm == 2 ? 112 * 1024 : SMALL_SMEM_MAX;
-  plan->split = 1;
-  while (plan->split < 8 && kblocks >= 16 * plan->split && tiles * plan->split * 4 <= (int64_t)3 * sms) plan->split *= 2;
+  plan->row_tile = cut.row_tile;
+  plan->split = cut.split;
+  const int64_t tiles = (int64_t)((p.units + tile_units - 1) / tile_units) * ((p.rows + plan->row_tile - 1) / plan->row_tile);
+  const int limit = plan->row_tile <= 32 ? 112 * 1024 : SMALL_SMEM_MAX;
   auto smem_of = [&](int stages) { return 1024 + small_ring_bytes(plan->row_tile, stages) + table_room; };
-  if (const char* e = dev_env("CVM_B200_DL_SPLIT")) plan->split = atoi(e);
   plan->stages = std::min((kblocks + plan->split - 1) / plan->split, MAX_STAGES);
   while (plan->stages > 2 && smem_of(plan->stages) > limit) --plan->stages;
   // (26 KB and more: beside a pair of CTAs of conv_tc_kernel, which takes its TMEM columns on two SMs, nothing of this kernel fits)
@@ -1105,6 +1135,7 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
   Params p;
   if (const int rc = make_params(*plan, &p)) return rc;
   const bool pair = plan->kernel == 1;
+  const int tile_units = p.gated ? 64 : 128;   // of the small kernel
   const int kind = !p.straight ? GENERAL : (!p.io ? TURNED : (p.io == 1 && p.table_s_dtype == CVMK_I8 ? USUAL : WIDE));
 
   static bool attr_of_device[64] = {false};
@@ -1148,5 +1179,5 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
         dense_lut_pair_kernel<USUAL>, dense_lut_pair_kernel<WIDE>, dense_lut_pair_kernel<TURNED>, dense_lut_pair_kernel<GENERAL>};
     return check_cuda(cudaLaunchKernelEx(&cfg, kernels[kind], tx, tw, tv, ty, tr, p), "dense_lut_pair_kernel launch");
   }
-  return check_cuda(cudaLaunchKernelEx(&cfg, plan->row_tile <= 32 ? dense_lut_small_kernel<4> : dense_lut_small_kernel<8>, tx, tw, tv, p), "dense_lut_small_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, tile_units / p.split * p.row_tile < 8 * THREADS ? dense_lut_small_kernel<4> : dense_lut_small_kernel<8>, tx, tw, tv, p), "dense_lut_small_kernel launch");
 }
