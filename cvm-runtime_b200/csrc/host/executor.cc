@@ -8,6 +8,13 @@
 #include <map>
 #include <thread>
 
+// Weak: where a device has no such launcher (the executor is tested on one made of host memory) the operators stay apart.
+extern "C" {
+__attribute__((weak)) int cvmk_dense_lut_supported(const cvmk_dense_lut_desc* d);
+__attribute__((weak)) int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_lut_plan* plan);
+__attribute__((weak)) int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_stream_t stream);
+}
+
 namespace cvm {
 
 #define CUDA_OK(expr)                                                                      \
@@ -935,6 +942,162 @@ struct Lowering {
     }
   }
 
+  // ---------------------------------------------------------------- feed-forward blocks
+  // A dense layer, or two of the same input, up to the element-wise operators behind a table look-up (cvm_lut) of the one and
+  // their product (broadcast_mul): one launch of cvmk_dense_lut_*, whose results are those of the operators one by one.
+  struct Side {
+    uint32_t dense;
+    std::vector<uint32_t> nodes;       // behind it
+    cvmk_epilogue before, after;       // scalar steps in front of the table (or of everything, without one) and behind it
+    uint32_t lut = UINT32_MAX;         // the node, if there is one
+    uint32_t end_eid;                  // what they compute
+  };
+  // The only consumer of an entry that nothing else reads, UINT32_MAX without one.
+  uint32_t only_consumer(uint32_t eid, uint32_t after) const {
+    if (is_head[eid] || uses[eid] != 1) return UINT32_MAX;
+    for (uint32_t nid = after + 1; nid < g.nodes.size(); ++nid)
+      for (const auto& e : g.nodes[nid].inputs)
+        if (g.entry_id(e) == eid) return absorbed[nid] ? UINT32_MAX : nid;
+    return UINT32_MAX;
+  }
+  static bool is_tensor_step(const cvmk_ep_step& st) { return st.op == CVMK_EP_ADD_T || st.op == CVMK_EP_SUB_T || st.op == CVMK_EP_RSUB_T; }
+  bool dense_side(uint32_t nid, Side* side) {
+    const Node& n = g.nodes[nid];
+    if (n.is_variable() || absorbed[nid] || n.op->name != "dense" || !g.params.count(g.entry_id(n.inputs[1]))) return false;
+    const bool use_bias = n.attrs.b("use_bias");
+    if (use_bias && !g.params.count(g.entry_id(n.inputs[2]))) return false;
+    side->dense = nid;
+    memset(&side->before, 0, sizeof(side->before));
+    memset(&side->after, 0, sizeof(side->after));
+    if (use_bias) side->before.s[side->before.n++].op = CVMK_EP_ADD_C;   // (its operand when the launch is made)
+    side->end_eid = g.entry_id(nid, 0);
+    uint32_t last = nid;
+    for (;;) {
+      const uint32_t next = only_consumer(side->end_eid, last);
+      if (next == UINT32_MAX) break;
+      const Node& c = g.nodes[next];
+      cvmk_epilogue& chain = side->lut == UINT32_MAX ? side->before : side->after;
+      cvmk_ep_step st;
+      if (c.op->name == "cvm_lut" && side->lut == UINT32_MAX && g.entry_id(c.inputs[0]) == side->end_eid && g.params.count(g.entry_id(c.inputs[1]))) {
+        side->lut = next;
+      } else if (chain.n < CVMK_MAX_EP_STEPS && node_as_step(next, side->end_eid, &st) && !is_tensor_step(st)) {
+        chain.s[chain.n++] = st;
+      } else {
+        break;
+      }
+      side->nodes.push_back(next);
+      side->end_eid = g.entry_id(next, 0);
+      last = next;
+    }
+    return true;
+  }
+  bool lower_dense_lut(uint32_t nid) {
+    if (!cvmk_dense_lut_supported || !cvmk_dense_lut_prepare || !cvmk_dense_lut_launch || !input_writers.empty() || dev_env("CVM_B200_NO_DENSE_LUT")) return false;
+    Side first, second;
+    if (!dense_side(nid, &first)) return false;
+    const uint32_t x_eid = g.entry_id(g.nodes[nid].inputs[0]);
+    const Shape& shape = g.shape[g.entry_id(nid, 0)];
+    std::vector<uint32_t> taken = first.nodes;
+    uint32_t tail = first.end_eid, last = first.nodes.empty() ? nid : first.nodes.back();
+    // gated: the product with another dense layer of the same input, exactly one of the two through a table
+    const uint32_t mul = only_consumer(first.end_eid, last);
+    bool gated = false;
+    if (mul != UINT32_MAX && g.nodes[mul].op->name == "broadcast_mul") {
+      const uint32_t e0 = g.entry_id(g.nodes[mul].inputs[0]), e1 = g.entry_id(g.nodes[mul].inputs[1]);
+      const uint32_t other = e0 == first.end_eid ? e1 : e0;
+      for (uint32_t m = nid + 1; !gated && e0 != e1 && m < mul; ++m) {
+        Side s;
+        if (dense_side(m, &s) && s.end_eid == other && g.entry_id(g.nodes[m].inputs[0]) == x_eid && g.shape[g.entry_id(m, 0)] == shape &&
+            (s.lut != UINT32_MAX) != (first.lut != UINT32_MAX)) {
+          second = s;
+          gated = true;
+        }
+      }
+      if (gated) {
+        taken.push_back(second.dense);
+        taken.insert(taken.end(), second.nodes.begin(), second.nodes.end());
+        taken.push_back(mul);
+        tail = g.entry_id(mul, 0);
+        last = mul;
+        if (first.lut == UINT32_MAX) std::swap(first, second);
+      }
+    }
+    if (first.lut == UINT32_MAX) return false;
+    for (const uint32_t t : taken)
+      if (g.shape[g.entry_id(t, 0)] != shape) return false;
+    // what follows: scalar steps and one sum with a tensor
+    cvmk_dense_lut_desc d;
+    memset(&d, 0, sizeof(d));
+    int tensors = 0;
+    if (!gated) d.chain_y = first.after;
+    while (d.chain_y.n < CVMK_MAX_EP_STEPS) {
+      const uint32_t next = only_consumer(tail, last);
+      cvmk_ep_step st;
+      if (next == UINT32_MAX || !node_as_step(next, tail, &st) || (is_tensor_step(st) && tensors == 1)) break;
+      tensors += is_tensor_step(st);
+      d.chain_y.s[d.chain_y.n++] = st;
+      taken.push_back(next);
+      tail = g.entry_id(next, 0);
+      last = next;
+    }
+    const HostTensor& table = g.params.find(g.entry_id(g.nodes[first.lut].inputs[1]))->second;
+    const bool narrow = safe8[g.entry_id(g.nodes[first.lut].inputs[1])];
+    d.rows = (int32_t)shape[0]; d.units = (int32_t)shape[1]; d.K = (int32_t)g.shape[x_eid][1];
+    d.y_dtype = buf[tail].dtype;
+    d.table_len = (int32_t)table.data.size();
+    d.table_dtype = narrow ? CVMK_I8 : CVMK_I32;
+    d.params_static = 1;
+    d.chain_w = first.before;
+    d.x = d.w = (const int8_t*)16;   // (sizes, types and chains decide)
+    if (gated) { d.chain_v = second.before; d.v = d.w; }
+    for (int i = 0; i < d.chain_y.n; ++i)
+      if (is_tensor_step(d.chain_y.s[i])) d.chain_y.s[i].ptr_dtype = buf[(uint32_t)((uintptr_t)d.chain_y.s[i].ptr - 1)].dtype;
+    if (!cvmk_dense_lut_supported(&d)) return false;
+
+    auto upload = [&](const HostTensor& t, bool as8) {
+      void* at = ex.dalloc(t.data.size() * (as8 ? 1 : 4));
+      if (as8) {
+        const std::vector<int8_t> v8(t.data.begin(), t.data.end());
+        CUDA_OK(cudaMemcpy(at, v8.data(), v8.size(), cudaMemcpyHostToDevice));
+      } else {
+        CUDA_OK(cudaMemcpy(at, t.data.data(), t.data.size() * 4, cudaMemcpyHostToDevice));
+      }
+      return at;
+    };
+    auto weights = [&](const Side& s) { return (const int8_t*)upload(g.params.find(g.entry_id(g.nodes[s.dense].inputs[1]))->second, true); };
+    auto bind_bias = [&](const Side& s, cvmk_epilogue* chain) {
+      if (chain->n && chain->s[0].op == CVMK_EP_ADD_C) chain->s[0].ptr = bias_vector(g.entry_id(g.nodes[s.dense].inputs[2]));
+    };
+    for (const uint32_t t : taken) absorbed[t] = 1;
+    const std::string label = "dense_lut:" + g.nodes[first.lut].name();
+    bind_chain(&d.chain_y);
+    bind_bias(first, &d.chain_w);
+    if (gated) bind_bias(second, &d.chain_v);
+    const DevBuf xin = i8_view(x_eid, label);
+    const DevBuf out = materialize(tail);
+    d.x = (const int8_t*)xin.ptr;
+    d.w = weights(first);
+    d.v = gated ? weights(second) : nullptr;
+    d.y = out.ptr;
+    d.status = ex.status_dev_;
+    d.table = upload(table, narrow);
+    if (gated && first.after.n) {
+      // steps between the table and the product are functions of an entry: the table goes through them once
+      void* through = ex.dalloc(table.data.size() * 4);
+      KERNEL_OK(cvmk_elemwise(d.table, d.table_dtype, through, CVMK_I32, (int64_t)table.data.size(), &first.after, ex.stream_));
+      CUDA_OK(cudaStreamSynchronize(ex.stream_));
+      d.table = through;
+      d.table_dtype = CVMK_I32;
+    }
+    void* mem = nullptr;
+    CHECK(posix_memalign(&mem, 64, sizeof(cvmk_dense_lut_plan)) == 0);
+    ex.lut_plans_.emplace_back((cvmk_dense_lut_plan*)mem, plan_deleter);
+    cvmk_dense_lut_plan* plan = ex.lut_plans_.back().get();
+    KERNEL_OK(cvmk_dense_lut_prepare(&d, plan));
+    add_step(label, [plan](cudaStream_t s) { return cvmk_dense_lut_launch(plan, s); });
+    return true;
+  }
+
   // Element-wise root: unary ops, elemwise_add/sub, broadcast with a scalar parameter.
   bool lower_elemwise_root(uint32_t nid) {
     const Node& n = g.nodes[nid];
@@ -1522,7 +1685,10 @@ struct Lowering {
     const Node& n = g.nodes[nid];
     const std::string& op = n.op->name;
     if (op == "conv2d") return lower_conv_like(nid, false);
-    if (op == "dense") return lower_conv_like(nid, true);
+    if (op == "dense") {
+      if (lower_dense_lut(nid)) return;
+      return lower_conv_like(nid, true);
+    }
     if (op == "max_pool2d") return lower_pool(nid);
     if (op == "upsampling") return lower_upsampling(nid);
     if (op == "concatenate") return lower_concat(nid);

@@ -8,7 +8,7 @@
 //   - a physical layout: 4-D entries are held channels-last (NHWC), everything else row-major;
 //   - fusion: chains of element-wise successors with a single consumer are folded into the
 //     producing kernel (conv2d / dense / reduce / element-wise), so their int32 intermediates are
-//     never written;
+//     never written; a dense layer with a table behind it, gated by a second one or not, is one kernel;
 //   - pre-packed int8 weights (OIHW -> OHWI) and TMA tensor maps for the tensor-core convolutions;
 //   - CUDA graphs: one of every step and the way of the heads to the host, behind a kernel that fetches
 //     the staging buffer where the input is small; and, for batches that upload while they compute,
@@ -139,6 +139,7 @@ class Executor {
   std::vector<void*> pinned_;
   std::vector<std::unique_ptr<cvmk_conv_plan, void (*)(void*)>> plans_;
   std::vector<std::unique_ptr<cvmk_stem_conv_plan, void (*)(void*)>> stem_plans_;
+  std::vector<std::unique_ptr<cvmk_dense_lut_plan, void (*)(void*)>> lut_plans_;
   size_t device_bytes_ = 0;
   // input staging
   void* in_host_ = nullptr;

@@ -149,6 +149,23 @@ class GraphBuilder:
             y = self.op("cvm_right_shift", [y], self.shape_of(y), {"precision": 8, "shift_bit": shift})
         return y
 
+    def lut(self, x, table, precision, offset=None):
+        """cvm_lut of x, moved by `offset` first (indices below 0 count as 0)."""
+        i = len(self.params)
+        if offset is not None:
+            x = self.op("broadcast_add", [x, self.var("o%d" % i, (1,), 16, np.array([offset], np.int32))], self.shape_of(x))
+        t = self.var("t%d" % i, (len(table),), precision, table)
+        return self.op("cvm_lut", [x, t], self.shape_of(x), {"in_dim": len(table)})
+
+    def gated(self, x, units, bits=8, shift=7):
+        """The first half of a decoder layer's feed-forward block: silu(dense(x)) * dense(x), to 8 bits."""
+        k = self.shape_of(x)[1]
+        down = self.default_shift(k) + 1
+        gate = self.op("cvm_right_shift", [self.dense(x, units)], (self.shape_of(x)[0], units), {"precision": bits, "shift_bit": max(1, down - (bits - 8))})
+        gate = self.lut(gate, silu_table(bits), 8, 1 << (bits - 1))
+        y = self.op("broadcast_mul", [gate, self.dense(x, units, down)], self.shape_of(gate))
+        return self.op("cvm_right_shift", [y], self.shape_of(y), {"precision": 8, "shift_bit": shift})
+
     def max_pool(self, x, k, stride, pad):
         n, c, h, w = self.shape_of(x)
         oh, ow = (h + 2 * pad - k) // stride + 1, (w + 2 * pad - k) // stride + 1
@@ -451,6 +468,32 @@ def ssd_full(batch=1, seed=0, size=128, input_seed=7, classes=8, score_threshold
         "id_index": 0, "score_index": 1, "coord_start": 2, "return_indices": False, "invalid_to_bottom": True})
     js, pb = g.finish(out)
     return js, pb, image_input(batch, size, input_seed)
+
+
+# ---------------------------------------------------------------------------------------------
+# A text model's token-wise part
+# ---------------------------------------------------------------------------------------------
+def silu_table(bits=8, span=6.0, top=127):
+    """x * sigmoid(x) over [-span, span) in 2^bits steps, `top` standing for `span`."""
+    x = (np.arange(1 << bits) - (1 << (bits - 1))) * (span / (1 << (bits - 1)))
+    return np.clip(np.rint(x / (1 + np.exp(-x)) * (top / span)), -top, top).astype(np.int8)
+
+
+def decoder_mlp(rows=4, hidden=256, inner=512, layers=2, vocab=1000, seed=0, input_seed=7, gated=True):
+    """The token-wise part of a quantised language model: feed-forward blocks with residual sums over `rows` tokens' hidden
+    vectors, and the projection to int32 scores over a vocabulary."""
+    g = GraphBuilder(seed)
+    x = g.var("data", (rows, hidden), 8)
+    for _ in range(layers):
+        if gated:
+            h = g.gated(x, inner)
+        else:
+            h = g.lut(g.dense(x, inner, g.default_shift(hidden) + 1), silu_table(), 8, 128)
+        y = g.dense(h, hidden, g.default_shift(inner))
+        x = g.op("cvm_clip", [g.op("elemwise_add", [y, x], (rows, hidden))], (rows, hidden), {"precision": 8})
+    js, pb = g.finish(g.dense(x, vocab))
+    rng = np.random.RandomState(input_seed)
+    return js, pb, rng.randint(-127, 128, size=(rows, hidden)).astype(np.int8)
 
 
 def conv_ops_per_image(graph_json):
