@@ -895,6 +895,12 @@ Requant requant_of(const DevChain& c, int first, int len, int K) {
   return {1, (int)add, (int)lo, (int)hi, rs.d, (int)room};
 }
 
+// Whether y can be stored by TMA: rows begin on 16 bytes, and they end on them, because a store writes whole 16 bytes where the
+// last element of a row lies among them (1000 of 1008 bytes: the other eight came out 0).
+bool by_tma(const cvmk_dense_lut_desc& d) {
+  return !((uintptr_t)d.y & 15) && d.y_pitch * d.y_dtype % 16 == 0 && (int64_t)d.units * d.y_dtype % 16 == 0;
+}
+
 // Which kernel runs a layer, and how the small one cuts it (rows of x a tile, CTAs that share its reduction): every cut, and the
 // pairs of CTAs, are given a time, and the least of them is taken.  The terms, in microseconds of a launch in a chain of launches
 // (of 40 shapes, 1 to 2000 rows, 176 to 8192 long, 35 to 16384 units, each cut timed; most are within 10 %):
@@ -910,7 +916,7 @@ struct Cut { int row_tile, split; };   // split 0: pairs
 Cut choose(const cvmk_dense_lut_desc& d, int kblocks, int sms) {
   const double weights = (double)d.units * d.K * (d.v ? 2 : 1);
   const int64_t pair_tiles = (int64_t)((d.rows + 255) / 256) * ((d.units + (d.v ? 127 : 255)) / (d.v ? 128 : 256)), pairs = sms / 2;
-  const bool aligned = !((uintptr_t)d.y & 15) && d.y_pitch * d.y_dtype % 16 == 0;
+  const bool aligned = by_tma(d);
   Cut best = {256, 0};
   double least = (aligned ? 5.3 : 6.8) + 0.1 * kblocks + std::max((pair_tiles + pairs - 1) / pairs * std::max(0.28 * kblocks, 2.7), weights / 6e6);
   static const int at_once[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};   // clusters of 1, 2, 4 and 8 CTAs, one and two an SM; 148 SMs
@@ -1088,7 +1094,7 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
     // y in int8 leaves, and an int8 tensor operand comes, by TMA; a warp's piece of the tile waits in shared memory, twice with
     // an operand, for which the ring gives up two of its six stages
     const int wide = p.y_dtype == CVMK_I32;
-    plan->io = !((uintptr_t)p.y & 15) && p.y_pitch * p.y_dtype % 16 == 0 ? 1 + wide : 0;
+    plan->io = by_tma(p) ? 1 + wide : 0;
     const void* operand = nullptr;
     for (int i = 0; i < p.chain_y.n; ++i)
       if (is_tensor_step(p.chain_y.s[i])) {
@@ -1121,8 +1127,12 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   auto smem_of = [&](int stages) { return 1024 + small_ring_bytes(plan->row_tile, stages) + table_room; };
   plan->stages = std::min((kblocks + plan->split - 1) / plan->split, MAX_STAGES);
   while (plan->stages > 2 && smem_of(plan->stages) > limit) --plan->stages;
-  // (26 KB and more: beside a pair of CTAs of conv_tc_kernel, which takes its TMEM columns on two SMs, nothing of this kernel fits)
-  plan->smem_bytes = std::max(smem_of(plan->stages), 26 * 1024);
+  // The CTAs of a cluster wait for one another while they hold TMEM columns, so the columns of all CTAs that an SM has room for
+  // have to be there at once: shared memory in proportion to them (512 columns to 228 KB), whatever kernels run beside this one.
+  // (26 KB and more: beside a pair of CTAs of conv_tc_kernel, which takes its columns on two SMs, nothing of this kernel fits.)
+  int columns = 32;
+  while (columns < plan->row_tile) columns *= 2;
+  plan->smem_bytes = std::max({smem_of(plan->stages), 26 * 1024, columns * 460});
   plan->grid = (int)(tiles * plan->split);
 
   return encode_operands(plan, plan->row_tile, 64);

@@ -16,7 +16,8 @@ def kn(pkg):
 class Case:
     """Random operands of a call on the GPU, and what it has to give."""
 
-    def __init__(self, kn, rows, k, units, gated=True, table=(256, 1), y_dtype=1, residual=None, pad=0, seed=0, low=-128, after=None, bias=True):
+    def __init__(self, kn, rows, k, units, gated=True, table=(256, 1), y_dtype=1, residual=None, pad=0, seed=0, low=-128, after=None, bias=True, y_pitch=None,
+                 biases=9000, front=None, front_v=None):
         import torch
         rng = np.random.RandomState(seed)
         self.kn, self.rows, self.units, self.torch = kn, rows, units, torch
@@ -24,8 +25,8 @@ class Case:
         self.x, self.w, self.v = (rng.randint(low, 128, size=(n, pitch)).astype(np.int8) for n in (rows, units, units))
         n, kind = table
         self.table = rng.randint(-128, 128, n).astype(np.int8) if kind == 1 else rng.randint(-40000, 40000, n).astype(np.int32)
-        bw, bv = (rng.randint(-9000, 9000, units).astype(np.int32) for _ in range(2))
-        self.y_pitch = units + 3 * pad
+        bw, bv = (rng.randint(-biases, biases, units, dtype=np.int64).astype(np.int32) for _ in range(2))
+        self.y_pitch = y_pitch or units + 3 * pad
         res = None
         if residual:
             res = rng.randint(-100, 100, size=(rows, self.y_pitch)).astype(np.int8 if residual[1] == 1 else np.int32)
@@ -39,6 +40,7 @@ class Case:
         sw, sv = max(1, int(np.log2(spread * 3 / 2 ** (bits - 1)))), max(1, int(np.log2(spread * 3 / 128)))
         chain_w = ([(kn.ADD_C, at[4])] if bias else []) + [(kn.RSHIFT, sw, bits), (kn.ADD_S, n // 2)]
         chain_v = ([(kn.ADD_C, at[5])] if bias else []) + [(kn.RSHIFT, sv, 8)] if gated else []
+        chain_w, chain_v = chain_w if front is None else front, chain_v if front_v is None else front_v
         chain_y = [(kn.RSHIFT, (7 if gated else 1) + (0 if kind == 1 else 8), 8)] if after is None else after
         tensors = {at[4]: bw.astype(np.int64), at[5]: bv.astype(np.int64)}
         if residual:
@@ -196,3 +198,58 @@ def test_a_residual_that_is_the_result(kn):
         c.plan(chain_y=[s if s[0] != kn.ADD_T else (kn.ADD_T, c.y.data_ptr(), 1) for s in c.args["chain_y"]]).launch(torch.cuda.current_stream().cuda_stream)
         torch.cuda.synchronize()
         assert np.array_equal(c.y.cpu().numpy()[:rows], c.want) and res.shape == c.want.shape
+
+
+# Rows of y on 16 bytes that are longer than the result: nothing behind the units is touched
+@pytest.mark.parametrize("rows,units,pitch", [(5, 100, 112), (300, 100, 112), (300, 257, 288), (2100, 33, 48), (700, 1000, 1008)])
+@pytest.mark.parametrize("y_dtype", [1, 4])
+@pytest.mark.parametrize("residual", [None, 1, 4])
+def test_rows_longer_than_the_result(kn, rows, units, pitch, y_dtype, residual):
+    for gated in (True, False):
+        for table in ((256, 1), (300, 4)):
+            Case(kn, rows, 1100, units, gated, table, y_dtype, (kn.ADD_T, residual) if residual else None, seed=pitch, y_pitch=pitch).run()
+
+
+# Biases near the ends of 32 bits, whose sums wrap: some of a tile's, or all
+@pytest.mark.parametrize("rows,units", [(3, 70), (40, 200), (1100, 1000)])
+@pytest.mark.parametrize("gated", [True, False])
+def test_sums_that_wrap(kn, rows, units, gated):
+    for biases in (2**31 - 1, 2**31 - 2**20, 2**25):
+        Case(kn, rows, 900, units, gated, biases=biases, seed=units, y_pitch=(units + 15) // 16 * 16).run()
+
+
+# Chains that are not a shift (and a sum with a constant) in front of the table, or on the other side
+@pytest.mark.parametrize("rows,units", [(3, 70), (1100, 1000)])
+@pytest.mark.parametrize("front", range(6))
+def test_other_chains(kn, rows, units, front):
+    w = [[], [(kn.RELU,), (kn.RSHIFT, 12, 8)], [(kn.MUL_S, 3), (kn.RSHIFT, 14, 8), (kn.ADD_S, 128), (kn.ABS,)], [(kn.RSHIFT, 11, 8), (kn.ADD_S, -300)],
+         [(kn.RSHIFT, 11, 8), (kn.ADD_S, 400)], [(kn.CLIP, -100000, 90000), (kn.RSHIFT, 9, 9), (kn.CLIP, 0, 250)]][front]
+    v = [[], [(kn.CLIP, -50, 50)], [(kn.RSHIFT, 13, 8), (kn.ADD_S, 7)], [(kn.RELU,), (kn.RSHIFT, 12, 8)], [(kn.RSHIFT, 20, 8)], [(kn.RSHIFT, 1, 16)]][front]
+    for gated in (True, False):
+        for y_dtype, after in ((4, []), (1, None)):
+            Case(kn, rows, 500, units, gated, (256, 1), y_dtype, after=after, front=w, front_v=v if gated else None, seed=front).run()
+
+
+def test_sizes_drawn_at_random(kn):
+    """Every cut that sizes of 1 to 3000 rows, 1 to 3000 long, 1 to 3000 units lead to."""
+    rng = np.random.RandomState(17)
+    cuts = set()
+    for i in range(60):
+        rows, k, units = (int(np.exp(rng.uniform(0, np.log(3000)))) for _ in range(3))
+        plan = Case(kn, rows, k, units, i % 2 == 0, [(256, 1), (1000, 4)][i % 3 == 0], [1, 4][i % 5 == 0], (kn.ADD_T, 1) if i % 4 == 0 else None, seed=i,
+                    y_pitch=(units + 15) // 16 * 16 if i % 7 < 3 else None).run(params_static=bool(i % 2))
+        cuts.add((plan.kernel, plan.split))
+    assert {kernel for kernel, _ in cuts} == {0, 1} and max(split for _, split in cuts) > 1
+
+
+def test_whole_rows_drawn_at_random(kn):
+    """Units that end on 16 bytes: results and operands that go by TMA."""
+    rng = np.random.RandomState(18)
+    ways = set()
+    for i in range(40):
+        rows, k, units = (int(np.exp(rng.uniform(np.log(lo), np.log(hi)))) for lo, hi in ((257, 3000), (1, 1000), (16, 3000)))
+        units = (units + 15) // 16 * 16
+        plan = Case(kn, rows, k, units, i % 2 == 0, [(256, 1), (1000, 4)][i % 3 == 0], [1, 4][i % 5 < 2], (kn.SUB_T, 1) if i % 4 < 2 else None, seed=i,
+                    y_pitch=units + 16 * (i % 7 < 3)).run(params_static=bool(i % 2))
+        ways.add((plan.kernel, plan.io))
+    assert ways >= {(1, 1), (1, 2)}

@@ -169,3 +169,51 @@ def test_captured_and_replayed(kn):
         torch.cuda.synchronize()
         for r in range(rows):
             assert int(token[r]) == ref.sample_row(x[r].cpu().numpy(), EXP, 30000, 40, ONE, 0, int(u[r]))[0]
+
+
+def test_two_streams_at_once(kn):
+    import torch
+    rng = np.random.RandomState(6)
+    cases = []
+    for rows, vocab in ((30, 9000), (2, 120000), (200, 30001)):
+        few = min(rows, 3)
+        x = logits(rng, few, vocab, "normal")[np.arange(rows) % few]
+        u, s = rng.randint(0, 2**31, few)[np.arange(rows) % few], settings(rng, few)
+        dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+        ops = [dev(x), dev(EXP), dev(np.full(rows, 30000)), dev(u)] + [dev(s[n][np.arange(rows) % few]) for n in ("top_k", "top_p", "min_p")]
+        token = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        at = [t.data_ptr() for t in ops]
+        call = kn.Sample(logits=at[0], rows=rows, vocab=vocab, table=at[1], table_len=4096, scale=at[2], random=at[3], top_k=at[4], top_p=at[5], min_p=at[6],
+                         token=token.data_ptr())
+        want = [ref.sample_row(x[r], EXP, 30000, *(int(s[n][r]) for n in ("top_k", "top_p", "min_p")), int(u[r]))[0] for r in range(few)]
+        cases.append((call, torch.cuda.Stream(), token, want, ops))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for call, stream, *_ in cases:
+            call.launch(stream.cuda_stream)
+    torch.cuda.synchronize()
+    for _, _, token, want, _ in cases:
+        got = token.cpu().numpy()
+        assert all(got[i] == want[i % len(want)] for i in range(len(got)))
+
+
+def test_scores_written_by_the_kernel_before(kn, pkg):
+    """dense to int32 scores, and the draw behind it on the same stream, again and again."""
+    import torch
+    import ctypes as ct
+    rng = np.random.RandomState(8)
+    lib, rows, vocab = pkg.runtime.lib(), 16, 6000
+    a, b = (torch.from_numpy(np.round(rng.randn(rows, vocab) * 1500).astype(np.int32)).cuda() for _ in range(2))
+    x = torch.empty_like(a)
+    tab, scale, u = torch.from_numpy(EXP).cuda(), torch.full((rows,), 30000, dtype=torch.int32, device="cuda"), torch.from_numpy(rng.randint(0, 2**31, rows).astype(np.int32)).cuda()
+    token = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    call = kn.Sample(logits=x.data_ptr(), rows=rows, vocab=vocab, table=tab.data_ptr(), table_len=4096, scale=scale.data_ptr(), random=u.data_ptr(), token=token.data_ptr())
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for turn in range(6):
+        source = (a, b)[turn % 2]
+        assert lib.cvmk_elemwise(ct.c_void_p(source.data_ptr()), 4, ct.c_void_p(x.data_ptr()), 4, ct.c_int64(rows * vocab), None, ct.c_void_p(stream.cuda_stream)) == 0
+        call.launch(stream.cuda_stream)
+        stream.synchronize()
+        host = source.cpu().numpy()
+        assert [int(t) for t in token] == [ref.sample_row(host[r], EXP, 30000, 0, ONE, 0, int(u[r]))[0] for r in range(rows)]
