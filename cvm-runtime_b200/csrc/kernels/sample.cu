@@ -40,6 +40,16 @@ struct Params {
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// The cluster's barrier, for warps whose lanes may come to it apart (behind a loop that polls, or a branch of some lanes): its
+// aligned form is undefined for such a warp.
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -176,8 +186,12 @@ struct Row {
     return min((((uint64_t)e << 16) + scale - 1) / scale, (uint64_t)1 << 32);
   }
   __device__ __forceinline__ void sync() const {
-    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    else __syncthreads();
+    if (split > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
   }
   // The values at places j .. j + 3, j a multiple of 4 (zeros, or what lies there in shared memory, outside the valid ones).
   template <bool RESIDENT>
@@ -484,7 +498,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&s.bar)));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for before anything is sent)
+  if (p.split > 1) cluster_arrive();   // (waited for before anything is sent)
   pdl_wait();
   // (what the set-up needs of global memory is requested at once: a trip each would be longer than the slice takes)
   constexpr int EARLY = TABLE_SMEM_MAX / 512;
@@ -535,7 +549,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     landed = ok != 0;
   }
 
-  if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (p.split > 1) cluster_wait();
 
   // ---- the largest and the smallest score, and the bound of the k-th largest
   int32_t lo = INT32_MAX, hi = INT32_MIN;
