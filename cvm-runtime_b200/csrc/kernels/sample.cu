@@ -17,6 +17,10 @@
 //   that way too, by weight.)
 // The draw then sums the weights in blocks of 512 elements, finds the block, and looks up the element in it.
 // Counts and weights are whole numbers, so their order of summation changes nothing.
+//
+// A launch ends whatever its operands do meanwhile: should another stream still write them, tokens mean nothing, but no place is
+// looked up outside the arrays, and every CTA of a row takes the same way from barrier to barrier: all go by one reading of the
+// row's parameters, by scores that are exchanged, and by counts and sums that each adds up from the same ones.
 #include <cuda_runtime.h>
 #include "common.cuh"
 
@@ -142,6 +146,10 @@ struct Shared {
   alignas(16) uint4 answer;
   alignas(16) uint4 sums[MAX_SPLIT];      // weight (low, high), ties, kept
   uint32_t late;                          // a slice has not arrived
+  uint32_t tie_weight;
+  uint32_t min_weight;
+  alignas(16) uint4 row;                  // the row's top_k, top_p, scale and random number, as they were read
+  alignas(16) uint4 row_of_all;           // by the first CTA
   uint64_t found_before, found_size;
   int found;
   uint32_t counts[MAX_SPLIT];             // elements on the CTAs' lists
@@ -163,12 +171,11 @@ struct Row {
   bool wide;             // the table lies in global memory
   int table_at;          // else at this place of the dynamic shared memory (known to be that: a look-up in a pointer's memory is twice as slow)
   __device__ __forceinline__ const int32_t* in_smem() const { return reinterpret_cast<const int32_t*>(dynamic_smem) + table_at; }
-  // entry() in fewer instructions where scale <= 2^16 and the table lies in shared memory: scores below floor_x have the last
-  // entry, as floor_x has, and above it (top - x) * scale is less than 2^31.
+  // entry() in fewer instructions where scale <= 2^16 and the table lies in shared memory: distances above `far` have the last
+  // entry, as `far` has, and far * scale is less than 2^31.
   bool gentle;
-  int32_t floor_x;
-  uint32_t minus_scale, top_scaled;
-  __device__ __forceinline__ uint32_t entry_of(int32_t v) const { return ((uint32_t)max(v, floor_x) * minus_scale + top_scaled) >> 16; }
+  uint32_t far;
+  __device__ __forceinline__ uint32_t entry_of(int32_t v) const { return min((uint32_t)top - (uint32_t)v, far) * scale >> 16; }
   __device__ __forceinline__ uint32_t dist(int32_t v) const { return (uint32_t)top - (uint32_t)v; }
   // min((d * scale) >> 16, last_entry): a table in shared memory has less than 2^15 entries, and every d above
   // saturated = (2^32 - 1) / scale has a product above 2^31.
@@ -283,6 +290,7 @@ __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t fro
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum += own[k];
     uint64_t before = block_scan(s, sum, total);
+    if (total < need) return {to, 0};   // (scores that change)
     if (before < need && need <= before + sum) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -341,6 +349,8 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
         if (tie_weight) c.ties = (uint32_t)min((uint64_t)whole.ties, (need - total + tie_weight - 1) / tie_weight);
         return c;
       }
+    } else if (total < need) {   // (scores that change)
+      return whole;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -517,14 +527,14 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   }
   if (RESIDENT && tid >= 32 && tid < 35 && r.first + tid - 32 < b0) slice_s[r.first + tid - 32] = at[r.first + tid - 32];
   if (RESIDENT && tid >= 35 && tid < 38 && b1 + tid - 35 < r.last) slice_s[b1 + tid - 35] = at[b1 + tid - 35];
-  const int k = d.top_k ? d.top_k[row] : 0;
-  const uint64_t top_p = d.top_p ? (uint64_t)min(max(d.top_p[row], 0), (int)ONE) : ONE;
   const uint64_t min_p = d.min_p ? (uint64_t)min(max(d.min_p[row], 0), (int)ONE) : 0;
-  const uint64_t u = (uint64_t)(d.random[row] & 0x7fffffff);
-  r.scale = (uint32_t)max(d.scale[row], 0);
-  r.saturated = r.scale ? 0xffffffffu / r.scale : 0xffffffffu;
+  const uint32_t min_weight = (uint32_t)((min_p * (uint64_t)max(d.table[0], 0) + ONE - 1) >> 30);
+  if (tid == 64) {
+    s.row = make_uint4(d.top_k ? (uint32_t)d.top_k[row] : 0u, d.top_p ? (uint32_t)min(max(d.top_p[row], 0), (int)ONE) : (uint32_t)ONE,
+                       (uint32_t)max(d.scale[row], 0), (uint32_t)d.random[row] & 0x7fffffffu);
+    s.min_weight = min_weight;
+  }
   r.last_entry = (uint32_t)d.table_len - 1u;
-  r.min_weight = (uint32_t)((min_p * (uint64_t)max(d.table[0], 0) + ONE - 1) >> 30);
   r.wide = !p.table_smem;
   r.table = d.table;
   r.table_at = RESIDENT ? p.slice : 0;
@@ -532,11 +542,13 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 #pragma unroll
   for (int i = 0; i < EARLY; ++i)
     if (p.table_smem && tid + i * threads < d.table_len) {
-      const int32_t w = (uint32_t)max(entry[i], 0) >= r.min_weight ? max(entry[i], 0) : 0;
+      const int32_t w = (uint32_t)max(entry[i], 0) >= min_weight ? max(entry[i], 0) : 0;
       table_s[tid + i * threads] = w;
       plain = plain && w > 0 && w < 1 << 27;
     }
   const bool plain_table = __syncthreads_and(plain) && p.table_smem;
+  uint4 of_row = s.row;
+  r.min_weight = s.min_weight;
   // (bounded: the copy is the only thing that is waited for)
   bool landed = !RESIDENT;
   for (uint32_t i = 0; !landed && i < (1u << 19); ++i) {
@@ -553,8 +565,8 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
 
   // ---- the largest and the smallest score, and the bound of the k-th largest
   int32_t lo = INT32_MAX, hi = INT32_MIN;
-  const bool by_count = k >= 1 && k < vocab;
-  if (by_count || top_p < ONE) {
+  const auto cut_by_k = [&]() { return (int32_t)of_row.x >= 1 && (int32_t)of_row.x < vocab; };
+  if (cut_by_k() || of_row.y < ONE) {
     r.each<RESIDENT>([&](int32_t v, int) {
       lo = min(lo, v);
       hi = max(hi, v);
@@ -572,8 +584,8 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   lo = __reduce_min_sync(FULL, lane < warps ? s.lo[lane] : INT32_MAX);
   hi = __reduce_max_sync(FULL, lane < warps ? s.hi[lane] : INT32_MIN);
   int32_t bound = INT32_MIN;
-  const int part = (k - 1) / p.split + 1;   // of k, for a CTA
-  if (by_count && part <= threads && __syncthreads_count(some) >= part) {
+  const int part = ((int32_t)of_row.x - 1) / p.split + 1;   // of top_k, for a CTA
+  if (cut_by_k() && part <= threads && __syncthreads_count(some) >= part) {
     const uint32_t far = (uint32_t)hi - (uint32_t)mine;
     uint32_t from = 0, to = (uint32_t)hi - (uint32_t)lo;
     for (int i = 0; i < 14 && from < to; ++i) {   // (to some ten-thousandth of the range)
@@ -585,9 +597,16 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   }
   if (warp == 0 && lane < p.split) {   // (a lane for every CTA)
     store128(remote(&s.scores[rank], (uint32_t)lane), make_uint4((uint32_t)lo, (uint32_t)hi, (uint32_t)bound, 0));
+    if (rank == 0) store128(remote(&s.row_of_all, (uint32_t)lane), of_row);
     if (!landed) store32(remote(&s.late, (uint32_t)lane), 1u);
   }
   r.sync();
+  of_row = s.row_of_all;
+  const int k = (int)of_row.x;
+  const bool by_count = cut_by_k();
+  const uint64_t top_p = of_row.y, u = of_row.w;
+  r.scale = of_row.z;
+  r.saturated = r.scale ? 0xffffffffu / r.scale : 0xffffffffu;
   const bool late = s.late != 0;
   {
     const int4 v = s.scores[min(lane, p.split - 1)];
@@ -604,9 +623,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   }
   r.top = hi;
   r.gentle = !r.wide && r.scale <= 65536;
-  r.floor_x = (int32_t)max((int64_t)hi - (int64_t)min(r.first_of(r.last_entry), (uint64_t)1 << 32), (int64_t)INT32_MIN);
-  r.minus_scale = 0u - r.scale;
-  r.top_scaled = (uint32_t)hi * r.scale;
+  r.far = (uint32_t)min(r.first_of(r.last_entry), ((uint64_t)1 << 32) - 1);
   const int range_bits = bits_of((uint32_t)hi - (uint32_t)lo);
 
   // ---- the cuts
@@ -681,7 +698,12 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   }
   if (top_p < ONE) {
     if (r.wide) {
-      const uint32_t w = cut.ties ? r.weight((uint32_t)cut.D) : 0u, ties = cut.ties;
+      const uint32_t ties = cut.ties;
+      if (ties) {   // (by one reading of the table)
+        if (rank == 0 && tid < p.split) store32(remote(&s.tie_weight, (uint32_t)tid), r.weight((uint32_t)cut.D));
+        r.sync();
+      }
+      const uint32_t w = ties ? s.tie_weight : 0u;
       cut = cut_by_weight<RESIDENT>(r, s, range_bits, [=](uint64_t strict) { return share_of(strict + (uint64_t)ties * w); }, cut, w);
     } else {
       // the elements that are left, by table entry
@@ -763,7 +785,6 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   }
 
   // ---- the draw: weights and ties of every block of the slice
-  uint32_t tie_weight = cut.ties ? r.weight((uint32_t)cut.D) : 0u;
   const int blocks = (r.last + BLOCK - 1) / BLOCK;
   uint32_t kept = 0;
   const uint32_t D32 = (uint32_t)min(cut.D, end - 1);
@@ -844,6 +865,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     const uint64_t mass = __shfl_sync(FULL, mi, 31);
     const uint32_t ties = __shfl_sync(FULL, (uint32_t)ti, 31);
     if (lane < p.split) store128(remote(&s.sums[rank], (uint32_t)lane), make_uint4((uint32_t)mass, (uint32_t)(mass >> 32), ties, kept));
+    if (rank == 0 && lane < p.split) store32(remote(&s.tie_weight, (uint32_t)lane), cut.ties ? r.weight((uint32_t)cut.D) : 0u);
   };
   if (warp == 0) {
     kept = __reduce_add_sync(FULL, lane < warps ? s.kept[lane] : 0u);
@@ -866,6 +888,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     }
   };
   add_up();
+  uint32_t tie_weight = s.tie_weight;
   if (cut.ties && tie_weight) all_kept += cut.ties;
   all += (uint64_t)cut.ties * tie_weight;
   const uint64_t target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
