@@ -1089,6 +1089,7 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   if (odd) { set_error("dense_lut_prepare: an operand is not aligned to its elements"); return CVMK_ERR_ARG; }
   if (!encoder()) { set_error("dense_lut_prepare: the driver has no cuTensorMapEncodeTiled"); return CVMK_ERR_CUDA; }
 
+  if (check_cuda(cudaGetDevice(&plan->device), "dense_lut_prepare: cudaGetDevice")) return CVMK_ERR_CUDA;
   const int sms = sm_count(), kblocks = (p.K + BLOCK_K - 1) / BLOCK_K, tile_units = p.v ? 64 : 128;
   const int64_t table_bytes = (int64_t)p.table_len * p.table_dtype;
   plan->table_smem = table_bytes <= TABLE_SMEM_MAX ? (int)table_bytes : 0;
@@ -1157,7 +1158,8 @@ extern "C" int cvmk_dense_lut_launch(const cvmk_dense_lut_plan* plan, cvmk_strea
 
   static bool attr_of_device[64] = {false};
   int dev = 0;
-  cudaGetDevice(&dev);
+  if (check_cuda(cudaGetDevice(&dev), "dense_lut_launch: cudaGetDevice")) return CVMK_ERR_CUDA;
+  if (dev != plan->device) { set_error("dense_lut_launch: the plan was made for device %d, and %d is current", plan->device, dev); return CVMK_ERR_ARG; }
   if (!attr_of_device[dev & 63]) {
     auto allow = [](auto k, int bytes) {
       const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);

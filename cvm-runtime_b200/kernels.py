@@ -54,7 +54,7 @@ class DenseLutDesc(ct.Structure):
 
 class DenseLutPlan(ct.Structure):
     _fields_ = ([(n, ct.c_uint8 * 128) for n in ("tmap_x", "tmap_w", "tmap_v", "tmap_y", "tmap_r")] + [("d", DenseLutDesc)] +
-                [(n, ct.c_int32) for n in ("kernel", "grid", "smem_bytes", "stages", "split", "row_tile", "table_smem", "io")] + [("reserved", ct.c_int32 * 4)])
+                [(n, ct.c_int32) for n in ("kernel", "grid", "smem_bytes", "stages", "split", "row_tile", "table_smem", "io", "device")] + [("reserved", ct.c_int32 * 3)])
 
 
 class SampleDesc(ct.Structure):

@@ -482,8 +482,8 @@ CVMK_API int cvmk_transpose_batched(const void* x, void* y, int32_t dtype, int64
  * operand may be y itself.
  *
  * cvmk_dense_lut_prepare() chooses the kernel and encodes the tensor maps into `plan` (host memory of the
- * caller, 64-byte aligned; to be repeated if x, w or v move); it wants the device current that will run
- * the launches.  cvmk_dense_lut_launch() only enqueues the kernel; launches of one plan may be on several
+ * caller, 64-byte aligned; to be repeated if an operand moves); it wants the device current that will run
+ * the launches, and a launch with another one current is refused (CVMK_ERR_ARG).  cvmk_dense_lut_launch() only enqueues the kernel; launches of one plan may be on several
  * streams at once where y is not read in between.  `status`: as in cvmk_conv_desc, or NULL.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {
@@ -518,7 +518,8 @@ typedef struct __attribute__((aligned(64))) {
   int32_t row_tile;     /* rows of x a tile */
   int32_t table_smem;   /* bytes of the table kept in shared memory, 0: read where it lies */
   int32_t io;           /* y and an int8 tensor operand go through shared memory by TMA: 1 y in int8, 2 in int32 */
-  int32_t reserved[4];
+  int32_t device;       /* that was current: launches with another one current are refused */
+  int32_t reserved[3];
 } cvmk_dense_lut_plan;
 
 /* 1 if the sizes, types and chains are taken; looks at no address. */

@@ -188,6 +188,18 @@ def test_two_streams_at_once(kn):
     b.check()
 
 
+def test_a_plan_of_another_device_is_refused(kn):
+    case = Case(kn, 5, 256, 300, seed=33)
+    plan = case.plan()
+    plan.plan.device += 1
+    with pytest.raises(kn.KernelError) as refused:
+        plan.launch()
+    assert refused.value.status == kn.ERR_ARG
+    plan.plan.device -= 1
+    plan.launch()
+    case.check()
+
+
 def test_a_residual_that_is_the_result(kn):
     """y += ...: the tensor operand may be y itself."""
     import torch
