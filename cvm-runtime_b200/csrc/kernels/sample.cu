@@ -7,8 +7,8 @@
 // nor list the row.
 //   top_k   In a CTA, the n-th largest of the maxima of its threads is a lower bound of its n-th largest element (that many
 //           threads have one as large).  So the row's k-th is not below the least of the CTAs' bounds for n = k / CTAs.  The
-//           elements that are not below it are few more than k; they are put on a list, and the cuts of top_k and top_p are
-//           found on it by bisection: a thread holds an element, and a count over the CTA is one barrier.
+//           elements that are not below it are few more than k; they are put on a list, and one CTA does all the rest on it:
+//           a thread holds an element and compares it with every other one, for its rank and the weight in front of it.
 //   top_p   An element's weight is a function of its table index, so the elements of every index are counted; the running
 //           sum of count * weight gives the index in which the share is reached and how many of its elements are needed, and
 //           the cut among those is one by count again.
@@ -38,11 +38,12 @@ constexpr int MAX_WARPS = 32;
 constexpr int DIGIT = 12, BINS = 1 << DIGIT;       // of counts
 constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bin
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
-constexpr int LIST = 1024;              // elements on a list
+constexpr int LIST = 512;               // elements on a list
 constexpr int MAX_SPLIT = 8;
 constexpr int BLOCK = 512, GROUPS = BLOCK / 128, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / BLOCK + 2;
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr uint64_t ONE = 1u << 30;
+constexpr int RANK_BITS = 10;           // behind a weight: one each for the elements in front
 
 struct Params {
   cvmk_sample_desc d;
@@ -132,8 +133,11 @@ struct Shared {
   union {
     alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 16 bits, and the rest
     struct {                           // (a row whose cuts are found on its list needs no histogram behind it)
-      alignas(16) int2 list[LIST];     // of the slice's elements: score and index
-      alignas(16) uint2 all[LIST];     // of the row's: distance and index
+      alignas(16) uint4 all[LIST];     // of the row's elements: index, distance, and 64 bits to be added up
+      union {
+        alignas(16) int2 list[LIST];     // of the slice's: score and index
+        uint2 sorted[LIST];              // those that stay, by rank: index and weight
+      };
     };
   };
   union {
@@ -141,10 +145,11 @@ struct Shared {
       uint64_t block_mass[MAX_BLOCKS];
       uint32_t block_ties[MAX_BLOCKS];
     };
-    uint32_t all_weight[LIST];
+    uint64_t sums_of_list[32 * MAX_WARPS];
   };
+  uint64_t mass, mass_left;               // of the list behind top_k, and behind top_p
+  uint32_t left;                          // elements of it then
   uint64_t scan[MAX_WARPS];
-  uint32_t reached[2][MAX_WARPS];
   int32_t lo[MAX_WARPS], hi[MAX_WARPS];
   uint32_t kept[MAX_WARPS];
   uint32_t listed;
@@ -381,8 +386,8 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
   }
 }
 
-// Puts the elements with d <= last, of all CTAs, on the list s.all of every CTA: their number, or -1 if they are more than
-// threads.  `index0`: the index of place 0.
+// Puts the elements with d <= last, of all CTAs, on the list s.all of the first CTA: their number, in every CTA, or -1 if they
+// are more than LIST.  `index0`: the index of place 0.
 template <bool RESIDENT>
 __device__ int collect(const Row& r, Shared& s, uint32_t last, int rank, int index0) {
   if (threadIdx.x == 0) s.listed = 0;
@@ -398,57 +403,41 @@ __device__ int collect(const Row& r, Shared& s, uint32_t last, int rank, int ind
   if (threadIdx.x < r.split) store32(remote(&s.counts[rank], threadIdx.x), s.listed);
   r.sync();
   const uint32_t mine = lane < (int)r.split ? s.counts[lane] : 0u;
-  const bool fits = !__any_sync(FULL, mine > LIST) && __reduce_add_sync(FULL, mine) <= blockDim.x;
-  const uint32_t sums = (uint32_t)warp_scan(mine), n = __shfl_sync(FULL, sums, 31);
+  const uint32_t in_all = __reduce_add_sync(FULL, min(mine, LIST + 1u));
+  if (in_all == 0 || in_all > LIST) return -1;   // (none: scores that change)
+  const uint32_t sums = (uint32_t)warp_scan(mine);
   // (a warp for every CTA's list)
   const uint32_t c = threadIdx.x >> 5, count = __shfl_sync(FULL, mine, (int)(c & 31)), at = __shfl_sync(FULL, sums - mine, (int)(c & 31));
-  if (fits && c < r.split)
+  if (rank == 0 && c < r.split)
     for (uint32_t i = lane; i < count; i += 32) {
-      const uint32_t from = remote(&s.list[i], c), v = load32(from), index = load32(from + 4);
-      s.all[at + i] = make_uint2(r.dist((int32_t)v), index);
+      const uint32_t from = remote(&s.list[i], c), index = load32(from + 4), d = r.dist((int32_t)load32(from));
+      const uint64_t add = (uint64_t)r.weight(d) << RANK_BITS | 1u;
+      s.all[at + i] = make_uint4(index, d, (uint32_t)add, (uint32_t)(add >> 32));
     }
-  __syncthreads();
-  return fits ? (int)n : -1;
+  r.sync();   // (the lists have been read)
+  return (int)in_all;
 }
 
-// The cut that leaves `need` elements of a list, one a thread (`mine`: the thread has one, at distance d <= last).
-__device__ Cut cut_list_by_count(uint64_t need, bool mine, uint32_t d, uint32_t last) {
-  uint32_t from = 0, to = last;
-  while (from < to) {
-    const uint32_t mid = from + (to - from) / 2;
-    if ((uint64_t)__syncthreads_count(mine && d <= mid) >= need) to = mid;
-    else from = mid + 1;
-  }
-  return {from, (uint32_t)(need - (uint64_t)__syncthreads_count(mine && d < from))};
-}
-// The smallest K in [from, to] for which the weights of the list's elements with key <= K sum to `need` or more (those up to
-// `to` do).  Every warp adds up the list for a place of its own between `from` and `to`, so a turn cuts what is left to a 17th
-// (512 threads): five turns for any index, where halving takes eighteen.
-template <typename Key>
-__device__ uint32_t search_list(Shared& s, int n, uint32_t from, uint32_t to, uint64_t need, const Key& key) {
+// For the thread's element of n (tid < n): what f(sum, its own, j) adds up for all j < n.  n * n turns of a few
+// instructions, a warp for 32 elements and, where warps are left, for a part of the others (200 elements and 512 threads:
+// 1.8 us; a search for both sums by halving took 6).
+template <typename Own, typename F>
+__device__ __forceinline__ uint64_t against_all(Shared& s, int n, const Own& own_of, const F& f) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  for (int turn = 0; from < to; ++turn) {
-    const uint64_t range = to - from;
-    const auto place = [&](int i) { return from + (uint32_t)(range * (uint32_t)(i + 1) / (uint32_t)(warps + 1)); };
-    const uint32_t at = place(warp);
+  const int blocks = (n + 31) >> 5, parts = warps / blocks, part = warp / blocks, t = (warp - part * blocks) * 32 + lane;
+  if (part < parts) {
+    const auto own = own_of(min(t, n - 1));
+    const int end = n * (part + 1) / parts;
     uint64_t sum = 0;
-    for (int i = lane; i < n; i += 32) sum += key(s.all[i]) <= at ? s.all_weight[i] : 0u;   // (below 2^36)
-    sum = warp_sum(sum);
-    if (lane == 0) s.reached[turn & 1][warp] = sum >= need;
-    __syncthreads();
-    const uint32_t mask = __ballot_sync(FULL, lane < warps && s.reached[turn & 1][lane]);
-    const int first = mask ? __ffs(mask) - 1 : warps;
-    const uint32_t lower = first > 0 ? place(first - 1) + 1 : from;
-    if (mask) to = place(first);
-    from = lower;
+#pragma unroll 8
+    for (int j = n * part / parts; j < end; ++j) f(sum, own, j);
+    s.sums_of_list[part * 32 * blocks + t] = sum;
   }
-  return from;
-}
-// Sum of the list's weights (every warp for itself).
-__device__ __forceinline__ uint64_t sum_of_list(const Shared& s, int n) {
+  __syncthreads();
   uint64_t sum = 0;
-  for (int i = threadIdx.x & 31; i < n; i += 32) sum += s.all_weight[i];
-  return warp_sum(sum);
+  if ((int)threadIdx.x < n)
+    for (int i = 0; i < parts; ++i) sum += s.sums_of_list[i * 32 * blocks + threadIdx.x];
+  return sum;
 }
 
 // The weights of the blocks b0, b0 + warps, .. < end of a row without a cut, all of whose places are valid, with a table of
@@ -644,61 +633,48 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     const uint32_t last = r.dist(bound);
     const int n = collect<RESIDENT>(r, s, last, rank, begin - skew);
     if (n >= 0) {
-      // Everything else is done on the list, by every CTA for itself.
+      if (rank != 0) return;   // (everything else is done on the list)
       const bool mine = tid < n;
-      const uint2 e = mine ? s.all[tid] : make_uint2(0, 0);
-      cut = cut_list_by_count((uint64_t)k, mine, e.x, last);
-      // of the elements at the cut the first ones by index: those up to `tie_index`
-      auto tie_index = [&]() {
-        uint32_t from = 0, to = (uint32_t)vocab - 1u;
-        if ((uint32_t)__syncthreads_count(mine && e.x == cut.D) <= cut.ties) return to;
-        while (from < to) {
-          const uint32_t mid = from + (to - from) / 2;
-          if ((uint32_t)__syncthreads_count(mine && e.x == cut.D && e.y <= mid) >= cut.ties) to = mid;
-          else from = mid + 1;
-        }
-        return from;
-      };
-      uint32_t ties_to = tie_index();
-      const uint32_t weight = mine ? r.weight(e.x) : 0u;
-      uint32_t w = e.x < cut.D || (e.x == cut.D && e.y <= ties_to) ? weight : 0u;
-      if (mine) s.all_weight[tid] = w;
+      // ranks, and the weights in front, in the order of the cuts: of (distance, index)
+      const uint64_t in_front = against_all(s, n, [&](int t) { return (uint64_t)s.all[t].y << 32 | s.all[t].x; }, [&](uint64_t& sum, uint64_t own, int j) {
+        const uint4 e = s.all[j];
+        if (((uint64_t)e.y << 32 | e.x) < own) sum += (uint64_t)e.w << 32 | e.z;
+      });
+      const uint32_t place = (uint32_t)in_front & ((1u << RANK_BITS) - 1u);
+      const uint4 e = s.all[mine ? tid : 0];
+      const uint32_t weight = (uint32_t)(((uint64_t)e.w << 32 | e.z) >> RANK_BITS);
+      const uint64_t before = in_front >> RANK_BITS;
+      bool left = mine && place < (uint32_t)k;
+      if (mine && (int)place == min(k, n) - 1) {   // the last one that top_k leaves
+        s.mass = s.mass_left = before + weight;
+        s.left = place + 1;
+      }
       __syncthreads();
-      uint64_t all = sum_of_list(s, n);
-      if (top_p < ONE && all) {
-        const uint64_t need = share_of(all);
-        const uint32_t at_d = search_list(s, n, 0, last, need, [](const uint2& v) { return v.x; });
-        // the elements in front of at_d, and of those at it as many as it takes
-        const uint32_t each = r.weight(at_d);
-        uint64_t before = 0;
-        for (int i = lane; i < n; i += 32) before += s.all[i].x < at_d ? s.all_weight[i] : 0u;
-        before = warp_sum(before);
-        const uint32_t taken = (uint32_t)((need - before + each - 1) / each);
-        if (at_d < cut.D || taken < cut.ties) {   // (else the cut of top_k stays)
-          cut = {at_d, taken};
-          ties_to = tie_index();
-          w = e.x < cut.D || (e.x == cut.D && e.y <= ties_to) ? weight : 0u;
+      const uint64_t mass = s.mass;
+      if (top_p < ONE && mass) {
+        const uint64_t need = share_of(mass);
+        left = left && before < need;
+        if (left && before + weight >= need) {   // the last one that top_p leaves
+          s.mass_left = before + weight;
+          s.left = place + 1;
         }
-        __syncthreads();   // (the weights have been read)
-        if (mine) s.all_weight[tid] = w;
-        __syncthreads();
-        all = sum_of_list(s, n);
       }
-      const uint32_t kept = (uint32_t)__syncthreads_count(mine && w > 0);
-      const uint64_t target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
-      if (all == 0) {   // nothing weighs anything: the first element with d = 0
-        if (mine) s.all_weight[tid] = e.x == 0;
-        __syncthreads();
-      }
-      const uint32_t token = search_list(s, n, 0, (uint32_t)vocab - 1u, target + 1, [](const uint2& v) { return v.y; });
-      if (rank == 0 && mine && e.y == token) {
-        d.token[row] = (int32_t)token;
-        if (d.weight) d.weight[row] = (int32_t)(all ? w : 0u);
+      if (left) s.sorted[place] = make_uint2(e.x, weight);
+      const uint32_t kept = (uint32_t)__syncthreads_count(left && weight > 0);
+      const uint64_t all = s.mass_left, target = u * (all >> 31) + ((u * (all & 0x7fffffffu)) >> 31);
+      const int m = (int)s.left;
+      const uint64_t up_to = against_all(s, m, [&](int t) { return s.sorted[t].x; }, [&](uint64_t& sum, uint32_t own, int j) {
+        const uint2 e = s.sorted[j];
+        if (e.x <= own) sum += e.y;
+      });
+      const uint2 drawn = s.sorted[tid < m ? tid : 0];
+      // (where nothing weighs anything, the first of the order)
+      if (tid < m && (all ? up_to > target && up_to - drawn.y <= target : tid == 0)) {
+        d.token[row] = (int32_t)drawn.x;
+        if (d.weight) d.weight[row] = (int32_t)drawn.y;
         if (d.mass) d.mass[row] = (int64_t)all;
         if (d.kept) d.kept[row] = (int32_t)kept;
       }
-      __syncwarp();
-      if (p.split > 1) r.sync();   // nobody still reads this CTA's list
       return;
     }
     cut = cut_by_count<RESIDENT>(r, s, (uint64_t)k, 0, (uint64_t)r.dist(lo) + 1);   // (hundreds of equal scores, or a large k)
