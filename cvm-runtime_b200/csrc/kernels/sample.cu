@@ -19,8 +19,8 @@
 // Counts and weights are whole numbers, so their order of summation changes nothing.
 //
 // What bounds it: few rows, the chain of passes and barriers, each a trip to L2 or over a cluster (1 row of 32000 elements, all
-// filters: 16 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 28 us, 2.6).  Many rows, the passes themselves: 256 rows
-// of 262144 elements take 107 us without cuts (read twice: once from memory, 41 us at the rate of a copy, once from L2), 142 with
+// filters: 9.5 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 27 us, 2.6).  Many rows, the passes themselves: 256 rows
+// of 262144 elements take 107 us without cuts (read twice: once from memory, 41 us at the rate of a copy, once from L2), 124 with
 // top_k, 251 with top_p, whose counting is an atomic in shared memory for every element above the table's last entry.  More loads
 // under way (the next four requested while four are worked on) spill at the 64 registers that two CTAs an SM leave: 190 against
 // 184 us over rows of all kinds; three CTAs an SM of 40 registers: 205.
@@ -34,7 +34,7 @@
 namespace cvmk {
 namespace {
 
-constexpr int MAX_WARPS = 32;
+constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int DIGIT = 12, BINS = 1 << DIGIT;       // of counts
 constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bin
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
@@ -145,13 +145,13 @@ struct Shared {
       uint64_t block_mass[MAX_BLOCKS];
       uint32_t block_ties[MAX_BLOCKS];
     };
-    uint64_t sums_of_list[32 * MAX_WARPS];
+    uint64_t sums_of_list[32 * WARPS];
   };
   uint64_t mass, mass_left;               // of the list behind top_k, and behind top_p
   uint32_t left;                          // elements of it then
-  uint64_t scan[MAX_WARPS];
-  int32_t lo[MAX_WARPS], hi[MAX_WARPS];
-  uint32_t kept[MAX_WARPS];
+  uint64_t scan[WARPS];
+  int32_t lo[WARPS], hi[WARPS];
+  uint32_t kept[WARPS];
   uint32_t listed;
   // what every CTA of the cluster says of its slice, sent here by it
   alignas(16) int4 scores[MAX_SPLIT];     // smallest, largest, bound
@@ -240,7 +240,7 @@ struct Row {
       f(v.w, 4 * g + 3);
     };
     constexpr int UNDER_WAY = RESIDENT ? 4 : 8;
-    const int step = blockDim.x;
+    constexpr int step = THREADS;
     int g = g0 + tid;
     for (; g + (UNDER_WAY - 1) * step < g1; g += UNDER_WAY * step) {
       int4 v[UNDER_WAY];
@@ -262,12 +262,12 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 
 // Exclusive sum of v over the threads of the CTA, and the sum of all.
 __device__ __forceinline__ uint64_t block_scan(Shared& s, uint64_t v, uint64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t inc = warp_scan(v);
   __syncthreads();   // (the scan before has been read)
   if (lane == 31) s.scan[warp] = inc;
   __syncthreads();
-  const uint64_t w = lane < warps ? s.scan[lane] : 0, sums = warp_scan(w);
+  const uint64_t w = lane < WARPS ? s.scan[lane] : 0, sums = warp_scan(w);
   total = __shfl_sync(FULL, sums, 31);
   return __shfl_sync(FULL, sums - w, warp) + inc - v;
 }
@@ -275,7 +275,7 @@ __device__ __forceinline__ uint64_t block_scan(Shared& s, uint64_t v, uint64_t& 
 // (no CTA still reads what was there: `r`, whose histogram it was)
 __device__ __forceinline__ void clear(const Row& r, uint32_t* hist) {
   r.sync();
-  for (int i = threadIdx.x; i < BINS / 4; i += blockDim.x) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < BINS / 4; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 }
 // The cut that leaves `need` of the elements with from <= d < to (there are as many), and all in front of them.
@@ -292,20 +292,22 @@ __device__ Cut cut_by_count(const Row& r, Shared& s, uint64_t need, uint64_t fro
       if (t <= span) atomicAdd(&hist[t >> shift], 1u);
     });
     r.sync();
-    const int per = BINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // four or eight bins a thread
-    uint32_t own[8];
+    constexpr int per = BINS / THREADS;
+    static_assert(per == 8, "two loads a thread");
+    const int bin0 = per * (int)threadIdx.x;
+    uint32_t own[per];
     const uint4 none = make_uint4(0, 0, 0, 0);   // (the last digit has fewer bits)
     const uint4 a = bin0 < 1 << bits ? sum_of_cluster(hist + bin0, r.split) : none;
-    const uint4 b = per > 4 && bin0 + 4 < 1 << bits ? sum_of_cluster(hist + bin0 + 4, r.split) : none;
+    const uint4 b = bin0 + 4 < 1 << bits ? sum_of_cluster(hist + bin0 + 4, r.split) : none;
     own[0] = a.x; own[1] = a.y; own[2] = a.z; own[3] = a.w; own[4] = b.x; own[5] = b.y; own[6] = b.z; own[7] = b.w;
     uint64_t sum = 0, total;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += own[k];
+    for (int k = 0; k < per; ++k) sum += own[k];
     uint64_t before = block_scan(s, sum, total);
     if (total < need) return {to, 0};   // (scores that change)
     if (before < need && need <= before + sum) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < per; ++k) {
         if (before < need && need <= before + own[k]) {
           s.found = bin0 + k;
           s.found_before = before;
@@ -343,16 +345,13 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
       }
     });
     r.sync();
-    const int per = WBINS / (int)blockDim.x, bin0 = per * (int)threadIdx.x;   // two or four bins a thread
+    static_assert(WBINS / THREADS == 4, "one load a thread and half of a bin");
+    const int bin0 = 4 * (int)threadIdx.x;
     uint64_t own[4], high[4];
-    sum_of_cluster(hist + (bin0 & ~3), r.split, own);
-    sum_of_cluster(hist + WBINS + (bin0 & ~3), r.split, high);
+    sum_of_cluster(hist + bin0, r.split, own);
+    sum_of_cluster(hist + WBINS + bin0, r.split, high);
 #pragma unroll
     for (int k = 0; k < 4; ++k) own[k] += high[k] << 16;
-    if (per == 2) {
-      if (bin0 & 2) { own[0] = own[2]; own[1] = own[3]; }
-      own[2] = own[3] = 0;
-    }
     uint64_t total, before = block_scan(s, own[0] + own[1] + own[2] + own[3], total);
     if (first) {
       need = need_of(total);
@@ -423,8 +422,8 @@ __device__ int collect(const Row& r, Shared& s, uint32_t last, int rank, int ind
 // 1.8 us; a search for both sums by halving took 6).
 template <typename Own, typename F>
 __device__ __forceinline__ uint64_t against_all(Shared& s, int n, const Own& own_of, const F& f) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int blocks = (n + 31) >> 5, parts = warps / blocks, part = warp / blocks, t = (warp - part * blocks) * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blocks = (n + 31) >> 5, parts = WARPS / blocks, part = warp / blocks, t = (warp - part * blocks) * 32 + lane;
   if (part < parts) {
     const auto own = own_of(min(t, n - 1));
     const int end = n * (part + 1) / parts;
@@ -440,12 +439,12 @@ __device__ __forceinline__ uint64_t against_all(Shared& s, int n, const Own& own
   return sum;
 }
 
-// The weights of the blocks b0, b0 + warps, .. < end of a row without a cut, all of whose places are valid, with a table of
+// The weights of the blocks b0, b0 + WARPS, .. < end of a row without a cut, all of whose places are valid, with a table of
 // weights below 2^27 (sixteen of them fit 32 bits) and above 0; returns how many elements the lane has seen.  A function of its
 // own, so that the registers hold the next block, on its way from global memory, and not what the kernel needs later.
 template <bool RESIDENT>
 __device__ __noinline__ uint32_t sum_blocks(const Row r, Shared& s, int b0, int end) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31;
   const int4* const at = reinterpret_cast<const int4*>(RESIDENT ? resident() : r.x);
   const int32_t* const table = r.in_smem();
   int4 next[GROUPS];
@@ -455,11 +454,11 @@ __device__ __noinline__ uint32_t sum_blocks(const Row r, Shared& s, int b0, int 
   };
   uint32_t seen = 0;
   if (b0 < end) request(b0);
-  for (int b = b0; b < end; b += warps) {
+  for (int b = b0; b < end; b += WARPS) {
     int4 v[GROUPS];
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) v[i] = next[i];
-    if (b + warps < end) request(b + warps);
+    if (b + WARPS < end) request(b + WARPS);
     uint32_t sum = 0;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
@@ -478,9 +477,9 @@ __device__ __noinline__ uint32_t sum_blocks(const Row r, Shared& s, int b0, int 
 __device__ __forceinline__ int bits_of(uint64_t range) { return max(1, 64 - __clzll((long long)range)); }   // of the largest distance
 
 template <bool RESIDENT>
-__global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ Params p) {
   __shared__ Shared s;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = p.split > 1 ? (int)cluster_rank() : 0, row = (int)blockIdx.x / p.split;
   int32_t* const slice_s = reinterpret_cast<int32_t*>(dynamic_smem);
   int32_t* const table_s = slice_s + (RESIDENT ? p.slice : 0);
@@ -507,10 +506,10 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   if (p.split > 1) cluster_arrive();   // (waited for before anything is sent)
   pdl_wait();
   // (what the set-up needs of global memory is requested at once: a trip each would be longer than the slice takes)
-  constexpr int EARLY = TABLE_SMEM_MAX / 512;
+  constexpr int EARLY = TABLE_SMEM_MAX / THREADS;
   int32_t entry[EARLY];
 #pragma unroll
-  for (int i = 0; i < EARLY; ++i) entry[i] = p.table_smem && tid + i * threads < d.table_len ? d.table[tid + i * threads] : 0;
+  for (int i = 0; i < EARLY; ++i) entry[i] = p.table_smem && tid + i * THREADS < d.table_len ? d.table[tid + i * THREADS] : 0;
   // whole 16-byte words by the bulk engine, the ragged ends by threads
   const int b0 = min((r.first + 3) & ~3, r.last), b1 = max(b0, r.last & ~3);
   if (RESIDENT && tid == 0) {
@@ -537,9 +536,9 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   bool plain = true;   // all entries are above 0 and below 2^27
 #pragma unroll
   for (int i = 0; i < EARLY; ++i)
-    if (p.table_smem && tid + i * threads < d.table_len) {
+    if (p.table_smem && tid + i * THREADS < d.table_len) {
       const int32_t w = (uint32_t)max(entry[i], 0) >= min_weight ? max(entry[i], 0) : 0;
-      table_s[tid + i * threads] = w;
+      table_s[tid + i * THREADS] = w;
       plain = plain && w > 0 && w < 1 << 27;
     }
   const bool plain_table = __syncthreads_and(plain) && p.table_smem;
@@ -577,11 +576,11 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   hi = __reduce_max_sync(FULL, hi);
   if (lane == 0) { s.lo[warp] = lo; s.hi[warp] = hi; }
   __syncthreads();
-  lo = __reduce_min_sync(FULL, lane < warps ? s.lo[lane] : INT32_MAX);
-  hi = __reduce_max_sync(FULL, lane < warps ? s.hi[lane] : INT32_MIN);
+  lo = __reduce_min_sync(FULL, lane < WARPS ? s.lo[lane] : INT32_MAX);
+  hi = __reduce_max_sync(FULL, lane < WARPS ? s.hi[lane] : INT32_MIN);
   int32_t bound = INT32_MIN;
   const int part = ((int32_t)of_row.x - 1) / p.split + 1;   // of top_k, for a CTA
-  if (cut_by_k() && part <= threads && __syncthreads_count(some) >= part) {
+  if (cut_by_k() && part <= THREADS && __syncthreads_count(some) >= part) {
     const uint32_t far = (uint32_t)hi - (uint32_t)mine;
     uint32_t from = 0, to = (uint32_t)hi - (uint32_t)lo;
     for (int i = 0; i < 14 && from < to; ++i) {   // (to some ten-thousandth of the range)
@@ -717,7 +716,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
       r.sync();
       // Every CTA adds up its share of the entries (a cluster's counts of all of them are 128 KB to fetch: 4 us), tells the
       // others its weight, and the one in whose share the target lies finds the entry for all.
-      const int parts = (int)r.split, part = parts > 1 ? rank : 0, share = BINS / parts, per = max(4, share / threads);
+      const int parts = (int)r.split, part = parts > 1 ? rank : 0, share = BINS / parts, per = max(4, share / THREADS);
       const uint32_t e0 = (uint32_t)(part * share + per * tid);
       const bool here = per * tid < share;
       const uint4 none = make_uint4(0, 0, 0, 0), a = here ? sum_of_cluster(hist + e0, r.split) : none;
@@ -776,10 +775,10 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
   const int whole0 = (r.first + BLOCK - 1) / BLOCK, whole1 = r.last / BLOCK;
   const bool straight = beyond && r.gentle && plain_table;
   if (straight) {
-    const int b0 = whole0 + (warp - whole0 % warps + warps) % warps;   // the warp's first of them
+    const int b0 = whole0 + (warp - whole0 % WARPS + WARPS) % WARPS;   // the warp's first of them
     kept += sum_blocks<RESIDENT>(r, s, b0, whole1);
   }
-  for (int b = warp; b < blocks; b += warps) {
+  for (int b = warp; b < blocks; b += WARPS) {
     const bool whole = b >= whole0 && b < whole1;
     if (straight && whole) continue;
     uint64_t mass = 0;
@@ -851,7 +850,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     if (rank == 0 && lane < p.split) store32(remote(&s.tie_weight, (uint32_t)lane), cut.ties ? r.weight((uint32_t)cut.D) : 0u);
   };
   if (warp == 0) {
-    kept = __reduce_add_sync(FULL, lane < warps ? s.kept[lane] : 0u);
+    kept = __reduce_add_sync(FULL, lane < WARPS ? s.kept[lane] : 0u);
     scan_blocks();
   }
   r.sync();
@@ -881,7 +880,7 @@ __global__ void __launch_bounds__(1024, 1) sample_kernel(const __grid_constant__
     cut = {0, 1};
     tie_weight = 1;
     r.sync();   // (nobody still reads the sums of before)
-    for (int b = warp; b < blocks; b += warps) {
+    for (int b = warp; b < blocks; b += WARPS) {
       uint32_t ties = 0;
       for (int j = max(b * BLOCK, r.first & ~31) + lane; j < min((b + 1) * BLOCK, r.last); j += 32) ties += j >= r.first && r.dist(x[j]) == 0;
       __syncwarp();
@@ -1001,27 +1000,27 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   // How many CTAs a row is cut over, and whether its slices are kept in shared memory.  The choice is by sizes, and by whether
   // rows may be cut (top_k or top_p given); us of one call in a chain of calls, kept (k) or read again from L2 (g), CTAs a row:
   //   - as many CTAs a row as are resident at once, two an SM (of clusters of eight 33, not 37: GPCs have 16 to 20 SMs), each with
-  //     4000 elements or more.  50021 elements, 64 rows, with cuts: k4 28, k8 44, g2 37; 150 rows without: g1 21, g2 30, k4 33.
-  //   - kept where two slices fit an SM.  131072 elements, 8 rows with cuts: k8 29, g8 35.  A CTA an SM, of 1024 threads, only
-  //     for the few rows of which all are resident then: 262144 elements, 8 rows with cuts: k8 31, g8 41; 37 rows 61 and 48.
+  //     4000 elements or more.  50021 elements, 64 rows, with cuts: k4 25, k8 38, g2 35; 150 rows without: g1 23, g2 30, k4 30.
+  //   - kept where two slices fit an SM.  131072 elements, 8 rows with cuts: k8 22, g8 28.  Slices of which one fits, only for
+  //     the few rows of which all are resident then: 262144 elements, 8 rows with cuts: k8 23, g8 28; 37 rows 54 and 52.
   //   - with cuts rows differ in how long they take, and more and shorter CTAs even that out: slices of 65536 at most.
-  //     262144 elements, 256 rows: g1 239, g2 207, g4 193, g8 260; 131072, 150 rows: g1 88, g2 66, g4 83.
+  //     262144 elements, 256 rows: g1 260, g2 223, g4 201, g8 256; 131072, 150 rows: g1 102, g2 78, g4 82.  Long slices may
+  //     for that be more than are resident at once.  40 rows of 262144: g4 71, g8 56; 180 of 100000: g1 90, g2 71; 150 of
+  //     50021: g1 48, g2 39, but 200: g1 55, g2 58.
   const int room = 226 * 1024 - (int)sizeof(Shared), half = 113 * 1024 - (int)sizeof(Shared) - 1024;
   const bool cuts = d->top_k || d->top_p;
   static const int at_once[4] = {296, 148, 71, 33};   // clusters of 1, 2, 4 and 8 CTAs, two an SM; 148 SMs
   int log2 = 0;
-  while (log2 < 3 && (int64_t)d->rows * 148 <= (int64_t)at_once[log2 + 1] * sms && slice_of(2 << log2) >= 4000) ++log2;
+  const auto at_work = [&](int log) {
+    const int slice = slice_of(1 << log);
+    return (int64_t)at_once[log] * sms / 148 * (!cuts || slice < 20000 ? 100 : (slice < 30000 ? 110 : 150)) / 100;
+  };
+  while (log2 < 3 && d->rows <= at_work(log2 + 1) && slice_of(2 << log2) >= 4000) ++log2;
   while (cuts && log2 < 3 && slice_of(1 << log2) > 65536 + 4) ++log2;
   p.split = 1 << log2;
-  bool resident = smem_of(p.split) <= half;
-  int threads = 512;
-  if (!resident && p.split == 8 && d->rows <= 14 * sms / 148 && smem_of(8) <= room) {
-    resident = true;
-    threads = 1024;
-  }
+  bool resident = smem_of(p.split) <= half || (p.split == 8 && d->rows <= 14 * sms / 148 && smem_of(8) <= room);
   if (const char* e = dev_env("CVM_B200_SAMPLE_SPLIT")) p.split = atoi(e);
   if (const char* e = dev_env("CVM_B200_SAMPLE_STREAM")) resident = atoi(e) == 0;
-  if (const char* e = dev_env("CVM_B200_SAMPLE_THREADS")) threads = atoi(e);
   p.slice = slice_of(p.split);
   const int smem = resident ? smem_of(p.split) : (p.table_smem ? d->table_len * 4 : 0);
 
@@ -1036,7 +1035,7 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(d->rows * p.split));
-  cfg.blockDim = dim3((unsigned)threads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];
