@@ -136,6 +136,19 @@ def test_each_filter_alone_and_greedy(kn):
     assert np.array_equal(token, x.argmax(1))          # the lowest index of equal scores
 
 
+# Counts around what a list holds (512 elements), cuts among equal scores, weights of 31 bits
+@pytest.mark.parametrize("kind", ["normal", "ties", "equal"])
+@pytest.mark.parametrize("vocab", [601, 9001])
+def test_long_lists(kn, vocab, kind):
+    rng = np.random.RandomState(vocab + 1)
+    k = np.array([33, 64, 255, 256, 257, 400, 496, 511, 512, 513, 600], np.int64)
+    x = logits(rng, len(k), vocab, kind)
+    u = rng.randint(0, 2**31, len(k))
+    for table in (EXP, np.full(700, 2**31 - 1, np.int32), np.zeros(5, np.int32)):
+        run(kn, x, table, 20000, u, top_k=k)
+        run(kn, x, table, 20000, u, top_k=k, top_p=rng.choice([1, ONE // 3, ONE - 1], len(k)), min_p=rng.choice([0, ONE // 100], len(k)))
+
+
 def test_the_draw_follows_the_weights(kn):
     """Random numbers at even steps: every element comes up within one step of its share."""
     x = np.array([[0, -300, -600, -100000, 0, -50]], np.int32)
