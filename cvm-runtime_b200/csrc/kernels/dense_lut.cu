@@ -908,33 +908,39 @@ bool by_tma(const cvmk_dense_lut_desc& d) {
   return !((uintptr_t)d.y & 15) && d.y_pitch * d.y_dtype % 16 == 0 && (int64_t)d.units * d.y_dtype % 16 == 0;
 }
 
+bool is_tensor_step(const cvmk_ep_step& s) { return s.op == CVMK_EP_ADD_T || s.op == CVMK_EP_SUB_T || s.op == CVMK_EP_RSUB_T; }
+
 // Which kernel runs a layer, and how the small one cuts it (rows of x a tile, CTAs that share its reduction): every cut, and the
-// pairs of CTAs, are given a time, and the least of them is taken.  The terms, in microseconds of a launch in a chain of launches
-// (of 40 shapes, 1 to 2000 rows, 176 to 8192 long, 35 to 16384 units, each cut timed; most are within 10 %):
-//   small   4 for the launch, 0.045 a row of the tile for its last steps, 0.19 a block of K (a load's latency, a ring of several
-//           in flight), all operands at 8 MB a microsecond out of L2 and the weights at 6 out of memory, 1.1 for the exchange
-//           of partial sums; times the rounds of CTAs, two an SM up to 32 rows and one beyond, and of clusters as many as
-//           are resident at once (GPCs have 16 to 20 SMs).
-//   pairs   5.3 for the launch (6.8 where rows of y do not begin on 16 bytes), 0.1 a block of K to fill the ring, and a round of
-//           tiles the longer of 0.28 a block and 2.7 for its last steps.
+// pairs of CTAs, are given a time, and the least of them is taken.  The terms, in microseconds of a launch in a chain of launches,
+// fitted to 1500 shapes (1 to 8192 rows, 64 to 8192 long, 32 to 16384 units, each cut timed) and checked with 8500 others: what
+// is chosen takes 1.9 % longer than the best cut, in the mean:
+//   small   2.7 for the launch, 0.058 a row of the tile for its last steps, 0.35 a block of K (a load's latency, a ring of several
+//           in flight), all operands and tables at 9.4 MB a microsecond out of L2 and the weights at 6 out of memory, 2.2 for the
+//           exchange of partial sums; times the rounds of CTAs (0.5 each beyond the first), two an SM up to 64 rows and one
+//           beyond, and of clusters as many as are resident at once (GPCs have 16 to 20 SMs).
+//   pairs   5.3 for the launch, 0.1 a block of K to fill the ring, and a round of tiles the longer of 0.42 a block and its last
+//           steps: 2.7, or where rows of y do not begin on 16 bytes 3.3, 0.6 more for int32 and 1.2 with a tensor operand; the
+//           shorter of the two 1.9 times, in the first and the last round.
 // Cut over rows, a layer of few units uses the whole GPU: 128 rows 176 -> 122 14.8 us in one tile of rows and 5.4 in eight, 1000
 // rows 1024 -> 250 gated 6.2 in 63 (pairs 11.1).  Cut in K: 8 rows 4096 -> 4096 whole 10.6, in four 7.5.
 struct Cut { int row_tile, split; };   // split 0: pairs
 Cut choose(const cvmk_dense_lut_desc& d, int kblocks, int sms) {
   const double weights = (double)d.units * d.K * (d.v ? 2 : 1);
   const int64_t pair_tiles = (int64_t)((d.rows + 255) / 256) * ((d.units + (d.v ? 127 : 255)) / (d.v ? 128 : 256)), pairs = sms / 2;
-  const bool aligned = by_tma(d);
+  bool operand = false;
+  for (int i = 0; i < d.chain_y.n; ++i) operand = operand || is_tensor_step(d.chain_y.s[i]);
+  const double last = by_tma(d) ? 2.7 : 3.3 + (d.y_dtype == CVMK_I32 ? 0.6 : 0.0) + (operand ? 1.2 : 0.0), products = 0.42 * kblocks;
   Cut best = {256, 0};
-  double least = (aligned ? 5.3 : 6.8) + 0.1 * kblocks + std::max((pair_tiles + pairs - 1) / pairs * std::max(0.28 * kblocks, 2.7), weights / 6e6);
+  double least = 5.3 + 0.1 * kblocks + std::max((pair_tiles + pairs - 1) / pairs * std::max(products, last) + 1.9 * std::min(products, last), weights / 6e6);
   static const int at_once[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};   // clusters of 1, 2, 4 and 8 CTAs, one and two an SM; 148 SMs
-  for (int row_tile = 16; row_tile <= 128; row_tile *= 2) {
+  for (const int row_tile : {16, 32, 48, 64, 96, 128}) {
     const int rt = std::min(row_tile, (std::min(d.rows, 128) + 15) & ~15);
     const int64_t tiles = (int64_t)((d.units + (d.v ? 63 : 127)) / (d.v ? 64 : 128)) * ((d.rows + rt - 1) / rt);
     for (int log2 = 0; log2 < 4 && (log2 == 0 || kblocks >= 4 << log2); ++log2) {
       const int split = 1 << log2, per = (kblocks + split - 1) / split;
-      const int64_t room = std::max<int64_t>((int64_t)at_once[rt <= 32][log2] * sms / 148, 1), rounds = (tiles + room - 1) / room;
-      const double bytes = (double)tiles * split * per * (W_BYTES + rt * BLOCK_K);
-      const double us = 4.0 + 0.045 * rt * rounds + std::max({0.19 * per * rounds, bytes / 8e6, weights / 6e6}) + (split > 1 ? 1.1 : 0.0);
+      const int64_t room = std::max<int64_t>((int64_t)at_once[rt <= 64][log2] * sms / 148, 1), rounds = (tiles + room - 1) / room;
+      const double bytes = (double)tiles * split * (per * (W_BYTES + rt * BLOCK_K) + (double)d.table_len * d.table_dtype);
+      const double us = 2.7 + 0.058 * rt * rounds + std::max({0.35 * per * rounds, bytes / 9.4e6, weights / 6e6}) + (split > 1 ? 2.2 : 0.0) + 0.5 * (rounds - 1);
       if (us < least) {
         least = us;
         best = {rt, split};
@@ -963,7 +969,6 @@ int encode_operands(cvmk_dense_lut_plan* plan, int x_rows, int w_rows) {
   return CVMK_OK;
 }
 
-bool is_tensor_step(const cvmk_ep_step& s) { return s.op == CVMK_EP_ADD_T || s.op == CVMK_EP_SUB_T || s.op == CVMK_EP_RSUB_T; }
 bool is_tensor_op(int op) { return op == K_ADD_T || op == K_SUB_T || op == K_RSUB_T; }
 bool is_type(int t) { return t == CVMK_I8 || t == CVMK_I32; }
 
@@ -1131,7 +1136,8 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
   plan->row_tile = cut.row_tile;
   plan->split = cut.split;
   const int64_t tiles = (int64_t)((p.units + tile_units - 1) / tile_units) * ((p.rows + plan->row_tile - 1) / plan->row_tile);
-  const int limit = plan->row_tile <= 32 ? 112 * 1024 : SMALL_SMEM_MAX;
+  // (two CTAs an SM, with a shorter ring: 4835 rows 660 -> 293 in tiles of 64 13.4 us, one an SM 22.3)
+  const int limit = plan->row_tile <= 64 ? 112 * 1024 : SMALL_SMEM_MAX;
   auto smem_of = [&](int stages) { return 1024 + small_ring_bytes(plan->row_tile, stages) + table_room; };
   plan->stages = std::min((kblocks + plan->split - 1) / plan->split, MAX_STAGES);
   while (plan->stages > 2 && smem_of(plan->stages) > limit) --plan->stages;

@@ -80,6 +80,15 @@ def test_sizes(kn, rows, k, units, gated):
     Case(kn, rows, k, units, gated, pad=rows % 2, seed=rows + k, residual=(kn.ADD_T, 1) if units % 2 else None).run(params_static=bool(k % 2))
 
 
+@pytest.mark.parametrize("y_dtype", [1, 4])
+def test_tiles_of_48_and_96_rows(kn, y_dtype):
+    tiles = set()
+    for rows, k, units in ((33, 3051, 10231), (209, 1037, 2777), (517, 3340, 193), (2985, 5312, 84), (3904, 2368, 130)):
+        plan = Case(kn, rows, k, units, units < 10000, (256, 1), y_dtype, seed=rows, pad=1).run()
+        tiles.add(plan.row_tile)
+    assert {48, 96} <= tiles
+
+
 @pytest.mark.parametrize("rows,k,units", [(1, 256, 70), (37, 300, 200), (260, 192, 150), (700, 130, 300)])
 @pytest.mark.parametrize("table", [(1, 1), (2, 4), (300, 1), (1000, 4), (4096, 4), (4097, 4), (20000, 1)])
 @pytest.mark.parametrize("y_dtype", [1, 4])
@@ -242,8 +251,20 @@ def test_other_chains(kn, rows, units, front):
             Case(kn, rows, 500, units, gated, (256, 1), y_dtype, after=after, front=w, front_v=v if gated else None, seed=front).run()
 
 
+# Pairs of CTAs, results whose rows end off 16 bytes; tables that stay where they lie, and a chain step by step
+@pytest.mark.parametrize("rows,k,units", [(1100, 70, 6973), (2100, 130, 1999)])
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("residual", [None, ("ADD_T", 1), ("RSUB_T", 4)])
+@pytest.mark.parametrize("table", [(256, 1), (1000, 4), (20000, 1)])
+def test_pairs_off_16_bytes(kn, rows, k, units, gated, residual, table):
+    for y_dtype in (1, 4):
+        for front in (None, [(kn.CLIP, -100000, 90000), (kn.RSHIFT, 9, 9), (kn.CLIP, 0, 250)]):
+            plan = Case(kn, rows, k, units, gated, table, y_dtype, (getattr(kn, residual[0]), residual[1]) if residual else None, seed=units, front=front).run()
+            assert plan.kernel == 1 and plan.io == 0
+
+
 def test_sizes_drawn_at_random(kn):
-    """Every cut that sizes of 1 to 3000 rows, 1 to 3000 long, 1 to 3000 units lead to."""
+    """Every cut that sizes of 1 to 3000 rows, 1 to 3000 long, 1 to 3000 units lead to, and two that lead to pairs of CTAs."""
     rng = np.random.RandomState(17)
     cuts = set()
     for i in range(60):
@@ -251,6 +272,8 @@ def test_sizes_drawn_at_random(kn):
         plan = Case(kn, rows, k, units, i % 2 == 0, [(256, 1), (1000, 4)][i % 3 == 0], [1, 4][i % 5 == 0], (kn.ADD_T, 1) if i % 4 == 0 else None, seed=i,
                     y_pitch=(units + 15) // 16 * 16 if i % 7 < 3 else None).run(params_static=bool(i % 2))
         cuts.add((plan.kernel, plan.split))
+    for rows, k, units in ((300, 1200, 9000), (2800, 900, 2900)):
+        cuts.add((Case(kn, rows, k, units, seed=rows).run().kernel, 1))
     assert {kernel for kernel, _ in cuts} == {0, 1} and max(split for _, split in cuts) > 1
 
 
