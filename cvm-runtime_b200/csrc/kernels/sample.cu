@@ -998,27 +998,32 @@ extern "C" int cvmk_sample(const cvmk_sample_desc* d, cvmk_stream_t stream) {
   auto slice_of = [&](int split) { return ((d->vocab + 3 + split - 1) / split + 3) & ~3; };
   auto smem_of = [&](int split) { return slice_of(split) * 4 + (p.table_smem ? d->table_len * 4 : 0); };
   // How many CTAs a row is cut over, and whether its slices are kept in shared memory.  The choice is by sizes, and by whether
-  // rows may be cut (top_k or top_p given); us of one call in a chain of calls, kept (k) or read again from L2 (g), CTAs a row:
+  // rows may be cut (top_k or top_p given); of 14000 drawn sizes (1 to 512 rows, 300 to 262144 elements) it takes 2 % longer than
+  // the best, in the mean.  us of one call in a chain of calls, kept (k) or read again from L2 (g), CTAs a row:
   //   - as many CTAs a row as are resident at once, two an SM (of clusters of eight 33, not 37: GPCs have 16 to 20 SMs), each with
-  //     4000 elements or more.  50021 elements, 64 rows, with cuts: k4 25, k8 38, g2 35; 150 rows without: g1 23, g2 30, k4 30.
-  //   - kept where two slices fit an SM.  131072 elements, 8 rows with cuts: k8 22, g8 28.  Slices of which one fits, only for
-  //     the few rows of which all are resident then: 262144 elements, 8 rows with cuts: k8 23, g8 28; 37 rows 54 and 52.
-  //   - with cuts rows differ in how long they take, and more and shorter CTAs even that out: slices of 65536 at most.
-  //     262144 elements, 256 rows: g1 260, g2 223, g4 201, g8 256; 131072, 150 rows: g1 102, g2 78, g4 82.  Long slices may
-  //     for that be more than are resident at once.  40 rows of 262144: g4 71, g8 56; 180 of 100000: g1 90, g2 71; 150 of
-  //     50021: g1 48, g2 39, but 200: g1 55, g2 58.
+  //     4000 elements or more, with cuts 7000.  50021 elements, 64 rows, with cuts: k4 25, k8 38, g2 35; 150 rows without: g1 23,
+  //     g2 30, k4 30.
+  //   - with cuts rows differ in how long they take, and more and shorter CTAs even that out: slices of 90000 at most, and long
+  //     ones may be more than are resident at once.  262144 elements, 256 rows: g1 260, g2 223, g4 201, g8 256; 131072, 150 rows:
+  //     g1 102, g2 78, g4 82; 147285, 39 rows: g4 43, k8 29; 100000, 180 rows: g1 90, g2 71; but 50021, 200 rows: g1 55, g2 58.
+  //   - kept where two slices fit an SM, or one where no SM has two.  131072 elements, 8 rows with cuts: k8 22, g8 28; 262144:
+  //     k8 23, g8 28.  Where that many CTAs have an SM each, no more are made: 48375 elements, 129 rows without cuts k1 12, k2 17;
+  //     but with cuts only for one CTA a row: 131072 elements, 32 rows with top_k in all k4 14, k8 20, with top_p alone in
+  //     every third k4 32, k8 27.
   const int room = 226 * 1024 - (int)sizeof(Shared), half = 113 * 1024 - (int)sizeof(Shared) - 1024;
   const bool cuts = d->top_k || d->top_p;
-  static const int at_once[4] = {296, 148, 71, 33};   // clusters of 1, 2, 4 and 8 CTAs, two an SM; 148 SMs
-  int log2 = 0;
+  static const int two_an_sm[4] = {296, 148, 71, 33}, one_an_sm[4] = {148, 74, 33, 15};   // clusters of 1, 2, 4 and 8 CTAs; 148 SMs
   const auto at_work = [&](int log) {
     const int slice = slice_of(1 << log);
-    return (int64_t)at_once[log] * sms / 148 * (!cuts || slice < 20000 ? 100 : (slice < 30000 ? 110 : 150)) / 100;
+    return (int64_t)two_an_sm[log] * sms / 148 * (!cuts || slice < 12000 ? 100 : (slice < 30000 ? 120 : 150)) / 100;
   };
-  while (log2 < 3 && d->rows <= at_work(log2 + 1) && slice_of(2 << log2) >= 4000) ++log2;
-  while (cuts && log2 < 3 && slice_of(1 << log2) > 65536 + 4) ++log2;
+  const auto alone = [&](int log) { return d->rows <= (int64_t)one_an_sm[log] * sms / 148; };
+  int log2 = 0;
+  while (log2 < 3 && d->rows <= at_work(log2 + 1) && slice_of(2 << log2) >= (cuts ? 7000 : 4000) &&
+         !((!cuts || log2 == 0) && alone(log2) && !alone(log2 + 1) && smem_of(1 << log2) <= room)) ++log2;
+  while (cuts && log2 < 3 && slice_of(1 << log2) > 90000) ++log2;
   p.split = 1 << log2;
-  bool resident = smem_of(p.split) <= half || (p.split == 8 && d->rows <= 14 * sms / 148 && smem_of(8) <= room);
+  bool resident = smem_of(p.split) <= half || (smem_of(p.split) <= room && alone(log2));
   if (const char* e = dev_env("CVM_B200_SAMPLE_SPLIT")) p.split = atoi(e);
   if (const char* e = dev_env("CVM_B200_SAMPLE_STREAM")) resident = atoi(e) == 0;
   p.slice = slice_of(p.split);
