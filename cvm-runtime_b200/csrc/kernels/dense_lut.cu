@@ -13,7 +13,7 @@
 // tiles with the requantisation of one beside the products of the next (two accumulators).
 //
 // What bounds them (one B200, among other launches): the small kernel the stream of weights (24 rows 4096 -> 16384 gated,
-// 134 MB: 24.7 us, 0.83 of the copy rate) or, under 10 us, a trip to memory and the steps of a tile one after another (1 row
+// 134 MB: 24 us, 0.85 of the copy rate) or, under 10 us, a trip to memory and the steps of a tile one after another (1 row
 // 2048 -> 8192 gated, 33.6 MB: 7.8 us); the pair kernel the tensor pipe (4096 rows 4096 -> 16384 gated: 316 us in a burst, 0.78 of
 // the measured rate of its instructions, 366 where a long run meets the power limit), and the requantisation where K is short
 // (6000 rows 2048 -> 8192 with a residual: 73 us in a burst, 89 in a long run, 45 for the products alone).

@@ -19,7 +19,7 @@
 // Counts and weights are whole numbers, so their order of summation changes nothing.
 //
 // What bounds it: few rows, the chain of passes and barriers, each a trip to L2 or over a cluster (1 row of 32000 elements, all
-// filters: 9.5 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 27 us, 2.6).  Many rows, the passes themselves: 256 rows
+// filters: 9.9 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 27 us, 2.6).  Many rows, the passes themselves: 256 rows
 // of 262144 elements take 107 us without cuts (read twice: once from memory, 41 us at the rate of a copy, once from L2), 124 with
 // top_k, 251 with top_p, whose counting is an atomic in shared memory for every element above the table's last entry.  More loads
 // under way (the next four requested while four are worked on) spill at the 64 registers that two CTAs an SM leave: 190 against
