@@ -15,11 +15,11 @@
 //   A cut by count is found digit by digit: a histogram of the next twelve bits of d over the elements that share the bits
 //   before, and the bin in which the running count reaches the target.  (With a table too long for shared memory top_p goes
 //   that way too, by weight.)
-// The draw then sums the weights in blocks of 512 elements, finds the block, and looks up the element in it.
+// The draw then sums the weights in blocks of 256 or 512 elements, finds the block, and looks up the element in it.
 // Counts and weights are whole numbers, so their order of summation changes nothing.
 //
 // What bounds it: few rows, the chain of passes and barriers, each a trip to L2 or over a cluster (1 row of 32000 elements, all
-// filters: 9.9 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 27 us, 2.6).  Many rows, the passes themselves: 256 rows
+// filters: 9.9 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 26 us, 2.6).  Many rows, the passes themselves: 256 rows
 // of 262144 elements take 107 us without cuts (read twice: once from memory, 41 us at the rate of a copy, once from L2), 124 with
 // top_k, 251 with top_p, whose counting is an atomic in shared memory for every element above the table's last entry.  More loads
 // under way (the next four requested while four are worked on) spill at the 64 registers that two CTAs an SM leave: 190 against
@@ -40,7 +40,13 @@ constexpr int WDIGIT = 11, WBINS = 1 << WDIGIT;    // of weights, two words a bi
 constexpr int TABLE_SMEM_MAX = 4096;    // entries; with more the table stays where it lies
 constexpr int LIST = 512;               // elements on a list
 constexpr int MAX_SPLIT = 8;
-constexpr int BLOCK = 512, GROUPS = BLOCK / 128, MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / BLOCK + 2;
+// Elements of a block of the draw: few, for even shares of the warps and a short search in the one that is hit, where they lie in
+// shared memory (32 rows of 131072: 25.9 us with 256, 27.0 with 512); more requests at once where they do not (256 rows of 262144:
+// 175 us with 512, 181 with 256).
+template <bool RESIDENT>
+constexpr int BLOCK_OF = RESIDENT ? 256 : 512;
+constexpr int MAX_BLOCKS = CVMK_SAMPLE_MAX_VOCAB / BLOCK_OF<false> + 2;   // (a resident slice has fewer: 56 K elements at most)
+static_assert(56 * 1024 / BLOCK_OF<true> + 2 <= MAX_BLOCKS, "room for the blocks of a resident slice");
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr uint64_t ONE = 1u << 30;
 constexpr int RANK_BITS = 10;           // behind a weight: one each for the elements in front
@@ -444,6 +450,7 @@ __device__ __forceinline__ uint64_t against_all(Shared& s, int n, const Own& own
 // own, so that the registers hold the next block, on its way from global memory, and not what the kernel needs later.
 template <bool RESIDENT>
 __device__ __noinline__ uint32_t sum_blocks(const Row r, Shared& s, int b0, int end) {
+  constexpr int BLOCK = BLOCK_OF<RESIDENT>, GROUPS = BLOCK / 128;
   const int lane = threadIdx.x & 31;
   const int4* const at = reinterpret_cast<const int4*>(RESIDENT ? resident() : r.x);
   const int32_t* const table = r.in_smem();
@@ -767,6 +774,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   }
 
   // ---- the draw: weights and ties of every block of the slice
+  constexpr int BLOCK = BLOCK_OF<RESIDENT>, GROUPS = BLOCK / 128;
   const int blocks = (r.last + BLOCK - 1) / BLOCK;
   uint32_t kept = 0;
   const uint32_t D32 = (uint32_t)min(cut.D, end - 1);
