@@ -137,7 +137,7 @@ struct Cut {
 
 struct Shared {
   union {
-    alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 16 bits, and the rest
+    alignas(16) uint32_t hist[BINS];   // counts by digit or table index; weights by digit: the low 32 bits, and the high ones
     struct {                           // (a row whose cuts are found on its list needs no histogram behind it)
       alignas(16) uint4 all[LIST];     // of the row's elements: index, distance, and 64 bits to be added up
       union {
@@ -345,9 +345,10 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
     r.each<RESIDENT>([&](int32_t v, int) {
       const uint32_t d = r.dist(v);
       if (d < whole.D && (uint64_t)d >> (shift + bits) == prefix) {
+        // 64 bits a bin, whatever a slice holds: the low word as it wraps, and how often it did.  (Two additions of half a weight,
+        // which need no answer, hold 65537 elements a bin, and slices are longer.  256 rows of 262144, 8192 entries: 514 us, with those 501.)
         const uint32_t w = r.weight(d), bin = (d >> shift) & ((1u << bits) - 1u);
-        if (w & 0xffffu) atomicAdd(&hist[bin], w & 0xffffu);
-        if (w >> 16) atomicAdd(&hist[WBINS + bin], w >> 16);
+        if (w && atomicAdd(&hist[bin], w) > 0xffffffffu - w) atomicAdd(&hist[WBINS + bin], 1u);
       }
     });
     r.sync();
@@ -357,7 +358,7 @@ __device__ Cut cut_by_weight(const Row& r, Shared& s, int range_bits, const Need
     sum_of_cluster(hist + bin0, r.split, own);
     sum_of_cluster(hist + WBINS + bin0, r.split, high);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) own[k] += high[k] << 16;
+    for (int k = 0; k < 4; ++k) own[k] += high[k] << 32;
     uint64_t total, before = block_scan(s, own[0] + own[1] + own[2] + own[3], total);
     if (first) {
       need = need_of(total);
