@@ -42,7 +42,8 @@ constexpr uint32_t FULL_MASK = 0xffffffffu;
 
 // A chain of a rounding shift with clamps, and for the one in front of a table the sum with a constant and the table's
 // bounds, in three instructions: max(min(sum + (bias + add), hi), lo) >> shift.  The clamps come before the shift, which
-// is monotone; nothing overflows while |bias + add| <= room, which the kernel looks at 32 biases at a time.
+// is monotone.  That is the definition's result where neither sum + bias, which wraps there, nor sum + bias + add overflows:
+// while |bias| <= room and |bias + add| <= room, which the kernel looks at 32 biases at a time.
 struct Requant {
   int on, add, lo, hi, shift, room;
 };
@@ -132,8 +133,8 @@ __device__ __forceinline__ void copy_table(const Params& p, uint8_t* table_s, in
 
 // Whether the bias leaves room for the sum (see Requant).
 __device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) {
-  const long long b = (long long)bias + q.add;
-  return b <= q.room && b >= -(long long)q.room;
+  const long long room = q.room, moved = (long long)bias + q.add;
+  return bias <= room && bias >= -room && moved <= room && moved >= -room;
 }
 // One channel's sums; `bias` has q.add in it.
 template <int V>
