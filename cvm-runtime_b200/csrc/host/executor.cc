@@ -1054,14 +1054,13 @@ struct Lowering {
       if (is_tensor_step(d.chain_y.s[i])) d.chain_y.s[i].ptr_dtype = buf[(uint32_t)((uintptr_t)d.chain_y.s[i].ptr - 1)].dtype;
     if (!cvmk_dense_lut_supported(&d)) return false;
 
+    // (on the stream whose kernel reads the table below: a small cudaMemcpy() may return when its bytes are staged, and this stream
+    // does not wait for the default one)
     auto upload = [&](const HostTensor& t, bool as8) {
       void* at = ex.dalloc(t.data.size() * (as8 ? 1 : 4));
-      if (as8) {
-        const std::vector<int8_t> v8(t.data.begin(), t.data.end());
-        CUDA_OK(cudaMemcpy(at, v8.data(), v8.size(), cudaMemcpyHostToDevice));
-      } else {
-        CUDA_OK(cudaMemcpy(at, t.data.data(), t.data.size() * 4, cudaMemcpyHostToDevice));
-      }
+      const std::vector<int8_t> v8(as8 ? t.data.begin() : t.data.end(), t.data.end());
+      CUDA_OK(cudaMemcpyAsync(at, as8 ? (const void*)v8.data() : t.data.data(), t.data.size() * (as8 ? 1 : 4), cudaMemcpyHostToDevice, ex.stream_));
+      CUDA_OK(cudaStreamSynchronize(ex.stream_));
       return at;
     };
     auto weights = [&](const Side& s) { return (const int8_t*)upload(g.params.find(g.entry_id(g.nodes[s.dense].inputs[1]))->second, true); };
