@@ -43,9 +43,9 @@ constexpr uint32_t FULL_MASK = 0xffffffffu;
 // A chain of a rounding shift with clamps, and for the one in front of a table the sum with a constant and the table's
 // bounds, in three instructions: max(min(sum + (bias + add), hi), lo) >> shift.  The clamps come before the shift, which
 // is monotone.  That is the definition's result where neither sum + bias, which wraps there, nor sum + bias + add overflows:
-// while |bias| <= room and |bias + add| <= room, which the kernel looks at 32 biases at a time.
+// for biases from `least` to `most`, which the kernel looks at 32 biases at a time.
 struct Requant {
-  int on, add, lo, hi, shift, room;
+  int on, add, lo, hi, shift, least, most;
 };
 
 struct Params {
@@ -132,10 +132,7 @@ __device__ __forceinline__ void copy_table(const Params& p, uint8_t* table_s, in
 }
 
 // Whether the bias leaves room for the sum (see Requant).
-__device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) {
-  const long long room = q.room, moved = (long long)bias + q.add;
-  return bias <= room && bias >= -room && moved <= room && moved >= -room;
-}
+__device__ __forceinline__ bool in_room(int32_t bias, const Requant& q) { return bias >= q.least && bias <= q.most; }
 // One channel's sums; `bias` has q.add in it.
 template <int V>
 __device__ __forceinline__ void requant_one(int32_t bias, const Requant& q, int32_t (&v)[V]) {
@@ -888,7 +885,7 @@ CUresult encode_matrix(CUtensorMap* map, const void* base, int64_t rows, int64_t
 
 // The three-instruction form of a lowered chain from step `first` on, in front of a table of `len` entries or not (0).
 Requant requant_of(const DevChain& c, int first, int len, int K) {
-  Requant q = {0, 0, 0, 0, 0, 0};
+  Requant q = {0, 0, 0, 0, 0, 0, 0};
   const int left = c.n - first;
   if (left < 1 || left > (len ? 2 : 1) || c.s[first].op != K_RS_CLAMP || (left == 2 && c.s[first + 1].op != K_ADD_S)) return q;
   const DevStep& rs = c.s[first];
@@ -898,9 +895,10 @@ Requant requant_of(const DevChain& c, int first, int len, int K) {
     lo = std::max<int64_t>(lo, 0);
     hi = std::min<int64_t>(hi, ((int64_t)len << rs.d) - 1);
   }
-  const int64_t room = (int64_t)INT32_MAX - ((int64_t)K << 14);
-  if (lo > hi || lo < INT32_MIN || hi > INT32_MAX || add < INT32_MIN || add > INT32_MAX || room < 0) return q;
-  return {1, (int)add, (int)lo, (int)hi, rs.d, (int)room};
+  const int64_t room = (int64_t)INT32_MAX - ((int64_t)K << 14);   // |bias| and |bias + add| up to this; a sum is K * 2^14 at most
+  const int64_t least = std::max(-room, -room - add), most = std::min(room, room - add);
+  if (lo > hi || lo < INT32_MIN || hi > INT32_MAX || add < INT32_MIN || add > INT32_MAX || least > most) return q;
+  return {1, (int)add, (int)lo, (int)hi, rs.d, (int)least, (int)most};
 }
 
 // Whether y can be stored by TMA: rows begin on 16 bytes, and they end on them, because a store writes whole 16 bytes where the
