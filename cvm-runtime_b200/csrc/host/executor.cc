@@ -1029,7 +1029,6 @@ struct Lowering {
     cvmk_dense_lut_desc d;
     memset(&d, 0, sizeof(d));
     int tensors = 0;
-    if (!gated) d.chain_y = first.after;
     while (d.chain_y.n < CVMK_MAX_EP_STEPS) {
       const uint32_t next = only_consumer(tail, last);
       cvmk_ep_step st;
@@ -1045,7 +1044,8 @@ struct Lowering {
     d.rows = (int32_t)shape[0]; d.units = (int32_t)shape[1]; d.K = (int32_t)g.shape[x_eid][1];
     d.y_dtype = buf[tail].dtype;
     d.table_len = (int32_t)table.data.size();
-    d.table_dtype = narrow ? CVMK_I8 : CVMK_I32;
+    // Steps between the table and the product, or what follows it, are functions of an entry: the table goes through them once, here.
+    d.table_dtype = (first.after.n ? safe8[first.end_eid] : narrow) ? CVMK_I8 : CVMK_I32;
     d.params_static = 1;
     d.chain_w = first.before;
     d.x = d.w = (const int8_t*)16;   // (sizes, types and chains decide)
@@ -1080,13 +1080,11 @@ struct Lowering {
     d.y = out.ptr;
     d.status = ex.status_dev_;
     d.table = upload(table, narrow);
-    if (gated && first.after.n) {
-      // steps between the table and the product are functions of an entry: the table goes through them once
-      void* through = ex.dalloc(table.data.size() * 4);
-      KERNEL_OK(cvmk_elemwise(d.table, d.table_dtype, through, CVMK_I32, (int64_t)table.data.size(), &first.after, ex.stream_));
+    if (first.after.n) {
+      void* through = ex.dalloc(table.data.size() * d.table_dtype);
+      KERNEL_OK(cvmk_elemwise(d.table, narrow ? CVMK_I8 : CVMK_I32, through, d.table_dtype, (int64_t)table.data.size(), &first.after, ex.stream_));
       CUDA_OK(cudaStreamSynchronize(ex.stream_));
       d.table = through;
-      d.table_dtype = CVMK_I32;
     }
     void* mem = nullptr;
     CHECK(posix_memalign(&mem, 64, sizeof(cvmk_dense_lut_plan)) == 0);
