@@ -1125,6 +1125,11 @@ extern "C" int cvmk_dense_lut_prepare(const cvmk_dense_lut_desc* d, cvmk_dense_l
       if (is_tensor_step(e->s[i])) odd |= (uintptr_t)e->s[i].ptr & (e->s[i].ptr_dtype - 1);
     }
   if (odd) { set_error("dense_lut_prepare: an operand is not aligned to its elements"); return CVMK_ERR_ARG; }
+  for (int i = 0; i < p.chain_y.n; ++i)
+    if (is_tensor_step(p.chain_y.s[i]) && p.chain_y.s[i].ptr == p.y && p.chain_y.s[i].ptr_dtype != p.y_dtype) {
+      set_error("dense_lut_prepare: a tensor operand that is y has y's type");   // (another thread's result would lie on it)
+      return CVMK_ERR_ARG;
+    }
   if (!encoder()) { set_error("dense_lut_prepare: the driver has no cuTensorMapEncodeTiled"); return CVMK_ERR_CUDA; }
 
   if (check_cuda(cudaGetDevice(&plan->device), "dense_lut_prepare: cudaGetDevice")) return CVMK_ERR_CUDA;

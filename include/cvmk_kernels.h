@@ -479,7 +479,7 @@ CVMK_API int cvmk_transpose_batched(const void* x, void* y, int32_t dtype, int64
  * rows >= 0 (none: the launch does nothing), 1 <= units, table_len < 2^31.
  * chain_w and chain_v may begin with ADD_C (the bias, `units` int32) and hold no other step with an operand;
  * chain_y may hold one *_T step, whose tensor has y's shape and pitch.  No two tensors overlap, but a *_T
- * operand may be y itself.
+ * operand of y's type may be y itself.
  *
  * cvmk_dense_lut_prepare() chooses the kernel and encodes the tensor maps into `plan` (host memory of the
  * caller, 64-byte aligned; to be repeated if an operand moves); it wants the device current that will run
