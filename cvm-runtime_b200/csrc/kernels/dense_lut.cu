@@ -13,10 +13,10 @@
 // tiles with the requantisation of one beside the products of the next (two accumulators).
 //
 // What bounds them (one B200, among other launches): the small kernel the stream of weights (24 rows 4096 -> 16384 gated,
-// 134 MB: 24 us, 0.85 of the copy rate) or, under 10 us, a trip to memory and the steps of a tile one after another (1 row
+// 134 MB: 24.2 us, 0.85 of the copy rate) or, under 10 us, a trip to memory and the steps of a tile one after another (1 row
 // 2048 -> 8192 gated, 33.6 MB: 7.8 us); the pair kernel the tensor pipe (4096 rows 4096 -> 16384 gated: 316 us in a burst, 0.78 of
 // the measured rate of its instructions, 366 where a long run meets the power limit), and the requantisation where K is short
-// (6000 rows 2048 -> 8192 with a residual: 73 us in a burst, 89 in a long run, 45 for the products alone).
+// (6000 rows 2048 -> 8192 with a residual: 73 us in a burst, 88 in a long run, 45 for the products alone).
 //
 // Reproduces dense -> [chain] -> cvm_lut -> broadcast_mul -> [chain] of the reference's operators
 // (src/runtime/cpu/ops/ops.cc:34-75, :947-956, cpu/ops/broadcast.cc:33-36) bit for bit.

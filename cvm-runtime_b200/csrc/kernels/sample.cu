@@ -6,9 +6,12 @@
 // d = max - x < D and the first `ties` ones, in index order, with d = D: the filters only look for that cut, and neither sort
 // nor list the row.
 //   top_k   In a CTA, the n-th largest of the maxima of its threads is a lower bound of its n-th largest element (that many
-//           threads have one as large).  So the row's k-th is not below the least of the CTAs' bounds for n = k / CTAs.  The
-//           elements that are not below it are few more than k; they are put on a list, and one CTA does all the rest on it:
-//           a thread holds an element and compares it with every other one, for its rank and the weight in front of it.
+//           threads have one as large); it is bisected to a thousandth of the range of the CTA's scores, downwards.  So the
+//           row's k-th is not below the least of the CTAs' bounds for n = k / CTAs.  The elements that are not below it are
+//           mostly few more than k; they are put on a list, and one CTA does all the rest on it: a thread holds an element and
+//           compares it with every other one, for its rank and the weight in front of it.  Where the list has no room (k beyond
+//           it, hundreds of equal scores, or a score far below the others, which makes the range wide: one masked to the type's
+//           lowest value) the cut is one by count: 32 rows of 131072, top_k 50, 17 us, with 2000 of each masked 76.
 //   top_p   An element's weight is a function of its table index, so the elements of every index are counted; the running
 //           sum of count * weight gives the index in which the share is reached and how many of its elements are needed, and
 //           the cut among those is one by count again.
@@ -19,7 +22,7 @@
 // Counts and weights are whole numbers, so their order of summation changes nothing.
 //
 // What bounds it: few rows, the chain of passes and barriers, each a trip to L2 or over a cluster (1 row of 32000 elements, all
-// filters: 9.6 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 26 us, 2.6).  Many rows, the passes themselves: 256 rows
+// filters: 9.8 us, of which reading its 128 KB is 0.02; 32 rows of 131072: 23 to 26 us, 2.6).  Many rows, the passes themselves: 256 rows
 // of 262144 elements take 107 us without cuts (read twice: once from memory, 41 us at the rate of a copy, once from L2), 124 with
 // top_k, 251 with top_p, whose counting is an atomic in shared memory for every element above the table's last entry.  More loads
 // under way (the next four requested while four are worked on) spill at the 64 registers that two CTAs an SM leave: 190 against
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
       }
       return;
     }
-    cut = cut_by_count<RESIDENT>(r, s, (uint64_t)k, 0, (uint64_t)r.dist(lo) + 1);   // (hundreds of equal scores, or a large k)
+    cut = cut_by_count<RESIDENT>(r, s, (uint64_t)k, 0, (uint64_t)r.dist(lo) + 1);   // (the list had no room)
   }
   if (top_p < ONE) {
     if (r.wide) {
